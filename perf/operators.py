@@ -1,0 +1,486 @@
+"""The operators of the 8-bit (E4M3) KV cache: what is measured of them.
+
+Three operators, next to each other as a decode or prefill step uses them:
+
+  write    rows of keys and values go into the paged cache, optionally with the
+           per-head RMS norm of queries and keys and always with the NEOX
+           rotation in the same pass; each (16-token page, KV head) block of K
+           and of V is held as E4M3 codes times one power of two.  The touched
+           pages are read back as F16.
+  decode   attention of one new token per slot over its cached rows (with the
+           new row's write in the same call where `step` is true).
+  window   attention of several new tokens per slot, token i over the rows up
+           to its own position.
+
+A case is {"op", "heads" (KV heads; 4 query heads each), "slots", "lo", "hi"
+(rows cached before the call), "new_lo", "new_hi" (new tokens per slot),
+"dtype", "norm", "step", "mix" (which lengths between lo and hi)}.
+
+`own` false: elementary torch operations in F32.  `own` true: the calls of the
+framework.  Both start from the same rows, quantised by the same definition.
+"""
+import math
+import os
+import random
+import sys
+
+import numpy as np
+import torch
+
+own = False
+
+D = 128          # dims of a head
+GROUP = 4        # query heads of a KV head
+PAGE = 16        # tokens of a page: one scale for each page, KV head, K or V
+EXP_MIN = -100   # the scale exponent of an all-zero block
+EPS = 1e-6
+DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def listed():
+    return [
+        # one request, one token: the write of a batch-1 decode step (launch latency)
+        {"name": "write_one", "op": "write", "heads": 8, "slots": 1, "lo": 1024, "hi": 1024, "new_lo": 1, "new_hi": 1,
+         "dtype": "f32", "norm": False, "mix": 1},
+        # one token for each of 32 live requests
+        {"name": "write_batch", "op": "write", "heads": 8, "slots": 32, "lo": 2048, "hi": 16384, "new_lo": 1, "new_hi": 1,
+         "dtype": "f32", "norm": False, "mix": 2},
+        # a prompt's rows into an empty slot
+        {"name": "write_prompt", "op": "write", "heads": 8, "slots": 1, "lo": 0, "hi": 0, "new_lo": 1500, "new_hi": 1500,
+         "dtype": "f32", "norm": False, "mix": 3},
+        # one token for each of 16 requests from a packed bf16 projection, norms of q and k included
+        {"name": "norm_write_step", "op": "write", "heads": 8, "slots": 16, "lo": 256, "hi": 4096, "new_lo": 1, "new_hi": 1,
+         "dtype": "bf16", "norm": True, "mix": 4},
+        # ragged prompts behind shared prefixes of odd lengths, packed bf16 projections
+        {"name": "norm_write_prompts", "op": "write", "heads": 8, "slots": 12, "lo": 0, "hi": 770, "new_lo": 1, "new_hi": 1930,
+         "dtype": "bf16", "norm": True, "mix": 5},
+        # batch-1 decode behind a prefix of 1024 positions
+        {"name": "decode_one", "op": "decode", "heads": 8, "slots": 1, "lo": 1024, "hi": 1024, "step": True, "mix": 6},
+        # 16 requests with contexts of 256 to 4096 positions
+        {"name": "decode_batch", "op": "decode", "heads": 8, "slots": 16, "lo": 256, "hi": 4096, "step": True, "mix": 7},
+        # one GPU's 32 requests of the scale-out workload
+        {"name": "decode_shard", "op": "decode", "heads": 8, "slots": 32, "lo": 2048, "hi": 16384, "step": True, "mix": 8},
+        # one request near the context's end
+        {"name": "decode_long", "op": "decode", "heads": 8, "slots": 1, "lo": 32700, "hi": 32700, "step": False, "mix": 9},
+        # a refreshed window behind a reference prompt, F32 as the backbone's activations
+        {"name": "window_refresh", "op": "window", "heads": 8, "slots": 1, "lo": 770, "hi": 770, "new_lo": 37, "new_hi": 37,
+         "dtype": "f32", "mix": 10},
+        # a long prompt at once
+        {"name": "window_prompt", "op": "window", "heads": 8, "slots": 1, "lo": 0, "hi": 0, "new_lo": 8100, "new_hi": 8100,
+         "dtype": "bf16", "mix": 11},
+        # ragged prompts behind contexts of several requests
+        {"name": "window_ragged", "op": "window", "heads": 8, "slots": 8, "lo": 0, "hi": 4000, "new_lo": 1, "new_hi": 1024,
+         "dtype": "f32", "mix": 12},
+    ]
+
+
+def draw(rng):
+    def logint(lo, hi):
+        return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+    op = rng.choice(["write", "decode", "window"])
+    heads = rng.choice([1, 2, 4, 8])
+    case = {"op": op, "heads": heads, "mix": rng.randrange(1 << 30)}
+    if op == "decode":
+        slots = logint(1, 32)
+        hi = logint(1, 16000 if slots > 1 else 32000)
+        return {**case, "slots": slots, "lo": rng.randint(0, hi), "hi": hi, "step": rng.random() < 0.5}
+    slots = logint(1, 12)
+    hi = rng.choice([0, logint(1, 1000), logint(1, 4000)])
+    new_hi = logint(1, max(1, (9000 if op == "write" else 5000) // slots))
+    case = {**case, "slots": slots, "lo": rng.randint(0, hi), "hi": hi, "new_lo": rng.randint(1, new_hi), "new_hi": new_hi,
+            "dtype": rng.choice(["f32", "f16", "bf16"])}
+    if op == "write":
+        case["norm"] = rng.random() < 0.5
+    return case
+
+
+def lengths(case):
+    """Rows cached before the call and new tokens, for each slot."""
+    r = random.Random(case["mix"])
+    n = case["slots"]
+    old = [r.randint(case["lo"], case["hi"]) for _ in range(n)]
+    new = [r.randint(case.get("new_lo", 1), case.get("new_hi", 1)) for _ in range(n)]
+    if n > 1:
+        old[0], new[-1] = case["hi"], case.get("new_hi", 1)
+    return old, new
+
+
+# ------------------------------------------------------------------ the inputs
+def rows(gen, n, heads, gain):
+    """n rows [n, heads, D] in F32: normal values times a gain for each dim and a gain for each token."""
+    x = torch.randn((n, heads, D), generator=gen, device="cuda")
+    t = torch.randn((n, 1, 1), generator=gen, device="cuda").mul_(0.3).exp_()
+    return x.mul_(gain).mul_(t)
+
+
+def rotation(n):
+    """cos and sin of the NEOX rotation for positions [0, n): angles in F32, values rounded to bf16."""
+    inv = torch.tensor([1.0 / np.float32(1e6 ** (2 * i / D)) for i in range(D // 2)], dtype=torch.float32, device="cuda")
+    a = (torch.arange(n, device="cuda", dtype=torch.float32)[:, None] * inv).double()
+    return a.cos().float().bfloat16().float(), a.sin().float().bfloat16().float()
+
+
+def prepare(case, seed):
+    heads, n = case["heads"], case["slots"]
+    old, new = lengths(case)
+    gen = torch.Generator(device="cuda").manual_seed(1000003 * int(seed) + 17)
+    gain = torch.randn((heads, D), generator=gen, device="cuda").mul_(0.4).exp_()
+    total = sum(new)
+    dt = DTYPES[case.get("dtype", "f32")]
+    s = {"case": case, "old": old, "new": new}
+    s["norm"] = bool(case.get("norm"))
+    qn, kn = (torch.rand((2, D), generator=gen, device="cuda") + 0.5).unbind(0)
+    s["q_norm"], s["k_norm"] = qn.contiguous(), kn.contiguous()
+    if case["op"] == "write":
+        if s["norm"]:  # q, k and v side by side, as one projection gives them
+            x = torch.randn((total, (GROUP + 2) * heads, D), generator=gen, device="cuda")
+            x[:, GROUP * heads:(GROUP + 1) * heads] *= gain
+            s["qkv"] = x.to(dt)
+            s["q_out"] = torch.empty((total, GROUP * heads, D), dtype=dt, device="cuda")
+        else:
+            s["k"] = rows(gen, total, heads, gain).to(dt)
+            s["v"] = rows(gen, total, heads, 1.0).to(dt)
+        first = [p // PAGE * PAGE for p in old]
+        s["first"], s["back"] = first, [p + t - f for p, t, f in zip(old, new, first)]
+        m = sum(s["back"])
+        s["k_out"], s["v_out"] = torch.empty((2, m, heads, D), dtype=torch.float16, device="cuda").unbind(0)
+    else:
+        s["q"] = torch.randn((total, GROUP * heads, D), generator=gen, device="cuda").to(dt)
+        s["k"] = rows(gen, total, heads, gain)
+        s["v"] = rows(gen, total, heads, 1.0)
+        s["out"] = torch.empty((total, GROUP * heads * D), dtype=dt, device="cuda")
+    most = max(p + t for p, t in zip(old, new))
+    if own:
+        sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "higgs-audio.cpp_b200"))
+        import hkv
+        pages = sum((p + t + PAGE - 1) // PAGE for p, t in zip(old, new))
+        eng = hkv.Engine(n_layers=1, n_head=GROUP * heads, n_head_kv=heads, n_pages=pages, max_slots=n,
+                         context_length=most, device=0, shuffle_seed=11, cache="e4m3")
+        s["eng"], s["slots"] = eng, [eng.acquire(p + t) for p, t in zip(old, new)]
+        s["dtype"] = {"f32": hkv.F32, "f16": hkv.F16, "bf16": hkv.BF16}[case.get("dtype", "f32")]
+    else:
+        s["cos"], s["sin"] = rotation(most)
+        cap = (most + PAGE - 1) // PAGE * PAGE
+        s["kc"], s["vc"] = torch.zeros((2, n, cap, heads, D), dtype=torch.float8_e4m3fn, device="cuda").unbind(0)
+        s["ke"], s["ve"] = torch.full((2, n, cap // PAGE, heads), EXP_MIN, dtype=torch.int32, device="cuda").unbind(0)
+        s["at"] = torch.tensor(old, device="cuda")
+        s["count"] = torch.tensor(new, device="cuda")
+        slot = torch.repeat_interleave(torch.arange(n, device="cuda"), s["count"])
+        start = torch.cumsum(s["count"], 0) - s["count"]
+        s["slot"], s["pos"] = slot, torch.arange(total, device="cuda") - start[slot] + s["at"][slot]
+    # the rows cached before the call, and for attention without a write in it the new ones as well
+    behind = case["op"] == "window" or (case["op"] == "decode" and not case["step"])
+    at = 0
+    for e, (p, t) in enumerate(zip(old, new)):
+        k, v = rows(gen, p, heads, gain), rows(gen, p, heads, 1.0)
+        if own:
+            if p:
+                eng.rope_append_range(0, s["slots"][e], p, k, v)
+                eng.advance([s["slots"][e]], p)
+            if behind:
+                eng.rope_append_range(0, s["slots"][e], t, s["k"][at:at + t], s["v"][at:at + t])
+        else:
+            for x, c, x_e in ((rotate(k, s["cos"][:p, None], s["sin"][:p, None]), s["kc"], s["ke"]), (v, s["vc"], s["ve"])):
+                full = (p + PAGE - 1) // PAGE * PAGE
+                block = torch.zeros((full, heads, D), device="cuda")
+                block[:p] = x
+                block = block.view(-1, PAGE, heads, D)
+                exp = block_exponent(block.abs().amax((1, 3)))
+                c[e, :full] = codes(block, exp[:, None, :, None]).view(full, heads, D)
+                x_e[e, :full // PAGE] = exp
+        at += t
+    if behind and not own:
+        write_rows(s, rotate(s["k"], s["cos"][s["pos"]][:, None], s["sin"][s["pos"]][:, None]), s["v"])
+    return s
+
+
+# ------------------------------------------------------------- the plain forms
+def rotate(x, c, s):
+    """NEOX rotation of rows x [..., D]: halves (a, b) -> (a c - b s, a s + b c), every product and sum rounded."""
+    a, b = x[..., :D // 2], x[..., D // 2:]
+    return torch.cat([a * c - b * s, a * s + b * c], -1)
+
+
+def block_exponent(amax):
+    """The least exponent e with amax <= 448 * 2^e, at least EXP_MIN."""
+    m, e = torch.frexp(amax)  # amax = m 2^e with m in [0.5, 1); 448 = 0.875 * 2^9
+    return torch.where(amax > 0, torch.clamp(e - 9 + (m > 0.875).int(), min=EXP_MIN), EXP_MIN).int()
+
+
+def pow2(e):
+    """2^e in F32, e in [-126, 127], from its bits."""
+    return ((e.int() + 127) << 23).view(torch.float32)
+
+
+def codes(x, exp):
+    """x / 2^exp rounded to E4M3 (nearest, ties to even): 4 significant bits, steps of 2^-9 at least."""
+    y = x * pow2(-exp)
+    step = torch.clamp(torch.frexp(y)[1] - 4, min=-9)
+    return (torch.round(y * pow2(-step)) * pow2(step)).to(torch.float8_e4m3fn)
+
+
+def write_rows(s, k, v):
+    """The rows k, v [total, heads, D] into the cache at (slot, pos).  A page's block takes the larger of its
+    exponent and what the new rows need; rows that were there are rounded again where it grows.  A page whose
+    first row is written starts anew."""
+    n, cap, heads, _ = s["kc"].shape
+    slot, pos = s["slot"], s["pos"]
+    index = slot * (cap // PAGE) + pos // PAGE
+    fresh = torch.zeros(n * (cap // PAGE), dtype=torch.bool, device="cuda")
+    fresh.index_fill_(0, index[pos % PAGE == 0], True)
+    # the first page of each slot that the call touches may hold earlier rows
+    page0 = torch.arange(n, device="cuda") * (cap // PAGE) + s["at"] // PAGE
+    for x, c, x_e in ((k, s["kc"], s["ke"]), (v, s["vc"], s["ve"])):
+        amax = torch.zeros((n * (cap // PAGE), heads), device="cuda")
+        amax.scatter_reduce_(0, index[:, None].expand(-1, heads), x.abs().amax(-1), "amax")
+        need = block_exponent(amax)
+        flat_e = x_e.view(-1, heads)
+        touched = torch.zeros_like(fresh)
+        touched.index_fill_(0, index, True)
+        exp = torch.where(fresh[:, None], need, torch.maximum(flat_e, need))
+        exp = torch.where(touched[:, None], exp, flat_e)
+        blocks = c.view(-1, PAGE, heads, D)
+        was = blocks[page0].float() * pow2(flat_e[page0])[:, None, :, None]
+        blocks[page0] = codes(was, exp[page0][:, None, :, None])
+        c.view(-1, heads, D)[slot * cap + pos] = codes(x, exp[index][..., None])
+        flat_e.copy_(exp)
+
+
+def values(c, x_e):
+    """The values that codes [n, cap, heads, D] and exponents [n, cap / PAGE, heads] stand for."""
+    n, cap, heads, _ = c.shape
+    return (c.view(n, -1, PAGE, heads, D).float() * pow2(x_e)[:, :, None, :, None]).view(n, cap, heads, D)
+
+
+def rms_norm(x, w):
+    return x * torch.rsqrt((x * x).mean(-1, keepdim=True) + EPS) * w
+
+
+def plain_write(s):
+    heads = s["case"]["heads"]
+    c, sn = s["cos"][s["pos"]][:, None], s["sin"][s["pos"]][:, None]
+    out = {}
+    if s["norm"]:
+        x = s["qkv"].float()
+        q, k, v = x[:, :GROUP * heads], x[:, GROUP * heads:(GROUP + 1) * heads], x[:, (GROUP + 1) * heads:]
+        out["q"] = rotate(rms_norm(q, s["q_norm"]), c, sn).to(s["qkv"].dtype)
+        k = rms_norm(k, s["k_norm"])
+    else:
+        k, v = s["k"].float(), s["v"].float()
+    write_rows(s, rotate(k, c, sn), v)
+    n, cap = s["kc"].shape[:2]
+    spread = torch.arange(cap, device="cuda")
+    first = s["at"] // PAGE * PAGE
+    take = (spread[None] >= first[:, None]) & (spread[None] < (s["at"] + s["count"])[:, None])
+    index = take.view(-1).nonzero().view(-1)
+    blocks = index // PAGE
+    for name, c8, x_e in (("k", s["kc"], s["ke"]), ("v", s["vc"], s["ve"])):
+        x = c8.view(-1, heads, D)[index].float()
+        out[name] = (x * pow2(x_e.view(-1, heads)[blocks])[..., None]).half()
+    return out
+
+
+def plain_attention(s, q):
+    """Rows q [total, 4 heads, D], already rotated, over the cached rows up to each row's own position."""
+    n, cap, heads, _ = s["kc"].shape
+    most = max(s["new"])
+    slot, pos = s["slot"], s["pos"]
+    i = pos - s["at"][slot]
+    x = torch.zeros((n, heads, GROUP, most, D), device="cuda")
+    x[slot, :, :, i] = q.view(-1, heads, GROUP, D)
+    k = values(s["kc"], s["ke"]).permute(0, 2, 1, 3)
+    score = x.view(n, heads, GROUP * most, D) @ k.transpose(-1, -2)
+    del k
+    score = score.view(n, heads, GROUP, most, cap).mul_(1 / math.sqrt(D))
+    spread = torch.arange(cap, device="cuda")
+    limit = s["at"][:, None] + torch.arange(most, device="cuda")
+    seen = spread <= limit[..., None]  # [n, most, cap]
+    score.masked_fill_(~seen[:, None, None], -math.inf)
+    score.sub_(score.amax(-1, keepdim=True)).exp_()
+    total = score.sum(-1, keepdim=True)
+    v = values(s["vc"], s["ve"]).permute(0, 2, 1, 3)
+    o = (score.view(n, heads, GROUP * most, cap) @ v).view(n, heads, GROUP, most, D) / total
+    return o[slot, :, :, i].reshape(len(slot), -1)
+
+
+def plain_decode(s):
+    c, sn = s["cos"][s["pos"]][:, None], s["sin"][s["pos"]][:, None]
+    if s["case"]["step"]:
+        write_rows(s, rotate(s["k"], c, sn), s["v"])
+    return plain_attention(s, rotate(s["q"].float(), c, sn))
+
+
+# -------------------------------------------------------------------- one pass
+def own_write(s):
+    eng, slots, case = s["eng"], s["slots"], s["case"]
+    heads = case["heads"]
+    out = {}
+    if s["norm"]:
+        row = (GROUP + 2) * heads * D
+        eng.qkv_write(0, slots, s["new"], s["qkv"], s["qkv"][:, GROUP * heads:], s["qkv"][:, (GROUP + 1) * heads:],
+                      q_norm=s["q_norm"], k_norm=s["k_norm"], eps=EPS, q_out=s["q_out"], dtype=s["dtype"],
+                      q_stride=row, k_stride=row, v_stride=row)
+        out["q"] = s["q_out"]
+    elif case["dtype"] != "f32" or (max(s["new"]) > 1 and len(slots) > 1):
+        eng.qkv_write(0, slots, s["new"], None, s["k"], s["v"], dtype=s["dtype"])
+    elif len(slots) == 1:
+        eng.rope_append_range(0, slots[0], s["new"][0], s["k"], s["v"])
+    else:
+        eng.rope_append(0, slots, s["k"], s["v"])
+    eng.cache_read(0, slots, s["first"], s["back"], s["k_out"], s["v_out"])
+    out["k"], out["v"] = s["k_out"], s["v_out"]
+    return out
+
+
+def run(s):
+    op = s["case"]["op"]
+    if own:
+        if op == "write":
+            return own_write(s)
+        if op == "window":
+            s["eng"].window_attn(0, s["slots"], s["new"], s["q"], s["out"], dtype=s["dtype"])
+        elif s["case"]["step"]:
+            s["eng"].decode_step(0, s["slots"], s["q"], s["k"], s["v"], s["out"])
+        else:
+            s["eng"].decode_attn(0, s["slots"], s["q"], s["out"])
+        return s["out"]
+    if op == "write":
+        return plain_write(s)
+    if op == "decode":
+        return plain_decode(s)
+    return plain_attention(s, s["q"].float()).to(s["out"].dtype)
+
+
+def work(case):
+    heads = case["heads"]
+    old, new = lengths(case)
+    size = 4 if case.get("dtype", "f32") == "f32" else 2
+    total = sum(new)
+    if case["op"] == "write":
+        back = sum(p + t - p // PAGE * PAGE for p, t in zip(old, new))
+        row = 2 * heads * D
+        q = 2 * size * GROUP * heads * D * total if case["norm"] else 0
+        flops = (2 * (GROUP + 2) if case["norm"] else 4) * 3 * heads * D * total
+        return {"bytes": total * row * (size + 1) + back * row * (1 + 2) + q, "flops": flops}
+    held = sum(p + t for p, t in zip(old, new))
+    pairs = sum(t * p + t * (t + 1) // 2 for p, t in zip(old, new))
+    io = total * GROUP * heads * D * 2 * size
+    if case.get("step"):
+        io += total * 2 * heads * D * 4
+    return {"bytes": held * 2 * heads * D + (held // PAGE + len(old)) * 2 * heads * 4 + io,
+            "flops": 4 * pairs * GROUP * heads * D}
+
+
+# ---------------------------------------------------------- the definition in 64 bits
+def _grid():
+    """The 127 non-negative E4M3 values, in order."""
+    return torch.tensor([m / 8 * 2.0 ** -6 for m in range(8)] +
+                        [(1 + m / 8) * 2.0 ** (e - 7) for e in range(1, 16) for m in range(8) if (e, m) != (15, 7)],
+                        dtype=torch.float64, device="cuda")
+
+
+def _nearest(y, grid):
+    """The grid's value nearest to each y, ties to the even code."""
+    a = y.abs().contiguous()
+    hi = torch.searchsorted(grid, a).clamp_(max=126)
+    lo = (hi - 1).clamp_(min=0)
+    up, down = grid[hi] - a, a - grid[lo]
+    pick = torch.where(up < down, hi, torch.where(up > down, lo, torch.where(hi % 2 == 0, hi, lo)))
+    return torch.copysign(grid[pick], y)
+
+
+def _scale(amax):
+    """2^e, the least power with amax <= 448 * 2^e, in float64; amax [...] on the GPU."""
+    e = torch.ceil(torch.log2(torch.clamp(amax, min=1e-300) / 448))
+    e = torch.where(448 * torch.exp2(e - 1) >= amax, e - 1, e)
+    e = torch.where(448 * torch.exp2(e) < amax, e + 1, e)
+    return torch.exp2(torch.clamp(e, min=EXP_MIN))
+
+
+def _turn(x, pos, f32_rows):
+    """Row x [n, heads, D] float64 rotated at positions pos: the rotation's values are bf16; rows of the cache are
+    rounded to F32 after each product and sum, as its contents are defined."""
+    freq = np.array([np.float32(1) / np.float32(1e6 ** (j / (D // 2))) for j in range(D // 2)], np.float32)
+    ang = (pos.cpu().numpy().astype(np.float32)[:, None] * freq).astype(np.float64)
+    c, s = (torch.from_numpy(f(ang).astype(np.float32)).bfloat16().double().cuda()[:, None] for f in (np.cos, np.sin))
+    a, b = x.chunk(2, -1)
+    r = (lambda t: t.float().double()) if f32_rows else (lambda t: t)
+    return torch.cat([r(r(a * c) - r(b * s)), r(r(a * s) + r(b * c))], -1)
+
+
+def _cache(x, upto, grid, start=0, held=None, scale=None):
+    """Values of a block-scaled cache of rows x [L, heads, D] float64, written in one go at row `start` of its first
+    page; held [start, heads, D] and scale [heads] are that page's rows and scale before."""
+    full = -(-(start + upto) // PAGE) * PAGE
+    if not full:
+        return x, None
+    out = torch.zeros((full, x.shape[1], D), dtype=torch.float64, device="cuda")
+    out[start:start + upto] = x
+    blocks = out.view(-1, PAGE, x.shape[1], D)
+    sc = _scale(blocks.abs().amax((1, 3)))
+    if start:
+        sc[0] = torch.maximum(sc[0], scale)
+        out[:start] = held
+    got = _nearest(blocks / sc[:, None, :, None], grid) * sc[:, None, :, None]
+    return got.view(full, -1, D)[:start + upto], sc
+
+
+def exact(case, seed):
+    if case["op"] == "window" and work(case)["flops"] > 3e12:
+        return None
+    global own
+    was, own = own, False
+    try:
+        old, new = lengths(case)
+        heads, n = case["heads"], case["slots"]
+        gen = torch.Generator(device="cuda").manual_seed(1000003 * int(seed) + 17)
+        gain = torch.randn((heads, D), generator=gen, device="cuda").mul_(0.4).exp_()
+        total, dt = sum(new), DTYPES[case.get("dtype", "f32")]
+        qn, kn = (torch.rand((2, D), generator=gen, device="cuda") + 0.5).double().unbind(0)
+        q = None
+        if case["op"] == "write" and case["norm"]:
+            x = torch.randn((total, (GROUP + 2) * heads, D), generator=gen, device="cuda")
+            x[:, GROUP * heads:(GROUP + 1) * heads] *= gain
+            x = x.to(dt).double()
+            q, k, v = x.split([GROUP * heads, heads, heads], 1)
+            q, k = (y / (y.pow(2).mean(-1, keepdim=True) + EPS).sqrt() * w for y, w in ((q, qn), (k, kn)))
+        elif case["op"] == "write":
+            k, v = rows(gen, total, heads, gain).to(dt).double(), rows(gen, total, heads, 1.0).to(dt).double()
+        else:
+            q = torch.randn((total, GROUP * heads, D), generator=gen, device="cuda").to(dt).double()
+            k, v = rows(gen, total, heads, gain).double(), rows(gen, total, heads, 1.0).double()
+        grid = _grid()
+        at, outs_k, outs_v, outs = 0, [], [], []
+        for p, t in zip(old, new):
+            pos = torch.arange(p, p + t)
+            first, r = p // PAGE * PAGE, p % PAGE
+            hk, hv = rows(gen, p, heads, gain).double(), rows(gen, p, heads, 1.0).double()
+            k0, ks = _cache(_turn(hk, torch.arange(p), True), p, grid)
+            v0, vs = _cache(hv, p, grid)
+            tail = (k0[first:], ks[-1] if r else None, v0[first:], vs[-1] if r else None)
+            k1, _ = _cache(_turn(k[at:at + t], pos, not case.get("norm")), t, grid, r, tail[0], tail[1])
+            v1, _ = _cache(v[at:at + t], t, grid, r, tail[2], tail[3])
+            if case["op"] == "write":
+                outs_k.append(k1)
+                outs_v.append(v1)
+                if q is not None:
+                    outs.append(_turn(q[at:at + t], pos, False))
+            else:
+                kk, vv = torch.cat([k0[:first], k1]), torch.cat([v0[:first], v1])
+                qq = q[at:at + t]
+                if case["op"] == "decode":
+                    qq = _turn(qq, pos, False)
+                o = torch.empty_like(qq)
+                late = torch.arange(p + t, device="cuda")[None] > pos.cuda()[:, None]
+                for h in range(GROUP * heads):
+                    a = qq[:, h] @ kk[:, h // GROUP].T / D ** 0.5
+                    o[:, h] = torch.softmax(a.masked_fill_(late, -math.inf), -1) @ vv[:, h // GROUP]
+                outs.append(o.reshape(t, -1))
+            at += t
+        if case["op"] == "write":
+            got = {"k": torch.cat(outs_k), "v": torch.cat(outs_v)}
+            return {**got, "q": torch.cat(outs)} if q is not None else got
+        return torch.cat(outs)
+    finally:
+        own = was
