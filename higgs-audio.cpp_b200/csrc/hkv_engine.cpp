@@ -238,6 +238,21 @@ struct BatchCache {
     cudaStream_t consumer_stream = nullptr;
 };
 
+// Descriptor of a call over rows of several slots (hkv_qkv_write,
+// hkv_cache_read): one RowItem per touched page, kept until the rows change, so
+// the calls of a step's layers reuse one upload.
+struct RowCache {
+    bool valid = false;
+    uint64_t epoch = 0;
+    std::vector<int32_t> slots;
+    std::vector<int64_t> begin;
+    std::vector<int64_t> count;
+    const RowItem *items = nullptr;
+    int32_t n_items = 0;
+    bool consumed = false;
+    cudaStream_t consumer_stream = nullptr;
+};
+
 struct ProfileRecord {
     cudaEvent_t start;
     cudaEvent_t stop;
@@ -251,6 +266,7 @@ struct hkv_engine {
     mutable std::mutex mu;
     mutable std::string last_error;
     bool device_mode = false;
+    int32_t cache_type = HKV_CACHE_F16;
 
     // host bookkeeping
     std::vector<int32_t> refcnt;
@@ -277,7 +293,8 @@ struct hkv_engine {
     int64_t part_cap = 0;
     int num_sms = 0;
     float scale_log2 = 0.f;
-    hkv::Staging batch_stage, range_stage, gather_stage, cow_stage;
+    hkv::Staging batch_stage, range_stage, gather_stage, cow_stage, write_stage, read_stage;
+    hkv::RowCache write_rows, read_rows;
     // Copy-on-write copies decided on the host and not yet enqueued:
     // {source page, destination page} pairs, flushed as one kernel launch.
     std::vector<int32_t> cow_pending;
@@ -381,16 +398,6 @@ int32_t take_page(hkv_engine *eng, Slot &slot) {
     eng->free_pages.pop_back();
     eng->refcnt[page] = 1;
     return page;
-}
-
-// Bytes of one page within one layer's slab (K and V of every KV head).
-int64_t layer_page_bytes(const hkv_engine *eng) {
-    return 2ll * eng->cfg.n_head_kv * kHeadBlockBytes;
-}
-
-uint8_t *page_ptr(const hkv_engine *eng, int32_t layer, int32_t page) {
-    return eng->pool +
-           (static_cast<int64_t>(layer) * eng->cfg.n_pages + page) * layer_page_bytes(eng);
 }
 
 // Pages `slot` must newly take to own every page touched by rows
@@ -507,6 +514,7 @@ PoolView pool_view(const hkv_engine *eng) {
     v.n_pages = eng->cfg.n_pages;
     v.n_layers = eng->cfg.n_layers;
     v.n_head_kv = eng->cfg.n_head_kv;
+    v.format = eng->cache_type;
     return v;
 }
 
@@ -661,7 +669,7 @@ int ensure_batch(hkv_engine *eng, int32_t n, const int32_t *slots, cudaStream_t 
     if (n == 1) {
         int32_t fit[5] = {0, 0, 0, 0, 0};
         for (int i = 1; i < 5; ++i) {
-            fit[i] = attention_cluster_fit(1 << i);
+            fit[i] = attention_cluster_fit(1 << i, eng->cache_type);
         }
         C = plan_cluster(n, G, total_pages, max_warps, fit);
     }
@@ -702,6 +710,145 @@ int launch_status(hkv_engine *eng, const char *what) {
     return HKV_OK;
 }
 
+// Arguments of a write of K and V rows alone.
+WriteArgs kv_write_args(const RowItem *items, int32_t n_items, int32_t layer, int32_t dtype, const void *k,
+                        const void *v, int64_t k_stride, int64_t v_stride, bool rope) {
+    WriteArgs a{};
+    a.items = items;
+    a.n_items = n_items;
+    a.layer = layer;
+    a.dtype = dtype;
+    a.k = k;
+    a.v = v;
+    a.k_stride = k_stride;
+    a.v_stride = v_stride;
+    a.rope = rope;
+    return a;
+}
+
+int64_t row_item_count(int64_t begin, int64_t count) {
+    return count > 0 ? (begin + count - 1) / kPageTokens - begin / kPageTokens + 1 : 0;
+}
+
+// Cuts rows [begin, begin + count) of a slot at page borders; row0 is the
+// packed row of position `begin`.
+RowItem *put_row_items(RowItem *out, const std::vector<int32_t> &pages, int64_t begin, int64_t count,
+                       int64_t row0) {
+    for (int64_t pos = begin; pos < begin + count;) {
+        const int64_t next = std::min(begin + count, (pos / kPageTokens + 1) * kPageTokens);
+        out->page = pages[static_cast<size_t>(pos / kPageTokens)];
+        out->pos0 = static_cast<int32_t>(pos);
+        out->row0 = static_cast<int32_t>(row0 + pos - begin);
+        out->count = static_cast<int32_t>(next - pos);
+        ++out;
+        pos = next;
+    }
+    return out;
+}
+
+bool row_cache_matches(const hkv_engine *eng, const RowCache &rc, int32_t n, const int32_t *slots,
+                       const int64_t *begin, const int64_t *count) {
+    if (!rc.valid || rc.epoch != eng->epoch || static_cast<int32_t>(rc.slots.size()) != n) {
+        return false;
+    }
+    for (int32_t e = 0; e < n; ++e) {
+        if (rc.slots[e] != slots[e] || !slot_ok(eng, slots[e]) || rc.begin[e] != begin[e] ||
+            rc.count[e] != count[e]) {
+            return false;
+        }
+    }
+    return true;
+}
+
+// Uploads the items of rows [begin[e], begin[e] + count[e]) of every slot.
+// The slots' page lists cover them.
+int upload_rows(hkv_engine *eng, Staging &stage, RowCache &rc, int32_t n, const int32_t *slots,
+                const int64_t *begin, const int64_t *count, cudaStream_t stream) {
+    int64_t n_items = 0;
+    for (int32_t e = 0; e < n; ++e) {
+        n_items += row_item_count(begin[e], count[e]);
+    }
+    rc.valid = false;
+    if (rc.consumed) {
+        HKV_CUDA_TRY(eng, stage.mark_used(rc.consumer_stream));
+        rc.consumed = false;
+    }
+    const size_t bytes = static_cast<size_t>(n_items) * sizeof(RowItem);
+    void *host = nullptr;
+    HKV_CUDA_TRY(eng, stage.begin(bytes, &host));
+    RowItem *out = static_cast<RowItem *>(host);
+    int64_t row0 = 0;
+    for (int32_t e = 0; e < n; ++e) {
+        out = put_row_items(out, eng->slots[slots[e]].pages, begin[e], count[e], row0);
+        row0 += count[e];
+    }
+    void *dev = nullptr;
+    ++eng->enqueue_seq;
+    HKV_CUDA_TRY(eng, stage.commit(bytes, stream, &dev));
+    rc.items = static_cast<const RowItem *>(dev);
+    rc.n_items = static_cast<int32_t>(n_items);
+    rc.slots.assign(slots, slots + n);
+    rc.begin.assign(begin, begin + n);
+    rc.count.assign(count, count + n);
+    rc.epoch = eng->epoch;
+    rc.valid = true;
+    return HKV_OK;
+}
+
+// Calls whose descriptor lives in the engine's staging buffers cannot be
+// captured: a replay would read the buffer after a later call rewrote it.
+int refuse_capture(hkv_engine *eng, cudaStream_t stream) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    HKV_CUDA_TRY(eng, cudaStreamIsCapturing(stream, &status));
+    if (status != cudaStreamCaptureStatusNone) {
+        return fail(eng, HKV_ERR_INVALID, "the call cannot be captured into a CUDA graph");
+    }
+    return HKV_OK;
+}
+
+// The slot list of a call over rows of several slots: live, none twice, and
+// every length in [0, context].  *total: the packed rows.
+int check_row_slots(hkv_engine *eng, int32_t n, const int32_t *slots, const int64_t *count, int64_t *total) {
+    if (n <= 0 || slots == nullptr || count == nullptr) {
+        return fail(eng, HKV_ERR_INVALID, "empty slot list");
+    }
+    *total = 0;
+    for (int32_t e = 0; e < n; ++e) {
+        if (!slot_ok(eng, slots[e])) {
+            return fail(eng, HKV_ERR_BAD_SLOT, "slot %d is not live (batch entry %d)", slots[e], e);
+        }
+        for (int32_t f = 0; f < e; ++f) {
+            if (slots[f] == slots[e]) {
+                return fail(eng, HKV_ERR_INVALID, "slot %d appears twice in one batch", slots[e]);
+            }
+        }
+        if (count[e] < 0 || count[e] > eng->cfg.context_length) {
+            return fail(eng, HKV_ERR_RANGE, "%lld rows for batch entry %d", static_cast<long long>(count[e]), e);
+        }
+        *total += count[e];
+    }
+    if (*total > INT32_MAX) {
+        return fail(eng, HKV_ERR_RANGE, "%lld rows in one call", static_cast<long long>(*total));
+    }
+    return HKV_OK;
+}
+
+size_t dtype_bytes(int32_t dtype) { return dtype == HKV_F32 ? 4 : 2; }
+
+// A row stride in elements: 0 stands for packed rows; otherwise at least the
+// row, in whole 16-byte steps.
+int check_stride(hkv_engine *eng, const char *name, int64_t row, int32_t dtype, int64_t *stride) {
+    if (*stride == 0) {
+        *stride = row;
+    }
+    if (*stride < row || *stride * static_cast<int64_t>(dtype_bytes(dtype)) % 16 != 0 ||
+        *stride > (int64_t{1} << 40)) {
+        return fail(eng, HKV_ERR_INVALID, "%s: a stride of %lld elements (rows of %lld, 16-byte steps)", name,
+                    static_cast<long long>(*stride), static_cast<long long>(row));
+    }
+    return HKV_OK;
+}
+
 int do_append(hkv_engine *eng, int32_t layer, int32_t n, const int32_t *slots, const float *k,
               const float *v, bool rope, cudaStream_t stream) {
     int st = check_compute(eng, layer);
@@ -714,8 +861,14 @@ int do_append(hkv_engine *eng, int32_t layer, int32_t n, const int32_t *slots, c
     ++eng->enqueue_seq;
     {
         ProfileScope ps(eng, HKV_KERNEL_APPEND, stream);
-        launch_append(pool_view(eng), rope_view(eng), eng->batch.view, layer, k, v, rope,
-                      eng->d_err, stream);
+        if (eng->cache_type == HKV_CACHE_E4M3) {
+            const int64_t row = static_cast<int64_t>(eng->cfg.n_head_kv) * kHeadDim;
+            launch_write(pool_view(eng), rope_view(eng), eng->batch.view,
+                         kv_write_args(nullptr, n, layer, HKV_F32, k, v, row, row, rope), eng->d_err, stream);
+        } else {
+            launch_append(pool_view(eng), rope_view(eng), eng->batch.view, layer, k, v, rope, eng->d_err,
+                          stream);
+        }
         ++eng->kernel_launches;
     }
     eng->batch.consumed = true;
@@ -775,6 +928,8 @@ void free_device(hkv_engine *eng) {
     eng->batch_stage.release();
     eng->range_stage.release();
     eng->gather_stage.release();
+    eng->write_stage.release();
+    eng->read_stage.release();
     eng->cow_stage.release();
     for (auto &list : eng->prof) {
         for (auto &r : list) {
@@ -840,10 +995,17 @@ int hkv_config_default(hkv_config *cfg) {
 }
 
 int hkv_engine_create(const hkv_config *cfg, hkv_engine **out) {
+    return hkv_engine_create_cache(cfg, HKV_CACHE_F16, out);
+}
+
+int hkv_engine_create_cache(const hkv_config *cfg, int32_t cache_type, hkv_engine **out) {
     if (cfg == nullptr || out == nullptr) {
         return HKV_ERR_INVALID;
     }
     *out = nullptr;
+    if (cache_type != HKV_CACHE_F16 && (cache_type != HKV_CACHE_E4M3 || HKV_CUDA_CORES)) {
+        return HKV_ERR_INVALID;  // the CUDA-core build attends F16 caches only
+    }
     if (cfg->head_dim != kHeadDim || cfg->page_tokens != kPageTokens || cfg->n_head_kv <= 0 ||
         cfg->n_head != kGqa * cfg->n_head_kv || cfg->n_layers <= 0 || cfg->context_length <= 0 ||
         cfg->max_slots <= 0 || cfg->n_pages <= 0 || cfg->n_pages > INT32_MAX ||
@@ -855,7 +1017,8 @@ int hkv_engine_create(const hkv_config *cfg, hkv_engine **out) {
         return HKV_ERR_OOM;
     }
     eng->cfg = *cfg;
-    eng->page_bytes = static_cast<int64_t>(cfg->n_layers) * 2 * cfg->n_head_kv * kHeadBlockBytes;
+    eng->cache_type = cache_type;
+    eng->page_bytes = static_cast<int64_t>(cfg->n_layers) * cfg->n_head_kv * cache_unit_bytes(cache_type);
     eng->refcnt.assign(static_cast<size_t>(cfg->n_pages), 0);
     eng->free_pages.resize(static_cast<size_t>(cfg->n_pages));
     for (int64_t i = 0; i < cfg->n_pages; ++i) {
@@ -1200,6 +1363,14 @@ int hkv_engine_config(const hkv_engine *eng, hkv_config *out) {
     return HKV_OK;
 }
 
+int hkv_engine_cache_type(const hkv_engine *eng, int32_t *out) {
+    if (eng == nullptr || out == nullptr) {
+        return HKV_ERR_INVALID;
+    }
+    *out = eng->cache_type;
+    return HKV_OK;
+}
+
 int hkv_pool_stats_get(const hkv_engine *eng, hkv_pool_stats *out) {
     if (eng == nullptr || out == nullptr) {
         return HKV_ERR_INVALID;
@@ -1269,16 +1440,30 @@ int hkv_rope_append_range(hkv_engine *eng, int32_t layer, int32_t slot, int64_t 
     const int64_t p0 = begin / kPageTokens;
     const int64_t p1 = (end - 1) / kPageTokens + 1;
     void *host = nullptr;
-    const size_t bytes = static_cast<size_t>(p1 - p0) * sizeof(int32_t);
+    const bool e4m3 = eng->cache_type == HKV_CACHE_E4M3;
+    const size_t bytes = static_cast<size_t>(p1 - p0) * (e4m3 ? sizeof(RowItem) : sizeof(int32_t));
     HKV_CUDA_TRY(eng, eng->range_stage.begin(bytes, &host));
-    std::memcpy(host, s.pages.data() + p0, bytes);
+    if (e4m3) {
+        put_row_items(static_cast<RowItem *>(host), s.pages, begin, n_tokens, 0);
+    } else {
+        std::memcpy(host, s.pages.data() + p0, bytes);
+    }
     void *dev = nullptr;
     ++eng->enqueue_seq;
     HKV_CUDA_TRY(eng, eng->range_stage.commit(bytes, stream, &dev));
     {
         ProfileScope ps(eng, HKV_KERNEL_APPEND, stream);
-        launch_append_range(pool_view(eng), rope_view(eng), static_cast<const int32_t *>(dev),
-                            begin, n_tokens, layer, k_prerope, v, true, eng->d_err, stream);
+        if (e4m3) {
+            const int64_t row = static_cast<int64_t>(eng->cfg.n_head_kv) * kHeadDim;
+            launch_write(pool_view(eng), rope_view(eng), BatchView{},
+                         kv_write_args(static_cast<const RowItem *>(dev),
+                                       static_cast<int32_t>(row_item_count(begin, n_tokens)), layer, HKV_F32,
+                                       k_prerope, v, row, row, true),
+                         eng->d_err, stream);
+        } else {
+            launch_append_range(pool_view(eng), rope_view(eng), static_cast<const int32_t *>(dev),
+                                begin, n_tokens, layer, k_prerope, v, true, eng->d_err, stream);
+        }
         ++eng->kernel_launches;
     }
     HKV_CUDA_TRY(eng, eng->range_stage.mark_used(stream));
@@ -1345,20 +1530,174 @@ int hkv_gather(hkv_engine *eng, int32_t slot, int32_t layer, int64_t pos0, int64
                     static_cast<long long>(covered));
     }
     void *host = nullptr;
-    const size_t bytes = s.pages.size() * sizeof(int32_t);
+    const bool e4m3 = eng->cache_type == HKV_CACHE_E4M3;
+    const size_t bytes = e4m3 ? static_cast<size_t>(row_item_count(pos0, n)) * sizeof(RowItem)
+                              : s.pages.size() * sizeof(int32_t);
     HKV_CUDA_TRY(eng, eng->gather_stage.begin(bytes, &host));
-    std::memcpy(host, s.pages.data(), bytes);
+    if (e4m3) {
+        put_row_items(static_cast<RowItem *>(host), s.pages, pos0, n, 0);
+    } else {
+        std::memcpy(host, s.pages.data(), bytes);
+    }
     void *dev = nullptr;
     ++eng->enqueue_seq;
     HKV_CUDA_TRY(eng, eng->gather_stage.commit(bytes, stream, &dev));
     {
         ProfileScope ps(eng, HKV_KERNEL_GATHER, stream);
-        launch_gather(pool_view(eng), static_cast<const int32_t *>(dev), pos0, n, layer, k_out,
-                      v_out, eng->d_err, stream);
+        if (e4m3) {
+            launch_read(pool_view(eng), static_cast<const RowItem *>(dev),
+                        static_cast<int32_t>(row_item_count(pos0, n)), layer, HKV_F16, k_out, v_out, eng->d_err,
+                        stream);
+        } else {
+            launch_gather(pool_view(eng), static_cast<const int32_t *>(dev), pos0, n, layer, k_out, v_out,
+                          eng->d_err, stream);
+        }
         ++eng->kernel_launches;
     }
     HKV_CUDA_TRY(eng, eng->gather_stage.mark_used(stream));
     return launch_status(eng, "gather kernel launch");
+}
+
+int hkv_qkv_write(hkv_engine *eng, const hkv_qkv_write_args *args, hkv_stream stream_h) {
+    if (eng == nullptr) return HKV_ERR_INVALID;
+    std::lock_guard<std::mutex> lock(eng->mu);
+    if (args == nullptr) {
+        return fail(eng, HKV_ERR_INVALID, "null arguments");
+    }
+    const hkv_qkv_write_args &a = *args;
+    DeviceGuard guard(eng->cfg.device);
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_h);
+    int64_t total = 0;
+    int st = check_row_slots(eng, a.n, a.slots, a.n_tokens, &total);
+    if (st != HKV_OK) return st;
+    const int64_t G = eng->cfg.n_head_kv;
+    if (a.dtype != HKV_F32 && a.dtype != HKV_F16 && a.dtype != HKV_BF16) {
+        return fail(eng, HKV_ERR_INVALID, "dtype %d", a.dtype);
+    }
+    if (a.k == nullptr || a.v == nullptr || !aligned16(a.k) || !aligned16(a.v)) {
+        return fail(eng, HKV_ERR_INVALID, "k and v must be non-null 16-byte aligned device pointers");
+    }
+    if ((a.q == nullptr) != (a.q_out == nullptr) || !aligned16(a.q) || !aligned16(a.q_out)) {
+        return fail(eng, HKV_ERR_INVALID, "q and q_out must be both given or both null, 16-byte aligned");
+    }
+    if (!aligned16(a.q_norm) || !aligned16(a.k_norm) || (a.q_norm != nullptr && a.q == nullptr)) {
+        return fail(eng, HKV_ERR_INVALID, "norm weights must be 16-byte aligned, q_norm only with q");
+    }
+    if ((a.q_norm != nullptr || a.k_norm != nullptr) && !(a.eps >= 0.f && std::isfinite(a.eps))) {
+        return fail(eng, HKV_ERR_INVALID, "eps must be finite and not negative");
+    }
+    WriteArgs w = kv_write_args(nullptr, 0, a.layer, a.dtype, a.k, a.v, a.k_stride, a.v_stride, true);
+    w.q = a.q;
+    w.q_out = a.q_out;
+    w.q_stride = a.q_stride;
+    w.q_out_stride = a.q_out_stride;
+    w.q_norm = a.q_norm;
+    w.k_norm = a.k_norm;
+    w.eps = a.eps;
+    st = check_stride(eng, "k", G * kHeadDim, a.dtype, &w.k_stride);
+    if (st == HKV_OK) st = check_stride(eng, "v", G * kHeadDim, a.dtype, &w.v_stride);
+    if (st == HKV_OK) st = check_stride(eng, "q", kGqa * G * kHeadDim, a.dtype, &w.q_stride);
+    if (st == HKV_OK) st = check_stride(eng, "q_out", kGqa * G * kHeadDim, a.dtype, &w.q_out_stride);
+    if (st != HKV_OK) return st;
+    if (a.q == a.q_out && w.q_stride != w.q_out_stride) {
+        return fail(eng, HKV_ERR_INVALID, "q in place needs equal strides");
+    }
+    std::vector<int64_t> begin(static_cast<size_t>(a.n));
+    for (int32_t e = 0; e < a.n; ++e) {
+        begin[e] = eng->slots[a.slots[e]].used;
+        if (begin[e] + a.n_tokens[e] > eng->cfg.context_length) {
+            return fail(eng, HKV_ERR_RANGE, "slot %d: rows [%lld, %lld) outside the context of %d", a.slots[e],
+                        static_cast<long long>(begin[e]), static_cast<long long>(begin[e] + a.n_tokens[e]),
+                        eng->cfg.context_length);
+        }
+    }
+    st = check_compute(eng, a.layer);
+    if (st != HKV_OK) return st;
+    st = refuse_capture(eng, stream);
+    if (st != HKV_OK) return st;
+    if (total == 0) {
+        return HKV_OK;
+    }
+    RowCache &rc = eng->write_rows;
+    if (!row_cache_matches(eng, rc, a.n, a.slots, begin.data(), a.n_tokens)) {
+        int64_t extra = 0;
+        for (int32_t e = 0; e < a.n; ++e) {
+            const Slot &s = eng->slots[a.slots[e]];
+            extra += pages_beyond_reservation(s, pages_needed(eng, s, begin[e], begin[e] + a.n_tokens[e]));
+        }
+        if (extra > unreserved_free(eng)) {
+            return fail(eng, HKV_ERR_OOM, "rows need %lld unreserved pages, %lld free",
+                        static_cast<long long>(extra), static_cast<long long>(unreserved_free(eng)));
+        }
+        for (int32_t e = 0; e < a.n; ++e) {
+            st = own_rows(eng, eng->slots[a.slots[e]], begin[e], begin[e] + a.n_tokens[e], stream);
+            if (st != HKV_OK) return st;
+        }
+        st = flush_cow(eng, stream);
+        if (st != HKV_OK) return st;
+        st = upload_rows(eng, eng->write_stage, rc, a.n, a.slots, begin.data(), a.n_tokens, stream);
+        if (st != HKV_OK) return st;
+    }
+    ++eng->enqueue_seq;
+    w.items = rc.items;
+    w.n_items = rc.n_items;
+    {
+        ProfileScope ps(eng, HKV_KERNEL_APPEND, stream);
+        launch_write(pool_view(eng), rope_view(eng), BatchView{}, w, eng->d_err, stream);
+        ++eng->kernel_launches;
+    }
+    rc.consumed = true;
+    rc.consumer_stream = stream;
+    return launch_status(eng, "write kernel launch");
+}
+
+int hkv_cache_read(hkv_engine *eng, int32_t layer, int32_t n, const int32_t *slots, const int64_t *pos0,
+                   const int64_t *n_rows, int32_t dtype, void *k_out, void *v_out, hkv_stream stream_h) {
+    if (eng == nullptr) return HKV_ERR_INVALID;
+    std::lock_guard<std::mutex> lock(eng->mu);
+    DeviceGuard guard(eng->cfg.device);
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_h);
+    int64_t total = 0;
+    int st = check_row_slots(eng, n, slots, n_rows, &total);
+    if (st != HKV_OK) return st;
+    if (pos0 == nullptr) {
+        return fail(eng, HKV_ERR_INVALID, "null first rows");
+    }
+    if (dtype != HKV_F32 && dtype != HKV_F16) {
+        return fail(eng, HKV_ERR_INVALID, "dtype %d: rows are read as F32 or F16", dtype);
+    }
+    if (k_out == nullptr || v_out == nullptr || !aligned16(k_out) || !aligned16(v_out)) {
+        return fail(eng, HKV_ERR_INVALID, "outputs must be non-null 16-byte aligned device pointers");
+    }
+    for (int32_t e = 0; e < n; ++e) {
+        const int64_t covered = static_cast<int64_t>(eng->slots[slots[e]].pages.size()) * kPageTokens;
+        if (pos0[e] < 0 || pos0[e] > covered || pos0[e] + n_rows[e] > covered) {
+            return fail(eng, HKV_ERR_RANGE, "slot %d: rows [%lld, %lld) outside the %lld mapped", slots[e],
+                        static_cast<long long>(pos0[e]), static_cast<long long>(pos0[e] + n_rows[e]),
+                        static_cast<long long>(covered));
+        }
+    }
+    st = check_compute(eng, layer);
+    if (st != HKV_OK) return st;
+    st = refuse_capture(eng, stream);
+    if (st != HKV_OK) return st;
+    if (total == 0) {
+        return HKV_OK;
+    }
+    RowCache &rc = eng->read_rows;
+    if (!row_cache_matches(eng, rc, n, slots, pos0, n_rows)) {
+        st = upload_rows(eng, eng->read_stage, rc, n, slots, pos0, n_rows, stream);
+        if (st != HKV_OK) return st;
+    }
+    ++eng->enqueue_seq;
+    {
+        ProfileScope ps(eng, HKV_KERNEL_GATHER, stream);
+        launch_read(pool_view(eng), rc.items, rc.n_items, layer, dtype, k_out, v_out, eng->d_err, stream);
+        ++eng->kernel_launches;
+    }
+    rc.consumed = true;
+    rc.consumer_stream = stream;
+    return launch_status(eng, "cache read kernel launch");
 }
 
 int hkv_sync_check(hkv_engine *eng, hkv_stream stream) {
@@ -1403,6 +1742,9 @@ int hkv_split_export(hkv_engine *eng, int32_t world, int32_t rank, void *handle_
     }
     if (world < 1 || rank < 0 || rank >= world) {
         return fail(eng, HKV_ERR_INVALID, "rank %d outside a world of %d", rank, world);
+    }
+    if (eng->cache_type != HKV_CACHE_F16) {
+        return fail(eng, HKV_ERR_INVALID, "the KV-head split runs on F16 caches");
     }
     DeviceGuard guard(eng->cfg.device);
     free_split(eng);

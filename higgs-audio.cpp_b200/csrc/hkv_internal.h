@@ -33,6 +33,26 @@ __host__ __device__ inline int64_t head_block_index(int64_t page, int layer, int
 }
 __host__ __device__ inline int swizzled_chunk(int row, int chunk) { return chunk ^ (row & 7); }
 
+// The 8-bit cache format: a value is an E4M3 code times 2^e, one exponent e per
+// block = (page, KV head, K or V).  The unit of a (page, KV head) is contiguous,
+//   unit(page, layer, head) = (layer * n_pages + page) * n_head_kv + head, 4128 B:
+//   K codes [16 rows][128], V codes [16 rows][128], then int32 {e of K, e of V}
+// so one bulk copy brings codes and exponents together (32 B of exponents and
+// padding keep units on 32-byte sectors: 0.8% of the bytes).  Row r keeps its
+// 16-byte chunk c (16 dims) at position c ^ (r & 7).
+constexpr int kCacheF16 = 0;
+constexpr int kCacheE4m3 = 1;
+constexpr int kCodeBlockBytes = kPageTokens * kHeadDim;
+constexpr int kCodeUnitBytes = 2 * kCodeBlockBytes + 32;
+__host__ __device__ inline int64_t code_unit_index(int64_t page, int layer, int head,
+                                                  int64_t n_pages, int n_head_kv) {
+    return (static_cast<int64_t>(layer) * n_pages + page) * n_head_kv + head;
+}
+// Bytes of K and V of one page and KV head.
+__host__ __device__ inline int cache_unit_bytes(int format) {
+    return format == kCacheE4m3 ? kCodeUnitBytes : 2 * kHeadBlockBytes;
+}
+
 // Device-side error record.  Kernels never trap: a failed bounds check or an
 // expired bounded wait stores its code here (first writer wins) and the
 // kernel returns; hkv_sync_check reads it.
@@ -99,6 +119,7 @@ struct PoolView {
     int64_t n_pages;
     int32_t n_layers;
     int32_t n_head_kv;
+    int32_t format = kCacheF16;
 };
 
 // Where finished outputs go.  n_ranks == 0: the caller's `out` only.
@@ -145,6 +166,10 @@ struct RopeView {
 #endif
 constexpr int kAttnWarps = HKV_ATTN_WARPS;    // consumer warps per CTA, one CTA per SM
 constexpr int kAttnStages = HKV_ATTN_STAGES;  // TMA ring depth per warp (K+V block per stage)
+#ifndef HKV_ATTN_STAGES_E4M3
+#define HKV_ATTN_STAGES_E4M3 4
+#endif
+constexpr int kAttnStagesE4m3 = HKV_ATTN_STAGES_E4M3;  // the same for the 8-bit cache
 
 void launch_append(const PoolView &pool, const RopeView &rope, const BatchView &batch, int layer,
                    const float *k, const float *v, bool apply_rope, DeviceError *err,
@@ -177,10 +202,39 @@ void launch_cow_copy(const PoolView &pool, const int32_t *pairs, int32_t n_pairs
 void launch_gather(const PoolView &pool, const int32_t *slot_pages, int64_t pos0, int64_t n,
                    int layer, uint16_t *k_out, uint16_t *v_out, DeviceError *err,
                    cudaStream_t stream);
-size_t attention_smem_bytes(bool cta_merge, bool cluster = false);
+size_t attention_smem_bytes(bool cta_merge, bool cluster = false, bool e4m3 = false);
+
+// Rows of a call, cut at page borders: rows [row0, row0 + count) of the packed
+// tensors are positions [pos0, pos0 + count) of one page of one slot.
+struct RowItem {
+    int32_t page;
+    int32_t pos0;
+    int32_t row0;
+    int32_t count;
+};
+
+// K and V rows into the cache, and q rows normed and rotated beside them
+// (hkv_cache.cu).  dtype: the HKV_F32 / HKV_F16 / HKV_BF16 of the tensors.
+struct WriteArgs {
+    const RowItem *items;  // nullptr: one row per entry of `batch`
+    int32_t n_items;
+    int32_t layer;
+    int32_t dtype;
+    const void *q, *k, *v;  // q may be nullptr
+    void *q_out;
+    int64_t q_stride, k_stride, v_stride, q_out_stride;  // elements per row
+    const float *q_norm, *k_norm;                        // nullptr: no norm
+    float eps;
+    bool rope;
+};
+void launch_write(const PoolView &pool, const RopeView &rope, const BatchView &batch,
+                  const WriteArgs &args, DeviceError *err, cudaStream_t stream);
+// Cached rows as values, F16 or F32 (dtype): [rows][n_head_kv][128] each.
+void launch_read(const PoolView &pool, const RowItem *items, int32_t n_items, int layer, int dtype,
+                 void *k_out, void *v_out, DeviceError *err, cudaStream_t stream);
 // Clusters of csize attention CTAs (2..16, the cluster-merge variant) that
 // can be resident at once on the current device; 0 if none (cached per
 // device).
-int attention_cluster_fit(int csize);
+int attention_cluster_fit(int csize, int format = kCacheF16);
 
 }  // namespace hkv

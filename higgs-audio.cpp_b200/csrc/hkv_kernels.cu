@@ -33,6 +33,7 @@
 #include <mutex>
 
 #include "hkv_device.cuh"
+#include "hkv_e4m3.cuh"
 #include "hkv_internal.h"
 
 namespace hkv {
@@ -44,8 +45,17 @@ constexpr int kStageBytes = 2 * kHeadBlockBytes;  // K block + V block
 constexpr int kQcStride = 136;                     // halves per staged-query row (272 B)
 constexpr int kQcBytes = 8 * kQcStride * 2;        // 8 rows: 4 heads x {hi, lo}
 constexpr int kPBufBytes = 16 * 16;                // 16 tokens x 8 halves
-constexpr int kBarBytes = (kAttnStages * 8 + 15) / 16 * 16;  // one 8-byte mbarrier per stage
-constexpr int kWarpSmem = kAttnStages * kStageBytes + kQcBytes + kPBufBytes + kBarBytes;
+// A warp's shared memory in each cache format: the ring of stages (one unit = K
+// and V of a page and KV head each), the staged queries, the P tile and one
+// 8-byte mbarrier per stage.  A unit of the 8-bit format is half as large, so
+// the same shared memory holds twice the stages.
+template <bool kE4m3>
+struct Ring {
+    static constexpr int kStages = kE4m3 ? kAttnStagesE4m3 : kAttnStages;
+    static constexpr int kStage = kE4m3 ? kCodeUnitBytes : kStageBytes;
+    static constexpr int kBarBytes = (kStages * 8 + 15) / 16 * 16;
+    static constexpr int kWarpSmem = kStages * kStage + kQcBytes + kPBufBytes + kBarBytes;
+};
 // CTA-level partials: two slots per warp (the run a warp does not start, and
 // the run it starts), each o[4][128] + (m, l)[4]; then one ticket per run.
 constexpr int kCtaPartFloats = kGqa * kHeadDim + 2 * kGqa;
@@ -55,15 +65,20 @@ constexpr int kCtaSmem = kAttnWarps * 2 * kCtaPartBytes + 32;
 // in the cluster's first CTA, then the mbarrier that counts the filled slots.
 constexpr int kMaxCluster = 16;
 constexpr int kClusterSmem = kMaxCluster * kCtaPartBytes + 16;
+constexpr int kPShift = 14;  // o's weights are p 2^14 in the 8-bit format: at most 16384 in F16
 constexpr int kWhereAppend = 0;
 constexpr int kWhereAttn = 1;
 constexpr int kWhereGather = 3;
 constexpr int kWhereCow = 4;
 constexpr int kWhereSplitWait = 5;
 
-static_assert(kWarpSmem % 16 == 0, "per-warp shared region must keep 16-byte alignment");
-static_assert(kBarBytes >= 8 * kAttnStages, "every stage needs its mbarrier inside the warp's region");
-static_assert(kAttnWarps * kWarpSmem + kCtaSmem + kClusterSmem <= 227 * 1024,
+static_assert(Ring<false>::kWarpSmem % 16 == 0 && Ring<true>::kWarpSmem % 16 == 0,
+              "per-warp shared region must keep 16-byte alignment");
+static_assert(Ring<false>::kBarBytes >= 8 * Ring<false>::kStages &&
+                  Ring<true>::kBarBytes >= 8 * Ring<true>::kStages,
+              "every stage needs its mbarrier inside the warp's region");
+static_assert(kAttnWarps * Ring<false>::kWarpSmem + kCtaSmem + kClusterSmem <= 227 * 1024 &&
+                  kAttnWarps * Ring<true>::kWarpSmem + kCtaSmem + kClusterSmem <= 227 * 1024,
               "attention CTA exceeds shared memory");
 static_assert(kCtaPartBytes % 16 == 0, "CTA partial slots must keep 16-byte alignment");
 static_assert(kAttnWarps <= 8, "one run ticket per warp in 32 bytes");
@@ -119,6 +134,23 @@ __device__ __forceinline__ void st_shared_u32(uint32_t addr, uint32_t v) {
 }
 __device__ __forceinline__ void st_shared_u16(uint32_t addr, uint16_t v) {
     asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(v) : "memory");
+}
+__device__ __forceinline__ int ld_shared_s32(uint32_t addr) {
+    int v;
+    asm volatile("ld.shared.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint4 v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                 : "memory");
 }
 // Shared-memory accessors of the CUDA-core variant (HKV_CUDA_CORES) only.
 #if HKV_CUDA_CORES
@@ -344,15 +376,22 @@ __device__ __forceinline__ void issue_unit(const PoolView &pool, int layer, int6
     bulk_load(stage, kb, kHeadBlockBytes, bar, policy);
     bulk_load(stage + kHeadBlockBytes, vb, kHeadBlockBytes, bar, policy);
 }
+// The 8-bit format: codes of K and V and both exponents in one copy.
+__device__ __forceinline__ void issue_unit_e4m3(const PoolView &pool, int layer, int64_t page, int h,
+                                                uint32_t stage, uint32_t bar, uint64_t policy) {
+    mbar_arrive_expect_tx(bar, kCodeUnitBytes);
+    bulk_load(stage, pool.base + code_unit_index(page, layer, h, pool.n_pages, pool.n_head_kv) * kCodeUnitBytes,
+              kCodeUnitBytes, bar, policy);
+}
 
 // The new K/V row of one (slot, KV head): lanes 0-15 rope and convert the
 // sixteen 8-dim chunks of K, lanes 16-31 convert those of V (same arithmetic
-// as append_kernel).  Returns the lane's 16-byte chunk.
-__device__ __forceinline__ uint4 new_row_chunk(const RopeView &rope, const float *k_row,
-                                               const float *v_row, int pos, int lane) {
+// as append_kernel).  new_row_values gives the lane's 8 values, new_row_chunk
+// their F16 chunk.
+__device__ __forceinline__ void new_row_values(const RopeView &rope, const float *k_row,
+                                               const float *v_row, int pos, int lane, float (&y)[8]) {
     const bool is_v = lane >= 16;
     const int c = lane & 15;
-    float y[8];
     if (is_v) {
         load8(v_row + c * 8, y);
     } else {
@@ -369,12 +408,79 @@ __device__ __forceinline__ uint4 new_row_chunk(const RopeView &rope, const float
             y[j] = c < 8 ? rope_lo(x0[j], x1[j], cs[j], sn[j]) : rope_hi(x0[j], x1[j], cs[j], sn[j]);
         }
     }
+}
+
+__device__ __forceinline__ uint4 new_row_chunk(const RopeView &rope, const float *k_row,
+                                               const float *v_row, int pos, int lane) {
+    float y[8];
+    new_row_values(rope, k_row, v_row, pos, lane, y);
     uint4 packed;
     packed.x = pack_half2(y[0], y[1]);
     packed.y = pack_half2(y[2], y[3]);
     packed.z = pack_half2(y[4], y[5]);
     packed.w = pack_half2(y[6], y[7]);
     return packed;
+}
+
+// The new row into the last page of a (slot, KV head) of the 8-bit cache, in
+// the pool and in the warp's staged copy (code blocks at kt and vt, exponents at
+// et): lanes 0-15 write K, lanes 16-31 V.  Where a row needs a larger exponent
+// than the rows before it were held under, the warp first rounds those again.
+__device__ __forceinline__ void append_row_e4m3(const PoolView &pool, const RopeView &rope, const float *k_row,
+                                                const float *v_row, int pos, int layer, int64_t page, int h,
+                                                uint32_t kt, uint32_t vt, uint32_t et, int lane) {
+    float y[8];
+    new_row_values(rope, k_row, v_row, pos, lane, y);
+    const bool is_v = lane >= 16;
+    const int r = pos & 15;
+    uint8_t *unit = pool.base + code_unit_index(page, layer, h, pool.n_pages, pool.n_head_kv) * kCodeUnitBytes;
+    float amax = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        amax = fmaxf(amax, finite_abs(y[j]));
+    }
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) {
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+    }
+    const int e_old = r > 0 ? ld_shared_s32(et + (is_v ? 4 : 0)) : kExpMin;
+    const int e = max(block_exponent(amax), e_old);
+    const int grow = r > 0 ? e - e_old : 0;
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+        const int d = __shfl_sync(0xffffffffu, grow, side * 16);
+        if (d > 0) {
+            for (int i = lane; i < kPageTokens * 8; i += 32) {
+                if ((i >> 3) != r) {
+                    // rows past the new one are not attended (the staged V
+                    // holds zeros there): they change in the pool only
+                    uint4 *held = reinterpret_cast<uint4 *>(unit + side * kCodeBlockBytes) + i;
+                    const bool past = (i >> 3) > r;
+                    uint4 c = past ? *held : ld_shared_v4((side ? vt : kt) + i * 16);
+                    c.x = rescale_codes4(c.x, d);
+                    c.y = rescale_codes4(c.y, d);
+                    c.z = rescale_codes4(c.z, d);
+                    c.w = rescale_codes4(c.w, d);
+                    if (!past) {
+                        st_shared_v4((side ? vt : kt) + i * 16, c);
+                    }
+                    *held = c;
+                }
+            }
+        }
+    }
+    const float inv = pow2(-e);
+    const uint2 codes = make_uint2(to_codes4(make_float4(y[0], y[1], y[2], y[3]), inv),
+                                   to_codes4(make_float4(y[4], y[5], y[6], y[7]), inv));
+    const int c = lane & 15;
+    const int off = r * kHeadDim + (((c >> 1) ^ (r & 7)) << 4) + (c & 1) * 8;
+    *reinterpret_cast<uint2 *>(unit + (is_v ? kCodeBlockBytes : 0) + off) = codes;
+    asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"((is_v ? vt : kt) + off), "r"(codes.x), "r"(codes.y)
+                 : "memory");
+    if (c == 0) {
+        reinterpret_cast<int *>(unit + 2 * kCodeBlockBytes)[is_v ? 1 : 0] = e;
+        st_shared_u32(et + (is_v ? 4 : 0), static_cast<uint32_t>(e));
+    }
 }
 
 // Merge of one (slot, KV head)'s partials by the warp that finished last.
@@ -669,7 +775,21 @@ __device__ __forceinline__ void signal_arrival(const Exchange &x, int layer, int
 
 // kCluster (with kCtaMerge): the launch is in clusters of batch.cluster CTAs,
 // one (slot, KV head) segment per cluster (plan_cluster).
-template <bool kAppend, bool kCtaMerge, bool kCluster>
+//
+// kE4m3: the 8-bit cache.  Codes become F16 in registers (exact) on their way
+// into the same MMAs, and both exponents stay out of the products:
+//   s_t = (q . c_t) 2^eK scale          one factor per page, on the logits
+//   o   = sum_t p_t 2^(eV - E) c_t      E: the largest eV of the share so far,
+// so the weights of the second product are at most 1 whatever the exponents
+// are, and o is scaled by 2^E when it leaves the registers.  The weights enter
+// 2^kPShift larger: their F16 parts then keep their bits for pages whose V is
+// far smaller than another page's.  l sums the unscaled p_t.
+// The dims of a head are permuted so that a lane's codes are whole 16-byte
+// chunks and no ldmatrix is needed: lane (g, t) = (lane / 4, lane % 4) reads
+// dims 32t .. 32t + 31 of K rows g and g + 8 (the MMA's k index may be any
+// permutation of the dims if q uses the same), and dims 16g .. 16g + 15 of V
+// rows 2t, 2t + 1, 2t + 8, 2t + 9, whose bytes pair up to the A fragment of V^T.
+template <bool kAppend, bool kCtaMerge, bool kCluster, bool kE4m3>
 __global__ void __launch_bounds__(kAttnWarps * 32, 1)
     attention_kernel(PoolView pool, RopeView rope, BatchView batch, int layer,
                      const float *__restrict__ q, const float *__restrict__ k_new,
@@ -683,6 +803,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
     const int G = pool.n_head_kv;
     const int W = batch.n_warps;
     static_assert(kCtaMerge || !kCluster, "the cluster merge starts from the CTA merge");
+    constexpr int kStages = Ring<kE4m3>::kStages;
+    constexpr int kStage = Ring<kE4m3>::kStage;
+    constexpr int kWarpSmem = Ring<kE4m3>::kWarpSmem;
     float *cta_slots = reinterpret_cast<float *>(smem + kAttnWarps * kWarpSmem);
     int *run_ticket = reinterpret_cast<int *>(smem + kAttnWarps * kWarpSmem + kAttnWarps * 2 * kCtaPartBytes);
     float *cl_slots = reinterpret_cast<float *>(smem + kAttnWarps * kWarpSmem + kCtaSmem);
@@ -718,14 +841,21 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
         return;
     }
     const uint32_t stage0 = smem_u32(smem + wid * kWarpSmem);
-    const uint32_t qc = stage0 + kAttnStages * kStageBytes;
+    const uint32_t qc = stage0 + kStages * kStage;
     const uint32_t pbuf = qc + kQcBytes;
     const uint32_t bar0 = pbuf + kPBufBytes;
     const uint64_t policy = evict_first_policy();
+    auto issue = [&](int64_t page, int h, uint32_t stage, uint32_t bar) {
+        if constexpr (kE4m3) {
+            issue_unit_e4m3(pool, layer, page, h, stage, bar, policy);
+        } else {
+            issue_unit(pool, layer, page, h, stage, bar, policy);
+        }
+    };
 
     if (lane == 0) {
 #pragma unroll
-        for (int s = 0; s < kAttnStages; ++s) {
+        for (int s = 0; s < kStages; ++s) {
             mbar_init(bar0 + 8 * s, 1);
         }
         fence_barrier_init();
@@ -745,15 +875,15 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
     if (lane == 0) {
         const int first_pages[3] = {ws1.y, ws1.z, ws1.w};
 #pragma unroll
-        for (int s = 0; s < kAttnStages; ++s) {
+        for (int s = 0; s < kStages; ++s) {
             if (u_begin + s < u_end) {
                 const int64_t page = checked_page(
                     pool, s < 3 ? first_pages[s] : batch.pages[prod.pbase + prod.i], prod.e, err);
-                issue_unit(pool, layer, page, prod.h, stage0 + s * kStageBytes, bar0 + 8 * s, policy);
+                issue(page, prod.h, stage0 + s * kStage, bar0 + 8 * s);
                 advance(batch, G, prod);
             }
         }
-        if (u_begin + kAttnStages < u_end) {
+        if (u_begin + kStages < u_end) {
             next_page = batch.pages[prod.pbase + prod.i];
         }
     }
@@ -782,6 +912,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
     float4 acc[kGqa];
 #endif
     float m_a = kNegInf, m_b = kNegInf, l_a = 0.f, l_b = 0.f;
+    int e_v = 0;  // E: o is held in units of 2^(E - kPShift)
     int seg_e = 0, seg_h = 0, seg_pos = 0, part = 0, p_first = 0, nparts = 1, ntok = 0;
     int run_w0 = wid, run_m = 1;  // this CTA's warps of the current segment: w0 .. w0 + m - 1
 
@@ -809,11 +940,15 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
         }
         __syncwarp();
 #endif
+        const float o_scale = kE4m3 ? pow2(max(e_v - kPShift, -126)) : 1.f;
 #pragma unroll
         for (int mt = 0; mt < 8; ++mt) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 o[mt][j] += __shfl_xor_sync(0xffffffffu, o[mt][j], 2);
+                if (kE4m3) {
+                    o[mt][j] *= o_scale;
+                }
             }
         }
         l_a += __shfl_xor_sync(0xffffffffu, l_a, 4);
@@ -824,6 +959,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
         l_b += __shfl_xor_sync(0xffffffffu, l_b, 16);
         const int ha = (lane & 1) * 2;
         const int d0 = lane >> 2;
+        // the two dims whose sums o[mt] holds
+        auto dim_lo = [&](int mt) { return kE4m3 ? 16 * d0 + 2 * mt : 16 * mt + d0; };
+        auto dim_hi = [&](int mt) { return kE4m3 ? 16 * d0 + 2 * mt + 1 : 16 * mt + d0 + 8; };
         const int n_dst = xchg.n_ranks == 0 ? 1 : xchg.n_ranks;
         if (nparts == 1 && run_m == 1) {
             // The whole (slot, KV head) was this warp's: write the output.
@@ -834,10 +972,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
                     float *ob = out_slice(out, xchg, r, layer, seg_e, seg_h, G);
 #pragma unroll
                     for (int mt = 0; mt < 8; ++mt) {
-                        ob[ha * kHeadDim + 16 * mt + d0] = o[mt][0] * ia;
-                        ob[(ha + 1) * kHeadDim + 16 * mt + d0] = o[mt][1] * ib;
-                        ob[ha * kHeadDim + 16 * mt + d0 + 8] = o[mt][2] * ia;
-                        ob[(ha + 1) * kHeadDim + 16 * mt + d0 + 8] = o[mt][3] * ib;
+                        ob[ha * kHeadDim + dim_lo(mt)] = o[mt][0] * ia;
+                        ob[(ha + 1) * kHeadDim + dim_lo(mt)] = o[mt][1] * ib;
+                        ob[ha * kHeadDim + dim_hi(mt)] = o[mt][2] * ia;
+                        ob[(ha + 1) * kHeadDim + dim_hi(mt)] = o[mt][3] * ib;
                     }
                 }
             }
@@ -858,10 +996,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
         if (!lo_side) {
 #pragma unroll
             for (int mt = 0; mt < 8; ++mt) {
-                po[ha * kHeadDim + 16 * mt + d0] = o[mt][0];
-                po[(ha + 1) * kHeadDim + 16 * mt + d0] = o[mt][1];
-                po[ha * kHeadDim + 16 * mt + d0 + 8] = o[mt][2];
-                po[(ha + 1) * kHeadDim + 16 * mt + d0 + 8] = o[mt][3];
+                po[ha * kHeadDim + dim_lo(mt)] = o[mt][0];
+                po[(ha + 1) * kHeadDim + dim_lo(mt)] = o[mt][1];
+                po[ha * kHeadDim + dim_hi(mt)] = o[mt][2];
+                po[(ha + 1) * kHeadDim + dim_hi(mt)] = o[mt][3];
             }
             if (d0 == 0) {
                 pm[ha * 2] = m_a;
@@ -1063,8 +1201,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
     };
 
     for (int u = u_begin, k = 0; u < u_end; ++u, ++k) {
-        const int s = k % kAttnStages;
-        const uint32_t parity = static_cast<uint32_t>(k / kAttnStages) & 1u;
+        const int s = k % kStages;
+        const uint32_t parity = static_cast<uint32_t>(k / kStages) & 1u;
         if (u == u_begin || cons.i == 0) {
             if (u != u_begin) {
                 flush(false);
@@ -1129,10 +1267,21 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
                 acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
             }
 #else
+            if constexpr (kE4m3) {
+#pragma unroll
+                for (int jj = 0; jj < 4; ++jj) {
+                    const uint4 w = ld_shared_v4(qc + ((lane >> 2) * kQcStride + (lane & 3) * 32 + jj * 8) * 2);
+                    qb[2 * jj][0] = w.x;
+                    qb[2 * jj][1] = w.y;
+                    qb[2 * jj + 1][0] = w.z;
+                    qb[2 * jj + 1][1] = w.w;
+                }
+            } else {
 #pragma unroll
             for (int jj = 0; jj < 4; ++jj) {
                 ldsm_x4(qc + (r7 * kQcStride + jj * 32 + mi * 8) * 2, qb[2 * jj][0],
                         qb[2 * jj][1], qb[2 * jj + 1][0], qb[2 * jj + 1][1]);
+            }
             }
 #endif
 #pragma unroll
@@ -1144,6 +1293,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
             }
             m_a = m_b = kNegInf;
             l_a = l_b = 0.f;
+            e_v = kExpMin;
         }
 
         // ---- wait for this unit's K and V head blocks
@@ -1154,34 +1304,40 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
                 record_error(err, kErrTimeout, kWhereAttn, u, blockIdx.x);
             }
             // Drain the copies this warp still has in flight, then leave.
-            for (int j = 1; j < kAttnStages && u + j < u_end; ++j) {
+            for (int j = 1; j < kStages && u + j < u_end; ++j) {
                 const int kk = k + j;
-                mbar_wait_bounded(bar0 + 8 * (kk % kAttnStages),
-                                  static_cast<uint32_t>(kk / kAttnStages) & 1u);
+                mbar_wait_bounded(bar0 + 8 * (kk % kStages),
+                                  static_cast<uint32_t>(kk / kStages) & 1u);
             }
             return;
         }
-        const uint32_t kt = stage0 + s * kStageBytes;
-        const uint32_t vt = kt + kHeadBlockBytes;
+        const uint32_t kt = stage0 + s * kStage;
+        const uint32_t vt = kt + (kE4m3 ? kCodeBlockBytes : kHeadBlockBytes);
+        const uint32_t et = kt + 2 * kCodeBlockBytes;  // exponents (8-bit format)
         const int row0 = cons.i * kPageTokens;
         const int valid = min(kPageTokens, ntok - row0);
         if (valid < kPageTokens) {
             // Rows past the slot's length hold whatever the page had before;
             // zero them in shared memory so 0 * garbage cannot poison PV.
-            for (int idx = lane; idx < (kPageTokens - valid) * 16; idx += 32) {
-                st_shared_zero16(vt + (valid + (idx >> 4)) * kRowBytes + (idx & 15) * 16);
+            constexpr int kRow = kE4m3 ? kHeadDim : kRowBytes;
+            for (int idx = lane; idx < (kPageTokens - valid) * (kRow / 16); idx += 32) {
+                st_shared_zero16(vt + valid * kRow + idx * 16);
             }
         }
         if (kAppend && cons.i == cons.np - 1) {
             // Fused append: this warp owns the slot's last page for this KV
             // head, so it writes the new row to HBM and into its copy of the
             // page (the copy arrived without it).
+            const int64_t row_base = (static_cast<int64_t>(seg_e) * G + seg_h) * kHeadDim;
+            const int64_t page = checked_page(pool, batch.pages[cons.pbase + cons.i], seg_e, err);
+            if constexpr (kE4m3) {
+                append_row_e4m3(pool, rope, k_new + row_base, v_new + row_base, seg_pos, layer, page, seg_h, kt,
+                                vt, et, lane);
+            } else {
             const int r = seg_pos & 15;
             const int c = lane & 15;
             const bool is_v = lane >= 16;
-            const int64_t row_base = (static_cast<int64_t>(seg_e) * G + seg_h) * kHeadDim;
             const uint4 chunk = new_row_chunk(rope, k_new + row_base, v_new + row_base, seg_pos, lane);
-            const int64_t page = checked_page(pool, batch.pages[cons.pbase + cons.i], seg_e, err);
             uint8_t *dst = pool.base +
                            head_block_index(page, layer, is_v ? 1 : 0, seg_h, pool.n_pages, G) *
                                kHeadBlockBytes +
@@ -1191,6 +1347,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
             asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(sdst), "r"(chunk.x),
                          "r"(chunk.y), "r"(chunk.z), "r"(chunk.w)
                          : "memory");
+            }
         }
         if (valid < kPageTokens || (kAppend && cons.i == cons.np - 1)) {
             fence_proxy_async_smem();
@@ -1239,6 +1396,23 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
         // Two accumulators (even / odd k-steps) halve the dependent mma chain.
         float sc[4] = {0.f, 0.f, 0.f, 0.f};
         float sd[4] = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (kE4m3) {
+            const int g = lane >> 2;
+            const int t = lane & 3;
+            uint32_t w0[8], w1[8];  // rows g and g + 8 (the same swizzle: g + 8 = g mod 8)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint4 lo = ld_shared_v4(kt + g * kHeadDim + (((2 * t + i) ^ g) << 4));
+                const uint4 hi = ld_shared_v4(kt + (g + 8) * kHeadDim + (((2 * t + i) ^ g) << 4));
+                w0[4 * i] = lo.x; w0[4 * i + 1] = lo.y; w0[4 * i + 2] = lo.z; w0[4 * i + 3] = lo.w;
+                w1[4 * i] = hi.x; w1[4 * i + 1] = hi.y; w1[4 * i + 2] = hi.z; w1[4 * i + 3] = hi.w;
+            }
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks) {
+                mma_16816(ks & 1 ? sd : sc, codes_to_half2(w0[ks]), codes_to_half2(w1[ks]),
+                          codes_to_half2_hi(w0[ks]), codes_to_half2_hi(w1[ks]), qb[ks][0], qb[ks][1]);
+            }
+        } else {
 #pragma unroll
         for (int ks = 0; ks < 8; ks += 2) {
             uint32_t a0, a1, a2, a3, b0, b1, b2, b3;
@@ -1247,6 +1421,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
             mma_16816(sc, a0, a1, a2, a3, qb[ks][0], qb[ks][1]);
             mma_16816(sd, b0, b1, b2, b3, qb[ks + 1][0], qb[ks + 1][1]);
         }
+        }
 #endif
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -1254,10 +1429,11 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
             sc[j] += __shfl_xor_sync(0xffffffffu, sc[j], 2);
         }
         const int tok = row0 + (lane >> 2);
-        const float s0 = tok < ntok ? sc[0] * scale_log2 : kNegInf;      // head a, row g
-        const float s1 = tok < ntok ? sc[1] * scale_log2 : kNegInf;      // head b, row g
-        const float s2 = tok + 8 < ntok ? sc[2] * scale_log2 : kNegInf;  // head a, row g+8
-        const float s3 = tok + 8 < ntok ? sc[3] * scale_log2 : kNegInf;  // head b, row g+8
+        const float s_scale = kE4m3 ? scale_log2 * pow2(ld_shared_s32(et)) : scale_log2;
+        const float s0 = tok < ntok ? sc[0] * s_scale : kNegInf;      // head a, row g
+        const float s1 = tok < ntok ? sc[1] * s_scale : kNegInf;      // head b, row g
+        const float s2 = tok + 8 < ntok ? sc[2] * s_scale : kNegInf;  // head a, row g+8
+        const float s3 = tok + 8 < ntok ? sc[3] * s_scale : kNegInf;  // head b, row g+8
         float mx_a = fmaxf(s0, s2);
         float mx_b = fmaxf(s1, s3);
 #pragma unroll
@@ -1267,16 +1443,30 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
         }
         const float mn_a = fmaxf(m_a, mx_a);
         const float mn_b = fmaxf(m_b, mx_b);
-        const float alpha_a = exp2f(m_a - mn_a);
-        const float alpha_b = exp2f(m_b - mn_b);
-        const float p0 = exp2f(s0 - mn_a);
-        const float p1 = exp2f(s1 - mn_b);
-        const float p2 = exp2f(s2 - mn_a);
-        const float p3 = exp2f(s3 - mn_b);
+        float alpha_a = exp2f(m_a - mn_a);
+        float alpha_b = exp2f(m_b - mn_b);
+        float p0 = exp2f(s0 - mn_a);
+        float p1 = exp2f(s1 - mn_b);
+        float p2 = exp2f(s2 - mn_a);
+        float p3 = exp2f(s3 - mn_b);
         l_a = l_a * alpha_a + (p0 + p2);
         l_b = l_b * alpha_b + (p1 + p3);
         m_a = mn_a;
         m_b = mn_b;
+        if (kE4m3) {
+            // from here on alpha rescales o only, and p are o's weights
+            const int e_page = ld_shared_s32(et + 4);
+            const int e_new = max(e_v, e_page);
+            const float grow = pow2(max(e_v - e_new, -126));
+            const float w = pow2(max(e_page - e_new + kPShift, -126));
+            e_v = e_new;
+            alpha_a *= grow;
+            alpha_b *= grow;
+            p0 *= w;
+            p1 *= w;
+            p2 *= w;
+            p3 *= w;
+        }
 #if HKV_CUDA_CORES
         // ---- CUDA cores: p (F32) to shared memory as [token][head], then each
         // lane accumulates its 4 dims of every head over the 16 tokens.
@@ -1338,6 +1528,33 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
         ldsm_x2_trans(pbuf + (lane & 15) * 16, pb0, pb1);
 
         // ---- O^T[dim][col] += V^T[dim][token] . P^T[token][col]
+        if constexpr (kE4m3) {
+            const int g = lane >> 2;
+            const int t = lane & 3;
+            uint32_t va[4], vb[4], vc[4], vd[4];  // rows 2t, 2t + 1, 2t + 8, 2t + 9
+            {
+                const int r = 2 * t;
+                const uint4 a = ld_shared_v4(vt + r * kHeadDim + ((g ^ r) << 4));
+                const uint4 b = ld_shared_v4(vt + (r + 1) * kHeadDim + ((g ^ (r + 1)) << 4));
+                const uint4 c = ld_shared_v4(vt + (r + 8) * kHeadDim + ((g ^ r) << 4));
+                const uint4 d = ld_shared_v4(vt + (r + 9) * kHeadDim + ((g ^ (r + 1)) << 4));
+                va[0] = a.x; va[1] = a.y; va[2] = a.z; va[3] = a.w;
+                vb[0] = b.x; vb[1] = b.y; vb[2] = b.z; vb[3] = b.w;
+                vc[0] = c.x; vc[1] = c.y; vc[2] = c.z; vc[3] = c.w;
+                vd[0] = d.x; vd[1] = d.y; vd[2] = d.z; vd[3] = d.w;
+            }
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    // dims 4w + 2 half and + 1 of the lane's 16, two rows a pair
+                    const uint32_t ab = __byte_perm(va[w], vb[w], half ? 0x7362 : 0x5140);
+                    const uint32_t cd = __byte_perm(vc[w], vd[w], half ? 0x7362 : 0x5140);
+                    mma_16816(o[2 * w + half], codes_to_half2(ab), codes_to_half2_hi(ab), codes_to_half2(cd),
+                              codes_to_half2_hi(cd), pb0, pb1);
+                }
+            }
+        } else {
 #pragma unroll
         for (int mt = 0; mt < 8; ++mt) {
             uint32_t a0, a1, a2, a3;
@@ -1345,14 +1562,14 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
             ldsm_x4_trans(vt + v_row_off + ((chunk ^ r7) << 4), a0, a1, a2, a3);
             mma_16816(o[mt], a0, a1, a2, a3, pb0, pb1);
         }
+        }
 #endif
         __syncwarp();
-        if (lane == 0 && u + kAttnStages < u_end) {
+        if (lane == 0 && u + kStages < u_end) {
             fence_proxy_async_smem();
-            issue_unit(pool, layer, checked_page(pool, next_page, prod.e, err), prod.h, kt, bar,
-                       policy);
+            issue(checked_page(pool, next_page, prod.e, err), prod.h, kt, bar);
             advance(batch, G, prod);
-            if (u + kAttnStages + 1 < u_end) {
+            if (u + kStages + 1 < u_end) {
                 next_page = batch.pages[prod.pbase + prod.i];
             }
         }
@@ -1501,7 +1718,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32)
 
 // ================================================================ copy-on-write
 // One block per (page pair, layer): copies the source page's K and V head
-// blocks of that layer (2 * n_head_kv * 4 KiB, contiguous in the layer's slab)
+// blocks of that layer (contiguous in the layer's slab, exponents included)
 // onto the destination page with 16-byte loads and stores.  All pending
 // copies of a call go out in this one launch.
 __global__ void __launch_bounds__(256) cow_copy_kernel(PoolView pool, const int2 *__restrict__ pairs,
@@ -1519,12 +1736,11 @@ __global__ void __launch_bounds__(256) cow_copy_kernel(PoolView pool, const int2
         }
         return;
     }
-    const int G = pool.n_head_kv;
+    const int64_t page_bytes = static_cast<int64_t>(pool.n_head_kv) * cache_unit_bytes(pool.format);
     const uint4 *src = reinterpret_cast<const uint4 *>(
-        pool.base + head_block_index(pr.x, layer, 0, 0, pool.n_pages, G) * kHeadBlockBytes);
-    uint4 *dst = reinterpret_cast<uint4 *>(
-        pool.base + head_block_index(pr.y, layer, 0, 0, pool.n_pages, G) * kHeadBlockBytes);
-    const int n16 = 2 * G * kHeadBlockBytes / 16;
+        pool.base + (layer * pool.n_pages + pr.x) * page_bytes);
+    uint4 *dst = reinterpret_cast<uint4 *>(pool.base + (layer * pool.n_pages + pr.y) * page_bytes);
+    const int n16 = static_cast<int>(page_bytes / 16);
     for (int i = threadIdx.x; i < n16; i += blockDim.x) {
         dst[i] = __ldcs(src + i);
     }
@@ -1564,22 +1780,22 @@ __global__ void gather_kernel(PoolView pool, const int32_t *__restrict__ slot_pa
 
 }  // namespace
 
-size_t attention_smem_bytes(bool cta_merge, bool cluster) {
-    return static_cast<size_t>(kAttnWarps) * kWarpSmem + (cta_merge ? kCtaSmem : 0) +
+size_t attention_smem_bytes(bool cta_merge, bool cluster, bool e4m3) {
+    return static_cast<size_t>(kAttnWarps) * (e4m3 ? Ring<true>::kWarpSmem : Ring<false>::kWarpSmem) + (cta_merge ? kCtaSmem : 0) +
            (cluster ? kClusterSmem : 0);
 }
 
 // The shared-memory opt-in (and, for the cluster variant, sizes up to 16) of
 // one attention kernel, once per device.
-template <bool kAppend, bool kCtaMerge, bool kCluster>
+template <bool kAppend, bool kCtaMerge, bool kCluster, bool kE4m3>
 void configure_attention(int dev) {
     static bool configured[64] = {};
     if (dev >= 0 && dev < 64 && configured[dev]) {
         return;
     }
-    auto kern = attention_kernel<kAppend, kCtaMerge, kCluster>;
+    auto kern = attention_kernel<kAppend, kCtaMerge, kCluster, kE4m3>;
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                         static_cast<int>(attention_smem_bytes(kCtaMerge, kCluster)));
+                         static_cast<int>(attention_smem_bytes(kCtaMerge, kCluster, kE4m3)));
     if (kCluster) {
         cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     }
@@ -1588,7 +1804,8 @@ void configure_attention(int dev) {
     }
 }
 
-int attention_cluster_fit(int csize) {
+template <bool kE4m3>
+int cluster_fit(int csize) {
     static std::mutex mu;
     static int cache[64][kMaxCluster + 1] = {};
     if (csize < 2 || csize > kMaxCluster) {
@@ -1602,11 +1819,11 @@ int attention_cluster_fit(int csize) {
     if (cache[dev][csize] != 0) {
         return cache[dev][csize] > 0 ? cache[dev][csize] : 0;
     }
-    configure_attention<true, true, true>(dev);
+    configure_attention<true, true, true, kE4m3>(dev);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(csize));
     cfg.blockDim = dim3(kAttnWarps * 32);
-    cfg.dynamicSmemBytes = attention_smem_bytes(true, true);
+    cfg.dynamicSmemBytes = attention_smem_bytes(true, true, kE4m3);
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = static_cast<unsigned>(csize);
@@ -1615,12 +1832,16 @@ int attention_cluster_fit(int csize) {
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, attention_kernel<true, true, true>, &cfg) != cudaSuccess) {
+    if (cudaOccupancyMaxActiveClusters(&n, attention_kernel<true, true, true, kE4m3>, &cfg) != cudaSuccess) {
         n = 0;
     }
     (void)cudaGetLastError();
     cache[dev][csize] = n > 0 ? n : -1;
     return n > 0 ? n : 0;
+}
+
+int attention_cluster_fit(int csize, int format) {
+    return format == kCacheE4m3 ? cluster_fit<true>(csize) : cluster_fit<false>(csize);
 }
 
 void launch_append(const PoolView &pool, const RopeView &rope, const BatchView &batch, int layer,
@@ -1652,7 +1873,7 @@ void launch_append_range(const PoolView &pool, const RopeView &rope, const int32
     }
 }
 
-template <bool kAppend, bool kCtaMerge, bool kCluster>
+template <bool kAppend, bool kCtaMerge, bool kCluster, bool kE4m3>
 void launch_attention_t(const PoolView &pool, const RopeView &rope, const BatchView &batch,
                         int layer, const float *q, const float *k_new, const float *v_new,
                         float *part_o, float *part_ml, int32_t *counters, float *out,
@@ -1660,12 +1881,12 @@ void launch_attention_t(const PoolView &pool, const RopeView &rope, const BatchV
                         bool overlap_previous, cudaStream_t stream) {
     int dev = 0;
     cudaGetDevice(&dev);
-    configure_attention<kAppend, kCtaMerge, kCluster>(dev);
+    configure_attention<kAppend, kCtaMerge, kCluster, kE4m3>(dev);
     const int grid = (batch.n_warps + kAttnWarps - 1) / kAttnWarps;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(grid));
     cfg.blockDim = dim3(kAttnWarps * 32);
-    cfg.dynamicSmemBytes = attention_smem_bytes(kCtaMerge, kCluster);
+    cfg.dynamicSmemBytes = attention_smem_bytes(kCtaMerge, kCluster, kE4m3);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     int n_attr = 0;
@@ -1683,7 +1904,7 @@ void launch_attention_t(const PoolView &pool, const RopeView &rope, const BatchV
     }
     cfg.attrs = attr;
     cfg.numAttrs = static_cast<unsigned>(n_attr);
-    cudaLaunchKernelEx(&cfg, attention_kernel<kAppend, kCtaMerge, kCluster>, pool, rope, batch, layer, q,
+    cudaLaunchKernelEx(&cfg, attention_kernel<kAppend, kCtaMerge, kCluster, kE4m3>, pool, rope, batch, layer, q,
                        k_new, v_new, part_o, part_ml, counters, out, xchg, scale_log2, err);
     if (batch.combine && batch.split_segments > 0) {
         cudaLaunchConfig_t cc = {};
@@ -1698,34 +1919,43 @@ void launch_attention_t(const PoolView &pool, const RopeView &rope, const BatchV
     }
 }
 
+template <bool kE4m3>
+void launch_attention_f(const PoolView &pool, const RopeView &rope, const BatchView &batch, int layer,
+                        const float *q, const float *k_new, const float *v_new, float *part_o,
+                        float *part_ml, int32_t *counters, float *out, const Exchange &xchg,
+                        float scale_log2, DeviceError *err, bool overlap_previous,
+                        cudaStream_t stream) {
+    const bool append = k_new != nullptr && v_new != nullptr;
+    if (!append) {
+        k_new = v_new = nullptr;
+    }
+    auto launch = [&](auto kernel_launch) {
+        kernel_launch(pool, rope, batch, layer, q, k_new, v_new, part_o, part_ml, counters, out, xchg, scale_log2,
+                      err, overlap_previous, stream);
+    };
+    if (append && batch.cluster > 0) {
+        launch(launch_attention_t<true, true, true, kE4m3>);
+    } else if (append && batch.cta_merge) {
+        launch(launch_attention_t<true, true, false, kE4m3>);
+    } else if (append) {
+        launch(launch_attention_t<true, false, false, kE4m3>);
+    } else if (batch.cluster > 0) {
+        launch(launch_attention_t<false, true, true, kE4m3>);
+    } else if (batch.cta_merge) {
+        launch(launch_attention_t<false, true, false, kE4m3>);
+    } else {
+        launch(launch_attention_t<false, false, false, kE4m3>);
+    }
+}
+
 void launch_attention(const PoolView &pool, const RopeView &rope, const BatchView &batch, int layer,
                       const float *q, const float *k_new, const float *v_new, float *part_o,
                       float *part_ml, int32_t *counters, float *out, const Exchange &xchg,
                       float scale_log2, DeviceError *err, bool overlap_previous,
                       cudaStream_t stream) {
-    const bool append = k_new != nullptr && v_new != nullptr;
-    if (!append) {
-        k_new = v_new = nullptr;
-    }
-    if (append && batch.cluster > 0) {
-        launch_attention_t<true, true, true>(pool, rope, batch, layer, q, k_new, v_new, part_o, part_ml,
-                                             counters, out, xchg, scale_log2, err, overlap_previous, stream);
-    } else if (append && batch.cta_merge) {
-        launch_attention_t<true, true, false>(pool, rope, batch, layer, q, k_new, v_new, part_o, part_ml,
-                                              counters, out, xchg, scale_log2, err, overlap_previous, stream);
-    } else if (append) {
-        launch_attention_t<true, false, false>(pool, rope, batch, layer, q, k_new, v_new, part_o, part_ml,
-                                               counters, out, xchg, scale_log2, err, overlap_previous, stream);
-    } else if (batch.cluster > 0) {
-        launch_attention_t<false, true, true>(pool, rope, batch, layer, q, k_new, v_new, part_o, part_ml,
-                                              counters, out, xchg, scale_log2, err, overlap_previous, stream);
-    } else if (batch.cta_merge) {
-        launch_attention_t<false, true, false>(pool, rope, batch, layer, q, k_new, v_new, part_o, part_ml,
-                                               counters, out, xchg, scale_log2, err, overlap_previous, stream);
-    } else {
-        launch_attention_t<false, false, false>(pool, rope, batch, layer, q, k_new, v_new, part_o, part_ml,
-                                                counters, out, xchg, scale_log2, err, overlap_previous, stream);
-    }
+    auto launch = pool.format == kCacheE4m3 ? launch_attention_f<true> : launch_attention_f<false>;
+    launch(pool, rope, batch, layer, q, k_new, v_new, part_o, part_ml, counters, out, xchg, scale_log2, err,
+           overlap_previous, stream);
 }
 
 // =================================================================== split wait

@@ -43,6 +43,15 @@ KERNEL_GATHER = 3
 KERNEL_STEP = 4
 
 
+CACHE_F16 = 0
+CACHE_E4M3 = 1
+CACHE_TYPES = {"f16": CACHE_F16, "e4m3": CACHE_E4M3}
+
+F32 = 0
+F16 = 1
+BF16 = 2
+
+
 class HkvError(RuntimeError):
     def __init__(self, status: int, message: str):
         super().__init__(message)
@@ -85,6 +94,18 @@ class PoolStats(ctypes.Structure):
         ("cow_copies", ctypes.c_int64),
         ("kernel_launches", ctypes.c_int64),
     ]
+
+
+class QkvWriteArgs(ctypes.Structure):
+    """hkv_qkv_write_args."""
+    _fields_ = [("layer", ctypes.c_int32), ("n", ctypes.c_int32),
+                ("slots", ctypes.POINTER(ctypes.c_int32)),
+                ("n_tokens", ctypes.POINTER(ctypes.c_int64)), ("dtype", ctypes.c_int32),
+                ("eps", ctypes.c_float), ("q", ctypes.c_void_p), ("k", ctypes.c_void_p),
+                ("v", ctypes.c_void_p), ("q_stride", ctypes.c_int64), ("k_stride", ctypes.c_int64),
+                ("v_stride", ctypes.c_int64), ("q_out_stride", ctypes.c_int64),
+                ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p),
+                ("q_out", ctypes.c_void_p)]
 
 
 class PagedView(ctypes.Structure):
@@ -147,6 +168,8 @@ SIGNATURES = {
     "hkv_last_error": ([_P], ctypes.c_char_p),
     "hkv_config_default": ([ctypes.POINTER(Config)], ctypes.c_int),
     "hkv_engine_create": ([ctypes.POINTER(Config), ctypes.POINTER(_P)], ctypes.c_int),
+    "hkv_engine_create_cache": ([ctypes.POINTER(Config), _I32, ctypes.POINTER(_P)], ctypes.c_int),
+    "hkv_engine_cache_type": ([_P, _I32P], ctypes.c_int),
     "hkv_engine_destroy": ([_P], ctypes.c_int),
     "hkv_slot_acquire": ([_P, _I64, ctypes.POINTER(PrefixKey), _I32P], ctypes.c_int),
     "hkv_slot_release": ([_P, _I32], ctypes.c_int),
@@ -164,6 +187,8 @@ SIGNATURES = {
     "hkv_decode_attn": ([_P, _I32, _I32, _I32P, _P, _P, _P], ctypes.c_int),
     "hkv_decode_step": ([_P, _I32, _I32, _I32P, _P, _P, _P, _P, _P], ctypes.c_int),
     "hkv_gather": ([_P, _I32, _I32, _I64, _I64, _P, _P, _P], ctypes.c_int),
+    "hkv_qkv_write": ([_P, ctypes.POINTER(QkvWriteArgs), _P], ctypes.c_int),
+    "hkv_cache_read": ([_P, _I32, _I32, _I32P, _I64P, _I64P, _I32, _P, _P, _P], ctypes.c_int),
     "hkv_sync_check": ([_P, _P], ctypes.c_int),
     "hkv_rope_tables": ([_P, _P, _P], ctypes.c_int),
     "hkv_decode_attn_noalloc": ([ctypes.POINTER(PagedView), _I32, _I32, _I32P, _I32P, _I32P,
@@ -249,6 +274,12 @@ def _slots_arg(slots: Sequence[int]):
     return len(slots), arr
 
 
+def _counts_arg(counts: Sequence[int], n: int):
+    if len(counts) != n:
+        raise ValueError(f"{len(counts)} lengths for {n} slots")
+    return (ctypes.c_int64 * n)(*[int(c) for c in counts])
+
+
 class ScopedBackendKvCacheSlot:
     """RAII slot lease (ScopedBackendKvCacheSlot, src/higgs_pipeline.cpp:372-403)."""
 
@@ -276,13 +307,18 @@ class Engine:
     def __init__(self, n_layers: int = 36, n_head: int = 32, n_head_kv: int = 8,
                  head_dim: int = 128, page_tokens: int = 16, context_length: int = 32768,
                  rope_freq_base: float = 1e6, max_slots: int = 256, n_pages: int = 4096,
-                 device: int = 0, shuffle_seed: int = 0, lib: Optional[ctypes.CDLL] = None):
+                 device: int = 0, shuffle_seed: int = 0, lib: Optional[ctypes.CDLL] = None,
+                 cache: str = "f16"):
+        """cache: "f16", or "e4m3" for 8 bits a value with a scale per page and KV head."""
+        if cache not in CACHE_TYPES:
+            raise ValueError(f"cache {cache!r}: one of {sorted(CACHE_TYPES)}")
         self.lib = lib or load_library()
         self.handle = None
         self.cfg = Config(n_layers, n_head, n_head_kv, head_dim, page_tokens, context_length,
                           rope_freq_base, max_slots, n_pages, device, shuffle_seed)
         h = ctypes.c_void_p()
-        st = self.lib.hkv_engine_create(ctypes.byref(self.cfg), ctypes.byref(h))
+        st = self.lib.hkv_engine_create_cache(ctypes.byref(self.cfg), CACHE_TYPES[cache],
+                                              ctypes.byref(h))
         if st != HKV_OK:
             raise HkvError(st, f"hkv_engine_create failed: "
                                f"{self.lib.hkv_status_string(st).decode()}")
@@ -399,6 +435,33 @@ class Engine:
     def gather(self, slot: int, layer: int, pos0: int, n: int, k_out, v_out, stream=None) -> None:
         self._check(self.lib.hkv_gather(self.handle, slot, layer, pos0, n, _ptr(k_out),
                                         _ptr(v_out), _stream(stream)))
+
+    @property
+    def cache(self) -> str:
+        """"f16" or "e4m3"."""
+        t = ctypes.c_int32()
+        self._check(self.lib.hkv_engine_cache_type(self.handle, ctypes.byref(t)))
+        return {v: k for k, v in CACHE_TYPES.items()}[t.value]
+
+    def qkv_write(self, layer: int, slots: Sequence[int], n_tokens: Sequence[int], q, k, v,
+                  q_norm=None, k_norm=None, eps: float = 1e-6, q_out=None, dtype: int = F32,
+                  q_stride: int = 0, k_stride: int = 0, v_stride: int = 0, q_out_stride: int = 0,
+                  stream=None) -> None:
+        """hkv_qkv_write: norm (optional) and rotation of q and k heads, K/V rows of several
+        slots into the cache, q to q_out.  Strides in elements, 0 for packed rows."""
+        n, arr = _slots_arg(slots)
+        a = QkvWriteArgs(layer, n, arr, _counts_arg(n_tokens, n), dtype, eps, _ptr(q), _ptr(k),
+                         _ptr(v), q_stride, k_stride, v_stride, q_out_stride, _ptr(q_norm),
+                         _ptr(k_norm), _ptr(q_out))
+        self._check(self.lib.hkv_qkv_write(self.handle, ctypes.byref(a), _stream(stream)))
+
+    def cache_read(self, layer: int, slots: Sequence[int], pos0: Sequence[int],
+                   n_rows: Sequence[int], k_out, v_out, dtype: int = F16, stream=None) -> None:
+        """hkv_cache_read: rows of several slots as F16 or F32 values, packed."""
+        n, arr = _slots_arg(slots)
+        self._check(self.lib.hkv_cache_read(self.handle, layer, n, arr, _counts_arg(pos0, n),
+                                            _counts_arg(n_rows, n), dtype, _ptr(k_out),
+                                            _ptr(v_out), _stream(stream)))
 
     def sync_check(self, stream=None) -> None:
         self._check(self.lib.hkv_sync_check(self.handle, _stream(stream)))

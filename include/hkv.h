@@ -9,7 +9,8 @@
  *
  * Storage model: one page pool per engine (per GPU).  A page holds 16
  * consecutive token positions of one slot for ALL layers (one block in each
- * layer's slab), K and V, all KV heads, in F16.  Each live slot owns a page list; pages are reference
+ * layer's slab), K and V, all KV heads, in F16 (or in 8 bits, see
+ * hkv_engine_create_cache).  Each live slot owns a page list; pages are reference
  * counted so slots can share a prefix (fork / published prefixes) and are
  * copied on the first write into a shared page (copy-on-write).
  *
@@ -135,6 +136,30 @@ const char *hkv_last_error(const hkv_engine *eng);
 const char *hkv_status_string(int status);
 int hkv_abi_version(void);
 
+/* ------------------------------------------------------- 8-bit cache -- */
+
+/* How an engine holds K and V.  HKV_CACHE_E4M3: 8 bits a value, one power of two
+ * for each block, a block being the 16 rows of one page, one KV head, K or V.  A
+ * value is code * 2^e with an E4M3 code; e is the least integer (at least -100)
+ * for which the block's largest finite value is at most 448 * 2^e.  Codes are
+ * rounded to nearest, ties to even: the error is at most 2^-4 of a value of at
+ * least 2^(e-6), and at most 2^(e-10) below that.  A value that is not finite is
+ * stored as NaN and leaves e alone.  As rows join a page, e only grows; the rows
+ * already there are then rounded once more.  A write to the first row of a page
+ * starts its blocks anew: the page's other rows are undefined until written. */
+typedef enum hkv_cache_type { HKV_CACHE_F16 = 0, HKV_CACHE_E4M3 = 1 } hkv_cache_type;
+
+/* hkv_engine_create with the cache format chosen (hkv_engine_create: F16).  Every
+ * slot, prefix and compute call of this header works on both; the KV-head split
+ * (hkv_split_*) and hkv_decode_attn_noalloc take F16 only.  On an E4M3 engine the
+ * appends quantise their rows, attention reads the codes, and hkv_gather returns
+ * the values the codes stand for, rounded to F16. */
+int hkv_engine_create_cache(const hkv_config *cfg, int32_t cache_type, hkv_engine **out);
+int hkv_engine_cache_type(const hkv_engine *eng, int32_t *out);
+
+/* Element types of hkv_qkv_write and hkv_cache_read. */
+typedef enum hkv_dtype { HKV_F32 = 0, HKV_F16 = 1, HKV_BF16 = 2 } hkv_dtype;
+
 /* ------------------------------------------------------------- slots -- */
 
 /* Rents a slot.  Replaces acquire_backend_kv_cache_slot (:1191-1208).
@@ -222,6 +247,39 @@ int hkv_decode_step(hkv_engine *eng, int32_t layer, int32_t n, const int32_t *sl
  * cache (:6980-6981).  k_out, v_out: device pointers. */
 int hkv_gather(hkv_engine *eng, int32_t slot, int32_t layer, int64_t pos0, int64_t n,
                uint16_t *k_out, uint16_t *v_out, hkv_stream stream);
+
+/* Rows of several slots into one layer's cache in one launch, with what comes
+ * before them: slot e takes n_tokens[e] rows at positions [used, used +
+ * n_tokens[e]) (0: none), the rows of all slots back to back in q, k, v and q_out.
+ * Each head of q and k is first normed where its weight is given,
+ *     y = x / sqrt(mean(x^2) + eps) * w        (:5727-5733),
+ * then rotated (NEOX, at its position); k and v go into the cache, q to q_out.
+ * Sums are F32; q_out is rounded once, to dtype.  For prompts, windows and batches of
+ * decode tokens whose projections are not hkv_q4k_qkv's; hkv_window_attn and
+ * a later hkv_slot_advance follow it as after hkv_rope_append_range.  Strides are in
+ * elements, 0 for packed rows, so q, k and v may lie side by side in one
+ * projection's output; each is a multiple of 16 bytes.  q_out may be q. */
+typedef struct hkv_qkv_write_args {
+    int32_t layer;
+    int32_t n;                /* slots, each at most once                       */
+    const int32_t *slots;     /* host [n]                                       */
+    const int64_t *n_tokens;  /* host [n]                                       */
+    int32_t dtype;            /* hkv_dtype of q, k, v and q_out                 */
+    float eps;
+    const void *q;            /* NULL or [rows][n_head][128]                    */
+    const void *k, *v;        /* [rows][n_head_kv][128]                         */
+    int64_t q_stride, k_stride, v_stride, q_out_stride;
+    const float *q_norm;      /* NULL or [128]                                  */
+    const float *k_norm;      /* NULL or [128]                                  */
+    void *q_out;              /* with q: [rows][n_head][128]                    */
+} hkv_qkv_write_args;
+int hkv_qkv_write(hkv_engine *eng, const hkv_qkv_write_args *args, hkv_stream stream);
+
+/* Rows [pos0[e], pos0[e] + n_rows[e]) of each slot as values (dtype F32, exact, or
+ * F16, rounded; from either cache format), the rows of all slots back to back in
+ * k_out and v_out [rows][n_head_kv][128]. */
+int hkv_cache_read(hkv_engine *eng, int32_t layer, int32_t n, const int32_t *slots, const int64_t *pos0,
+                   const int64_t *n_rows, int32_t dtype, void *k_out, void *v_out, hkv_stream stream);
 
 /* Waits for the engine's stream work, then reports a device-side error
  * (HKV_ERR_DEVICE / HKV_ERR_TIMEOUT) recorded by a kernel since the last
