@@ -253,6 +253,20 @@ struct RowCache {
     cudaStream_t consumer_stream = nullptr;
 };
 
+// Descriptor of a window attention call, kept like RowCache.
+struct WindowCache {
+    bool valid = false;
+    uint64_t epoch = 0;
+    std::vector<int32_t> slots;
+    std::vector<int64_t> begin;
+    std::vector<int64_t> count;
+    const WindowTile *tiles = nullptr;
+    const int32_t *pages = nullptr;
+    int32_t n_tiles = 0;
+    bool consumed = false;
+    cudaStream_t consumer_stream = nullptr;
+};
+
 struct ProfileRecord {
     cudaEvent_t start;
     cudaEvent_t stop;
@@ -293,8 +307,9 @@ struct hkv_engine {
     int64_t part_cap = 0;
     int num_sms = 0;
     float scale_log2 = 0.f;
-    hkv::Staging batch_stage, range_stage, gather_stage, cow_stage, write_stage, read_stage;
+    hkv::Staging batch_stage, range_stage, gather_stage, cow_stage, write_stage, read_stage, window_stage;
     hkv::RowCache write_rows, read_rows;
+    hkv::WindowCache window;
     // Copy-on-write copies decided on the host and not yet enqueued:
     // {source page, destination page} pairs, flushed as one kernel launch.
     std::vector<int32_t> cow_pending;
@@ -746,7 +761,8 @@ RowItem *put_row_items(RowItem *out, const std::vector<int32_t> &pages, int64_t 
     return out;
 }
 
-bool row_cache_matches(const hkv_engine *eng, const RowCache &rc, int32_t n, const int32_t *slots,
+template <class Cache>
+bool row_cache_matches(const hkv_engine *eng, const Cache &rc, int32_t n, const int32_t *slots,
                        const int64_t *begin, const int64_t *count) {
     if (!rc.valid || rc.epoch != eng->epoch || static_cast<int32_t>(rc.slots.size()) != n) {
         return false;
@@ -792,6 +808,57 @@ int upload_rows(hkv_engine *eng, Staging &stage, RowCache &rc, int32_t n, const 
     rc.count.assign(count, count + n);
     rc.epoch = eng->epoch;
     rc.valid = true;
+    return HKV_OK;
+}
+
+// Uploads the tiles and page lists of a window attention call.
+int upload_window(hkv_engine *eng, int32_t n, const int32_t *slots, const int64_t *begin,
+                  const int64_t *count, cudaStream_t stream) {
+    WindowCache &wc = eng->window;
+    wc.valid = false;
+    std::vector<WindowTile> tiles;
+    std::vector<int32_t> pages;
+    int64_t row0 = 0;
+    for (int32_t e = 0; e < n; ++e) {
+        for (int64_t i = 0; i < count[e]; i += kWindowTokens) {
+            WindowTile t;
+            t.row0 = static_cast<int32_t>(row0 + i);
+            t.tokens = static_cast<int32_t>(std::min<int64_t>(kWindowTokens, count[e] - i));
+            t.pos0 = static_cast<int32_t>(begin[e] + i);
+            t.page_off = static_cast<int32_t>(pages.size());
+            tiles.push_back(t);
+        }
+        if (count[e] > 0) {
+            const std::vector<int32_t> &list = eng->slots[slots[e]].pages;
+            pages.insert(pages.end(), list.begin(), list.begin() + pages_for(begin[e] + count[e]));
+        }
+        row0 += count[e];
+    }
+    // the longest tiles first: they bound the launch's end
+    std::stable_sort(tiles.begin(), tiles.end(), [](const WindowTile &a, const WindowTile &b) {
+        return a.pos0 + a.tokens > b.pos0 + b.tokens;
+    });
+    if (wc.consumed) {
+        HKV_CUDA_TRY(eng, eng->window_stage.mark_used(wc.consumer_stream));
+        wc.consumed = false;
+    }
+    const size_t tile_bytes = tiles.size() * sizeof(WindowTile);
+    const size_t bytes = tile_bytes + pages.size() * sizeof(int32_t);
+    void *host = nullptr;
+    HKV_CUDA_TRY(eng, eng->window_stage.begin(bytes, &host));
+    std::memcpy(host, tiles.data(), tile_bytes);
+    std::memcpy(static_cast<uint8_t *>(host) + tile_bytes, pages.data(), pages.size() * sizeof(int32_t));
+    void *dev = nullptr;
+    ++eng->enqueue_seq;
+    HKV_CUDA_TRY(eng, eng->window_stage.commit(bytes, stream, &dev));
+    wc.tiles = static_cast<const WindowTile *>(dev);
+    wc.pages = reinterpret_cast<const int32_t *>(static_cast<const uint8_t *>(dev) + tile_bytes);
+    wc.n_tiles = static_cast<int32_t>(tiles.size());
+    wc.slots.assign(slots, slots + n);
+    wc.begin.assign(begin, begin + n);
+    wc.count.assign(count, count + n);
+    wc.epoch = eng->epoch;
+    wc.valid = true;
     return HKV_OK;
 }
 
@@ -930,6 +997,7 @@ void free_device(hkv_engine *eng) {
     eng->gather_stage.release();
     eng->write_stage.release();
     eng->read_stage.release();
+    eng->window_stage.release();
     eng->cow_stage.release();
     for (auto &list : eng->prof) {
         for (auto &r : list) {
@@ -1649,6 +1717,72 @@ int hkv_qkv_write(hkv_engine *eng, const hkv_qkv_write_args *args, hkv_stream st
     rc.consumed = true;
     rc.consumer_stream = stream;
     return launch_status(eng, "write kernel launch");
+}
+
+int hkv_window_attn(hkv_engine *eng, const hkv_window_attn_args *args, hkv_stream stream_h) {
+    if (eng == nullptr) return HKV_ERR_INVALID;
+    std::lock_guard<std::mutex> lock(eng->mu);
+    if (args == nullptr) {
+        return fail(eng, HKV_ERR_INVALID, "null arguments");
+    }
+    const hkv_window_attn_args &a = *args;
+    DeviceGuard guard(eng->cfg.device);
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_h);
+    int64_t total = 0;
+    int st = check_row_slots(eng, a.n, a.slots, a.n_tokens, &total);
+    if (st != HKV_OK) return st;
+    if (a.dtype != HKV_F32 && a.dtype != HKV_F16 && a.dtype != HKV_BF16) {
+        return fail(eng, HKV_ERR_INVALID, "dtype %d", a.dtype);
+    }
+    if (a.q == nullptr || a.out == nullptr || !aligned16(a.q) || !aligned16(a.out)) {
+        return fail(eng, HKV_ERR_INVALID, "q and out must be non-null 16-byte aligned device pointers");
+    }
+    WindowArgs w{};
+    w.layer = a.layer;
+    w.dtype = a.dtype;
+    w.q = a.q;
+    w.out = a.out;
+    w.q_stride = a.q_stride;
+    w.out_stride = a.out_stride;
+    w.scale_log2 = eng->scale_log2;
+    const int64_t row = static_cast<int64_t>(eng->cfg.n_head) * kHeadDim;
+    st = check_stride(eng, "q", row, a.dtype, &w.q_stride);
+    if (st == HKV_OK) st = check_stride(eng, "out", row, a.dtype, &w.out_stride);
+    if (st != HKV_OK) return st;
+    std::vector<int64_t> begin(static_cast<size_t>(a.n));
+    for (int32_t e = 0; e < a.n; ++e) {
+        const Slot &s = eng->slots[a.slots[e]];
+        begin[e] = s.used;
+        if (begin[e] + a.n_tokens[e] > static_cast<int64_t>(s.pages.size()) * kPageTokens ||
+            begin[e] + a.n_tokens[e] > eng->cfg.context_length) {
+            return fail(eng, HKV_ERR_RANGE, "slot %d: rows [%lld, %lld) are not written", a.slots[e],
+                        static_cast<long long>(begin[e]), static_cast<long long>(begin[e] + a.n_tokens[e]));
+        }
+    }
+    st = check_compute(eng, a.layer);
+    if (st != HKV_OK) return st;
+    st = refuse_capture(eng, stream);
+    if (st != HKV_OK) return st;
+    if (total == 0) {
+        return HKV_OK;
+    }
+    WindowCache &wc = eng->window;
+    if (!row_cache_matches(eng, wc, a.n, a.slots, begin.data(), a.n_tokens)) {
+        st = upload_window(eng, a.n, a.slots, begin.data(), a.n_tokens, stream);
+        if (st != HKV_OK) return st;
+    }
+    ++eng->enqueue_seq;
+    w.tiles = wc.tiles;
+    w.pages = wc.pages;
+    w.n_tiles = wc.n_tiles;
+    {
+        ProfileScope ps(eng, HKV_KERNEL_ATTN, stream);
+        launch_window(pool_view(eng), w, eng->d_err, stream);
+        ++eng->kernel_launches;
+    }
+    wc.consumed = true;
+    wc.consumer_stream = stream;
+    return launch_status(eng, "window attention launch");
 }
 
 int hkv_cache_read(hkv_engine *eng, int32_t layer, int32_t n, const int32_t *slots, const int64_t *pos0,

@@ -229,6 +229,27 @@ struct WriteArgs {
 };
 void launch_write(const PoolView &pool, const RopeView &rope, const BatchView &batch,
                   const WriteArgs &args, DeviceError *err, cudaStream_t stream);
+// Up to kWindowTokens consecutive query tokens of one slot (hkv_window.cu).
+constexpr int kWindowTokens = 64;
+struct WindowTile {
+    int32_t row0;      // packed row of the first
+    int32_t tokens;
+    int32_t pos0;      // its position: token i sees keys [0, pos0 + i]
+    int32_t page_off;  // the slot's page list in `pages`
+};
+struct WindowArgs {
+    const WindowTile *tiles;
+    const int32_t *pages;
+    int32_t n_tiles;
+    int32_t layer;
+    int32_t dtype;
+    const void *q;
+    void *out;
+    int64_t q_stride, out_stride;  // elements per row
+    float scale_log2;
+};
+void launch_window(const PoolView &pool, const WindowArgs &args, DeviceError *err, cudaStream_t stream);
+
 // Cached rows as values, F16 or F32 (dtype): [rows][n_head_kv][128] each.
 void launch_read(const PoolView &pool, const RowItem *items, int32_t n_items, int layer, int dtype,
                  void *k_out, void *v_out, DeviceError *err, cudaStream_t stream);

@@ -108,6 +108,15 @@ class QkvWriteArgs(ctypes.Structure):
                 ("q_out", ctypes.c_void_p)]
 
 
+class WindowAttnArgs(ctypes.Structure):
+    """hkv_window_attn_args."""
+    _fields_ = [("layer", ctypes.c_int32), ("n", ctypes.c_int32),
+                ("slots", ctypes.POINTER(ctypes.c_int32)),
+                ("n_tokens", ctypes.POINTER(ctypes.c_int64)), ("dtype", ctypes.c_int32),
+                ("q", ctypes.c_void_p), ("out", ctypes.c_void_p), ("q_stride", ctypes.c_int64),
+                ("out_stride", ctypes.c_int64)]
+
+
 class PagedView(ctypes.Structure):
     """hkv_paged_view: caller-owned device memory in the engine's page layout."""
     _fields_ = [
@@ -188,6 +197,7 @@ SIGNATURES = {
     "hkv_decode_step": ([_P, _I32, _I32, _I32P, _P, _P, _P, _P, _P], ctypes.c_int),
     "hkv_gather": ([_P, _I32, _I32, _I64, _I64, _P, _P, _P], ctypes.c_int),
     "hkv_qkv_write": ([_P, ctypes.POINTER(QkvWriteArgs), _P], ctypes.c_int),
+    "hkv_window_attn": ([_P, ctypes.POINTER(WindowAttnArgs), _P], ctypes.c_int),
     "hkv_cache_read": ([_P, _I32, _I32, _I32P, _I64P, _I64P, _I32, _P, _P, _P], ctypes.c_int),
     "hkv_sync_check": ([_P, _P], ctypes.c_int),
     "hkv_rope_tables": ([_P, _P, _P], ctypes.c_int),
@@ -454,6 +464,14 @@ class Engine:
                          _ptr(v), q_stride, k_stride, v_stride, q_out_stride, _ptr(q_norm),
                          _ptr(k_norm), _ptr(q_out))
         self._check(self.lib.hkv_qkv_write(self.handle, ctypes.byref(a), _stream(stream)))
+
+    def window_attn(self, layer: int, slots: Sequence[int], n_tokens: Sequence[int], q, out,
+                    dtype: int = F32, q_stride: int = 0, out_stride: int = 0, stream=None) -> None:
+        """hkv_window_attn: token i of each slot over its rows [0, used + i]; q rotated."""
+        n, arr = _slots_arg(slots)
+        a = WindowAttnArgs(layer, n, arr, _counts_arg(n_tokens, n), dtype, _ptr(q), _ptr(out),
+                           q_stride, out_stride)
+        self._check(self.lib.hkv_window_attn(self.handle, ctypes.byref(a), _stream(stream)))
 
     def cache_read(self, layer: int, slots: Sequence[int], pos0: Sequence[int],
                    n_rows: Sequence[int], k_out, v_out, dtype: int = F16, stream=None) -> None:

@@ -157,7 +157,7 @@ typedef enum hkv_cache_type { HKV_CACHE_F16 = 0, HKV_CACHE_E4M3 = 1 } hkv_cache_
 int hkv_engine_create_cache(const hkv_config *cfg, int32_t cache_type, hkv_engine **out);
 int hkv_engine_cache_type(const hkv_engine *eng, int32_t *out);
 
-/* Element types of hkv_qkv_write and hkv_cache_read. */
+/* Element types of hkv_qkv_write, hkv_window_attn and hkv_cache_read. */
 typedef enum hkv_dtype { HKV_F32 = 0, HKV_F16 = 1, HKV_BF16 = 2 } hkv_dtype;
 
 /* ------------------------------------------------------------- slots -- */
@@ -274,6 +274,28 @@ typedef struct hkv_qkv_write_args {
     void *q_out;              /* with q: [rows][n_head][128]                    */
 } hkv_qkv_write_args;
 int hkv_qkv_write(hkv_engine *eng, const hkv_qkv_write_args *args, hkv_stream stream);
+
+/* GQA attention of several new tokens per slot, for one layer: token i of slot e
+ * sees rows [0, used + i], i < n_tokens[e] (0: none), all of them written (by
+ * hkv_qkv_write or hkv_rope_append_range at this `used`; hkv_slot_advance comes after
+ * the last layer).  The many-token form of hkv_decode_attn: prompts and refreshed
+ * windows (:6278-6279, :6603-6604).  q: [rows][n_head][128], rotated already
+ * (hkv_qkv_write's q_out); out: [rows][n_head * 128]; both of dtype, the rows of all
+ * slots back to back, strides in elements (0: packed), each a multiple of 16 bytes.
+ * Softmax statistics and sums are F32.  With F32 tensors q and the weights enter the
+ * products in two F16 parts (22 bits, as in hkv_decode_attn; |q| up to 65504); with
+ * F16 or BF16 ones q as it is and the weights rounded to F16. */
+typedef struct hkv_window_attn_args {
+    int32_t layer;
+    int32_t n;                /* slots, each at most once */
+    const int32_t *slots;     /* host [n]                 */
+    const int64_t *n_tokens;  /* host [n]                 */
+    int32_t dtype;            /* hkv_dtype of q and out   */
+    const void *q;
+    void *out;
+    int64_t q_stride, out_stride;
+} hkv_window_attn_args;
+int hkv_window_attn(hkv_engine *eng, const hkv_window_attn_args *args, hkv_stream stream);
 
 /* Rows [pos0[e], pos0[e] + n_rows[e]) of each slot as values (dtype F32, exact, or
  * F16, rounded; from either cache format), the rows of all slots back to back in

@@ -97,6 +97,24 @@ def test_cache_read_refusals(eng):
     refused(eng, hkv.HKV_ERR_NO_DEVICE, r, 0, [s], [0], [0], 16, 16)
 
 
+def test_window_attn_refusals(eng):
+    import hkv
+    s = eng.acquire(0)
+    inv = hkv.HKV_ERR_INVALID
+    w = eng.window_attn
+    refused(eng, inv, w, 0, [], [], 16, 16)
+    refused(eng, hkv.HKV_ERR_BAD_SLOT, w, 0, [5], [1], 16, 16)
+    refused(eng, inv, w, 0, [s, s], [0, 0], 16, 16)
+    refused(eng, hkv.HKV_ERR_RANGE, w, 0, [s], [-2], 16, 16)
+    refused(eng, hkv.HKV_ERR_RANGE, w, 0, [s], [1], 16, 16)        # no row written
+    refused(eng, inv, w, 0, [s], [0], None, 16)
+    refused(eng, inv, w, 0, [s], [0], 16, 8)
+    refused(eng, inv, w, 0, [s], [0], 16, 16, dtype=7)
+    refused(eng, inv, w, 0, [s], [0], 16, 16, q_stride=4095)
+    refused(eng, inv, w, 0, [s], [0], 16, 16, out_stride=4098)
+    refused(eng, hkv.HKV_ERR_NO_DEVICE, w, 0, [s], [0], 16, 16)
+
+
 def test_the_model_rounds_as_e4m3_does():
     """The model's own rounding against torch's E4M3 type over the whole range."""
     torch = pytest.importorskip("torch")
