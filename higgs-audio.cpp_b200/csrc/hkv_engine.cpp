@@ -261,8 +261,10 @@ struct WindowCache {
     std::vector<int64_t> begin;
     std::vector<int64_t> count;
     const WindowTile *tiles = nullptr;
+    const WindowMerge *merges = nullptr;
     const int32_t *pages = nullptr;
     int32_t n_tiles = 0;
+    int32_t n_merges = 0;
     bool consumed = false;
     cudaStream_t consumer_stream = nullptr;
 };
@@ -310,6 +312,8 @@ struct hkv_engine {
     hkv::Staging batch_stage, range_stage, gather_stage, cow_stage, write_stage, read_stage, window_stage;
     hkv::RowCache write_rows, read_rows;
     hkv::WindowCache window;
+    float *window_work = nullptr;   // parts of split window tiles, grown on demand
+    int64_t window_work_parts = 0;
     // Copy-on-write copies decided on the host and not yet enqueued:
     // {source page, destination page} pairs, flushed as one kernel launch.
     std::vector<int32_t> cow_pending;
@@ -811,22 +815,54 @@ int upload_rows(hkv_engine *eng, Staging &stage, RowCache &rc, int32_t n, const 
     return HKV_OK;
 }
 
+// The most key blocks one CTA of a window attention takes: enough CTAs for the GPU
+// where the tiles alone are too few, and no part shorter than two blocks (a CTA
+// costs about two blocks to start and join).
+int64_t window_split(int64_t total_blocks, int64_t n_head_kv, int64_t sms) {
+    return std::max<int64_t>(2, (total_blocks * n_head_kv + sms - 1) / sms);
+}
+
 // Uploads the tiles and page lists of a window attention call.
 int upload_window(hkv_engine *eng, int32_t n, const int32_t *slots, const int64_t *begin,
                   const int64_t *count, cudaStream_t stream) {
     WindowCache &wc = eng->window;
     wc.valid = false;
     std::vector<WindowTile> tiles;
+    std::vector<WindowMerge> merges;
     std::vector<int32_t> pages;
-    int64_t row0 = 0;
+    const int64_t G = eng->cfg.n_head_kv;
+    auto blocks_of = [&](int32_t e, int64_t i) {
+        const int64_t last = begin[e] + std::min<int64_t>(i + kWindowTokens, count[e]);
+        return (last + kWindowKeys - 1) / kWindowKeys;
+    };
+    int64_t total = 0;
     for (int32_t e = 0; e < n; ++e) {
         for (int64_t i = 0; i < count[e]; i += kWindowTokens) {
-            WindowTile t;
+            total += blocks_of(e, i);
+        }
+    }
+    const int64_t most = window_split(total, G, eng->num_sms);
+    int64_t row0 = 0;
+    int32_t parts = 0;
+    for (int32_t e = 0; e < n; ++e) {
+        for (int64_t i = 0; i < count[e]; i += kWindowTokens) {
+            WindowTile t{};
             t.row0 = static_cast<int32_t>(row0 + i);
             t.tokens = static_cast<int32_t>(std::min<int64_t>(kWindowTokens, count[e] - i));
             t.pos0 = static_cast<int32_t>(begin[e] + i);
             t.page_off = static_cast<int32_t>(pages.size());
-            tiles.push_back(t);
+            const int64_t blocks = blocks_of(e, i);
+            const int64_t cuts = (blocks + most - 1) / most;
+            if (cuts > 1) {
+                merges.push_back({t.row0, t.tokens, parts, static_cast<int32_t>(cuts)});
+            }
+            for (int64_t c = 0; c < cuts; ++c) {
+                const int64_t b0 = c * blocks / cuts;
+                t.key0 = static_cast<int32_t>(b0 * kWindowKeys);
+                t.blocks = static_cast<int32_t>((c + 1) * blocks / cuts - b0);
+                t.part = cuts > 1 ? parts++ : -1;
+                tiles.push_back(t);
+            }
         }
         if (count[e] > 0) {
             const std::vector<int32_t> &list = eng->slots[slots[e]].pages;
@@ -834,26 +870,41 @@ int upload_window(hkv_engine *eng, int32_t n, const int32_t *slots, const int64_
         }
         row0 += count[e];
     }
-    // the longest tiles first: they bound the launch's end
-    std::stable_sort(tiles.begin(), tiles.end(), [](const WindowTile &a, const WindowTile &b) {
-        return a.pos0 + a.tokens > b.pos0 + b.tokens;
-    });
+    if (parts > eng->window_work_parts) {
+        cudaFree(eng->window_work);  // waits for the kernels that use it
+        eng->window_work = nullptr;
+        eng->window_work_parts = 0;
+        HKV_CUDA_TRY(eng, cudaMalloc(&eng->window_work,
+                                     static_cast<size_t>(parts) * G * kWindowPartFloats * sizeof(float)));
+        eng->window_work_parts = parts;
+    }
+    // the longest runs first: they bound the launch's end
+    std::stable_sort(tiles.begin(), tiles.end(),
+                     [](const WindowTile &a, const WindowTile &b) { return a.blocks > b.blocks; });
     if (wc.consumed) {
         HKV_CUDA_TRY(eng, eng->window_stage.mark_used(wc.consumer_stream));
         wc.consumed = false;
     }
     const size_t tile_bytes = tiles.size() * sizeof(WindowTile);
-    const size_t bytes = tile_bytes + pages.size() * sizeof(int32_t);
+    const size_t merge_bytes = merges.size() * sizeof(WindowMerge);
+    const size_t bytes = tile_bytes + merge_bytes + pages.size() * sizeof(int32_t);
     void *host = nullptr;
     HKV_CUDA_TRY(eng, eng->window_stage.begin(bytes, &host));
-    std::memcpy(host, tiles.data(), tile_bytes);
-    std::memcpy(static_cast<uint8_t *>(host) + tile_bytes, pages.data(), pages.size() * sizeof(int32_t));
+    uint8_t *put = static_cast<uint8_t *>(host);
+    std::memcpy(put, tiles.data(), tile_bytes);
+    if (merge_bytes > 0) {
+        std::memcpy(put + tile_bytes, merges.data(), merge_bytes);
+    }
+    std::memcpy(put + tile_bytes + merge_bytes, pages.data(), pages.size() * sizeof(int32_t));
     void *dev = nullptr;
     ++eng->enqueue_seq;
     HKV_CUDA_TRY(eng, eng->window_stage.commit(bytes, stream, &dev));
-    wc.tiles = static_cast<const WindowTile *>(dev);
-    wc.pages = reinterpret_cast<const int32_t *>(static_cast<const uint8_t *>(dev) + tile_bytes);
+    const uint8_t *got = static_cast<const uint8_t *>(dev);
+    wc.tiles = reinterpret_cast<const WindowTile *>(got);
+    wc.merges = reinterpret_cast<const WindowMerge *>(got + tile_bytes);
+    wc.pages = reinterpret_cast<const int32_t *>(got + tile_bytes + merge_bytes);
     wc.n_tiles = static_cast<int32_t>(tiles.size());
+    wc.n_merges = static_cast<int32_t>(merges.size());
     wc.slots.assign(slots, slots + n);
     wc.begin.assign(begin, begin + n);
     wc.count.assign(count, count + n);
@@ -1017,6 +1068,8 @@ void free_device(hkv_engine *eng) {
     cudaFree(eng->part_o);
     cudaFree(eng->part_ml);
     cudaFree(eng->counters);
+    cudaFree(eng->window_work);
+    eng->window_work = nullptr;
     eng->pool = nullptr;
     eng->d_cos = eng->d_sin = nullptr;
     eng->d_err = nullptr;
@@ -1775,10 +1828,13 @@ int hkv_window_attn(hkv_engine *eng, const hkv_window_attn_args *args, hkv_strea
     w.tiles = wc.tiles;
     w.pages = wc.pages;
     w.n_tiles = wc.n_tiles;
+    w.merges = wc.merges;
+    w.n_merges = wc.n_merges;
+    w.work = eng->window_work;
     {
         ProfileScope ps(eng, HKV_KERNEL_ATTN, stream);
         launch_window(pool_view(eng), w, eng->d_err, stream);
-        ++eng->kernel_launches;
+        eng->kernel_launches += wc.n_merges > 0 ? 2 : 1;
     }
     wc.consumed = true;
     wc.consumer_stream = stream;

@@ -236,11 +236,28 @@ struct WindowTile {
     int32_t tokens;
     int32_t pos0;      // its position: token i sees keys [0, pos0 + i]
     int32_t page_off;  // the slot's page list in `pages`
+    int32_t key0;      // the first key this CTA takes, a multiple of kWindowKeys
+    int32_t blocks;    // blocks of kWindowKeys keys from there
+    int32_t part;      // -1: all keys, the output; else the part its result goes to
+    int32_t unused;
 };
+constexpr int kWindowKeys = 128;
+// A tile whose keys were split: its parts, joined by the launch that follows.
+struct WindowMerge {
+    int32_t row0;
+    int32_t tokens;
+    int32_t part0;
+    int32_t parts;
+};
+// A part per (tile, KV head): o [256 rows][128], then (m, l) [256].
+constexpr int64_t kWindowPartFloats = kWindowTokens * kGqa * (kHeadDim + 2);
 struct WindowArgs {
     const WindowTile *tiles;
     const int32_t *pages;
+    const WindowMerge *merges;
+    float *work;
     int32_t n_tiles;
+    int32_t n_merges;
     int32_t layer;
     int32_t dtype;
     const void *q;

@@ -23,6 +23,7 @@ LIB = LIB_DIR / "libhkv.so"
 SOURCES = [CSRC / "hkv_kernels.cu", CSRC / "hkv_engine.cpp", CSRC / "hkv_noalloc.cu",
            CSRC / "hkv_backbone.cu", CSRC / "hkv_cache.cu", CSRC / "hkv_window.cu"]
 HEADERS = [CSRC / "hkv_internal.h", CSRC / "hkv_plan.h", CSRC / "hkv_device.cuh", CSRC / "hkv_e4m3.cuh",
+           CSRC / "hkv_tcgen05.cuh",
            REPO / "include" / "hkv.h"]
 
 NVCC_FLAGS = [
