@@ -249,6 +249,7 @@ struct RowCache {
     std::vector<int64_t> count;
     const RowItem *items = nullptr;
     int32_t n_items = 0;
+    bool one_row = false;  // every item has one row
     bool consumed = false;
     cudaStream_t consumer_stream = nullptr;
 };
@@ -742,6 +743,7 @@ WriteArgs kv_write_args(const RowItem *items, int32_t n_items, int32_t layer, in
     a.k_stride = k_stride;
     a.v_stride = v_stride;
     a.rope = rope;
+    a.one_row = items == nullptr;
     return a;
 }
 
@@ -807,6 +809,7 @@ int upload_rows(hkv_engine *eng, Staging &stage, RowCache &rc, int32_t n, const 
     HKV_CUDA_TRY(eng, stage.commit(bytes, stream, &dev));
     rc.items = static_cast<const RowItem *>(dev);
     rc.n_items = static_cast<int32_t>(n_items);
+    rc.one_row = n_items == row0;
     rc.slots.assign(slots, slots + n);
     rc.begin.assign(begin, begin + n);
     rc.count.assign(count, count + n);
@@ -965,6 +968,45 @@ int check_stride(hkv_engine *eng, const char *name, int64_t row, int32_t dtype, 
                     static_cast<long long>(*stride), static_cast<long long>(row));
     }
     return HKV_OK;
+}
+
+// Owns rows [begin[e], begin[e] + count[e]) of every slot (checked: live, none
+// twice, within the context; total > 0) and writes them.
+int write_rows(hkv_engine *eng, WriteArgs w, int32_t n, const int32_t *slots, const int64_t *begin,
+               const int64_t *count, cudaStream_t stream) {
+    int st = HKV_OK;
+    RowCache &rc = eng->write_rows;
+    if (!row_cache_matches(eng, rc, n, slots, begin, count)) {
+        int64_t extra = 0;
+        for (int32_t e = 0; e < n; ++e) {
+            const Slot &s = eng->slots[slots[e]];
+            extra += pages_beyond_reservation(s, pages_needed(eng, s, begin[e], begin[e] + count[e]));
+        }
+        if (extra > unreserved_free(eng)) {
+            return fail(eng, HKV_ERR_OOM, "rows need %lld unreserved pages, %lld free",
+                        static_cast<long long>(extra), static_cast<long long>(unreserved_free(eng)));
+        }
+        for (int32_t e = 0; e < n; ++e) {
+            st = own_rows(eng, eng->slots[slots[e]], begin[e], begin[e] + count[e], stream);
+            if (st != HKV_OK) return st;
+        }
+        st = flush_cow(eng, stream);
+        if (st != HKV_OK) return st;
+        st = upload_rows(eng, eng->write_stage, rc, n, slots, begin, count, stream);
+        if (st != HKV_OK) return st;
+    }
+    ++eng->enqueue_seq;
+    w.items = rc.items;
+    w.n_items = rc.n_items;
+    w.one_row = rc.one_row;
+    {
+        ProfileScope ps(eng, HKV_KERNEL_APPEND, stream);
+        launch_write(pool_view(eng), rope_view(eng), BatchView{}, w, eng->d_err, stream);
+        ++eng->kernel_launches;
+    }
+    rc.consumed = true;
+    rc.consumer_stream = stream;
+    return launch_status(eng, "write kernel launch");
 }
 
 int do_append(hkv_engine *eng, int32_t layer, int32_t n, const int32_t *slots, const float *k,
@@ -1549,6 +1591,11 @@ int hkv_rope_append_range(hkv_engine *eng, int32_t layer, int32_t slot, int64_t 
     }
     const int64_t begin = s.used;
     const int64_t end = s.used + n_tokens;
+    if (eng->cache_type == HKV_CACHE_E4M3) {
+        const int64_t row = static_cast<int64_t>(eng->cfg.n_head_kv) * kHeadDim;
+        return write_rows(eng, kv_write_args(nullptr, 0, layer, HKV_F32, k_prerope, v, row, row, true), 1, &slot,
+                          &begin, &n_tokens, stream);
+    }
     const int64_t extra = pages_beyond_reservation(s, pages_needed(eng, s, begin, end));
     if (extra > unreserved_free(eng)) {
         return fail(eng, HKV_ERR_OOM, "range needs %lld unreserved pages, %lld free",
@@ -1561,30 +1608,16 @@ int hkv_rope_append_range(hkv_engine *eng, int32_t layer, int32_t slot, int64_t 
     const int64_t p0 = begin / kPageTokens;
     const int64_t p1 = (end - 1) / kPageTokens + 1;
     void *host = nullptr;
-    const bool e4m3 = eng->cache_type == HKV_CACHE_E4M3;
-    const size_t bytes = static_cast<size_t>(p1 - p0) * (e4m3 ? sizeof(RowItem) : sizeof(int32_t));
+    const size_t bytes = static_cast<size_t>(p1 - p0) * sizeof(int32_t);
     HKV_CUDA_TRY(eng, eng->range_stage.begin(bytes, &host));
-    if (e4m3) {
-        put_row_items(static_cast<RowItem *>(host), s.pages, begin, n_tokens, 0);
-    } else {
-        std::memcpy(host, s.pages.data() + p0, bytes);
-    }
+    std::memcpy(host, s.pages.data() + p0, bytes);
     void *dev = nullptr;
     ++eng->enqueue_seq;
     HKV_CUDA_TRY(eng, eng->range_stage.commit(bytes, stream, &dev));
     {
         ProfileScope ps(eng, HKV_KERNEL_APPEND, stream);
-        if (e4m3) {
-            const int64_t row = static_cast<int64_t>(eng->cfg.n_head_kv) * kHeadDim;
-            launch_write(pool_view(eng), rope_view(eng), BatchView{},
-                         kv_write_args(static_cast<const RowItem *>(dev),
-                                       static_cast<int32_t>(row_item_count(begin, n_tokens)), layer, HKV_F32,
-                                       k_prerope, v, row, row, true),
-                         eng->d_err, stream);
-        } else {
-            launch_append_range(pool_view(eng), rope_view(eng), static_cast<const int32_t *>(dev),
-                                begin, n_tokens, layer, k_prerope, v, true, eng->d_err, stream);
-        }
+        launch_append_range(pool_view(eng), rope_view(eng), static_cast<const int32_t *>(dev),
+                            begin, n_tokens, layer, k_prerope, v, true, eng->d_err, stream);
         ++eng->kernel_launches;
     }
     HKV_CUDA_TRY(eng, eng->range_stage.mark_used(stream));
@@ -1739,37 +1772,7 @@ int hkv_qkv_write(hkv_engine *eng, const hkv_qkv_write_args *args, hkv_stream st
     if (total == 0) {
         return HKV_OK;
     }
-    RowCache &rc = eng->write_rows;
-    if (!row_cache_matches(eng, rc, a.n, a.slots, begin.data(), a.n_tokens)) {
-        int64_t extra = 0;
-        for (int32_t e = 0; e < a.n; ++e) {
-            const Slot &s = eng->slots[a.slots[e]];
-            extra += pages_beyond_reservation(s, pages_needed(eng, s, begin[e], begin[e] + a.n_tokens[e]));
-        }
-        if (extra > unreserved_free(eng)) {
-            return fail(eng, HKV_ERR_OOM, "rows need %lld unreserved pages, %lld free",
-                        static_cast<long long>(extra), static_cast<long long>(unreserved_free(eng)));
-        }
-        for (int32_t e = 0; e < a.n; ++e) {
-            st = own_rows(eng, eng->slots[a.slots[e]], begin[e], begin[e] + a.n_tokens[e], stream);
-            if (st != HKV_OK) return st;
-        }
-        st = flush_cow(eng, stream);
-        if (st != HKV_OK) return st;
-        st = upload_rows(eng, eng->write_stage, rc, a.n, a.slots, begin.data(), a.n_tokens, stream);
-        if (st != HKV_OK) return st;
-    }
-    ++eng->enqueue_seq;
-    w.items = rc.items;
-    w.n_items = rc.n_items;
-    {
-        ProfileScope ps(eng, HKV_KERNEL_APPEND, stream);
-        launch_write(pool_view(eng), rope_view(eng), BatchView{}, w, eng->d_err, stream);
-        ++eng->kernel_launches;
-    }
-    rc.consumed = true;
-    rc.consumer_stream = stream;
-    return launch_status(eng, "write kernel launch");
+    return write_rows(eng, w, a.n, a.slots, begin.data(), a.n_tokens, stream);
 }
 
 int hkv_window_attn(hkv_engine *eng, const hkv_window_attn_args *args, hkv_stream stream_h) {

@@ -226,6 +226,7 @@ struct WriteArgs {
     const float *q_norm, *k_norm;                        // nullptr: no norm
     float eps;
     bool rope;
+    bool one_row;  // every item has one row
 };
 void launch_write(const PoolView &pool, const RopeView &rope, const BatchView &batch,
                   const WriteArgs &args, DeviceError *err, cudaStream_t stream);

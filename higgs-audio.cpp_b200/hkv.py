@@ -17,6 +17,7 @@ from __future__ import annotations
 import ctypes
 import os
 import re
+from array import array
 from pathlib import Path
 from typing import Optional, Sequence
 
@@ -280,14 +281,14 @@ def _stream(s) -> Optional[int]:
 
 
 def _slots_arg(slots: Sequence[int]):
-    arr = (ctypes.c_int32 * len(slots))(*[int(s) for s in slots])
-    return len(slots), arr
+    a = array("i", slots)
+    return len(a), (ctypes.c_int32 * len(a)).from_buffer(a)
 
 
 def _counts_arg(counts: Sequence[int], n: int):
     if len(counts) != n:
         raise ValueError(f"{len(counts)} lengths for {n} slots")
-    return (ctypes.c_int64 * n)(*[int(c) for c in counts])
+    return (ctypes.c_int64 * n).from_buffer(array("q", counts))
 
 
 class ScopedBackendKvCacheSlot:
