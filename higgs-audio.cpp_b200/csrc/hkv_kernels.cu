@@ -122,6 +122,12 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// An 8 x 8 F16 tile, two columns of a row a lane, transposed.
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t a) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&h);
@@ -872,6 +878,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
     // next unit to issue already loaded, one iteration ahead of its use.
     Cursor prod = cons;
     int64_t next_page = 0;
+    int64_t page_after = 0;  // 8-bit cache: of the unit after it, at `look`
+    Cursor look = cons;
     if (lane == 0) {
         const int first_pages[3] = {ws1.y, ws1.z, ws1.w};
 #pragma unroll
@@ -885,6 +893,11 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
         }
         if (u_begin + kStages < u_end) {
             next_page = batch.pages[prod.pbase + prod.i];
+        }
+        if (kE4m3 && u_begin + kStages + 1 < u_end) {
+            look = prod;
+            advance(batch, G, look);
+            page_after = batch.pages[look.pbase + look.i];
         }
     }
 
@@ -1296,6 +1309,187 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
             e_v = kExpMin;
         }
 
+        if constexpr (kE4m3) {
+            // ---- 8-bit cache: two pages of the segment at a time where it has them.
+            // The chain of a page (wait, products, maximum, exponentials, products) is
+            // far longer than its instructions: two in step nearly halve it.
+            const int cnt = u + 1 < u_end && cons.i + 1 < cons.np ? 2 : 1;
+            uint32_t st[2];
+            bool there = true;
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+                st[hh] = stage0 + ((k + hh) % kStages) * kStage;
+                if (hh < cnt) {
+                    there = mbar_wait_bounded(bar0 + 8 * ((k + hh) % kStages),
+                                              static_cast<uint32_t>((k + hh) / kStages) & 1u) &&
+                            there;
+                }
+            }
+            if (!__all_sync(0xffffffffu, there)) {
+                if (lane == 0) {
+                    record_error(err, kErrTimeout, kWhereAttn, u, blockIdx.x);
+                }
+                for (int j = 0; j < kStages && u + j < u_end; ++j) {
+                    mbar_wait_bounded(bar0 + 8 * ((k + j) % kStages),
+                                      static_cast<uint32_t>((k + j) / kStages) & 1u);
+                }
+                return;
+            }
+            const int row0 = cons.i * kPageTokens;
+            if (cons.i + cnt == cons.np) {
+                // the slot's last page: rows past its length hold whatever the page
+                // had before (0 * garbage must not reach o), and the fused append
+                // belongs here
+                const uint32_t kt = cnt == 2 ? st[1] : st[0];
+                const uint32_t vt = kt + kCodeBlockBytes;
+                const int valid = ntok - (cons.np - 1) * kPageTokens;
+                for (int idx = lane; idx < (kPageTokens - valid) * (kHeadDim / 16); idx += 32) {
+                    st_shared_zero16(vt + valid * kHeadDim + idx * 16);
+                }
+                if (kAppend) {
+                    const int64_t row_base = (static_cast<int64_t>(seg_e) * G + seg_h) * kHeadDim;
+                    const int64_t page = checked_page(pool, batch.pages[cons.pbase + cons.np - 1], seg_e, err);
+                    append_row_e4m3(pool, rope, k_new + row_base, v_new + row_base, seg_pos, layer, page, seg_h, kt,
+                                    vt, kt + 2 * kCodeBlockBytes, lane);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+            }
+            const int g = lane >> 2;
+            const int t = lane & 3;
+            float sv[2][4];  // logits of rows g (heads a, b) and g + 8 of each page
+            int ev[2] = {kExpMin, kExpMin};
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    sv[hh][j] = kNegInf;
+                }
+                if (hh < cnt) {
+                    float sc[4] = {0.f, 0.f, 0.f, 0.f};
+                    float sd[4] = {0.f, 0.f, 0.f, 0.f};
+                    const float s_scale = scale_log2 * pow2(ld_shared_s32(st[hh] + 2 * kCodeBlockBytes));
+                    ev[hh] = ld_shared_s32(st[hh] + 2 * kCodeBlockBytes + 4);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        // rows g and g + 8: the same swizzle
+                        const uint32_t at = st[hh] + g * kHeadDim + (((2 * t + i) ^ g) << 4);
+                        const uint4 x = ld_shared_v4(at);
+                        const uint4 y = ld_shared_v4(at + 8 * kHeadDim);
+                        const uint32_t w0[4] = {x.x, x.y, x.z, x.w};
+                        const uint32_t w1[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                        for (int ks = 0; ks < 4; ++ks) {
+                            mma_16816(ks & 1 ? sd : sc, codes_to_half2(w0[ks]), codes_to_half2(w1[ks]),
+                                      codes_to_half2_hi(w0[ks]), codes_to_half2_hi(w1[ks]), qb[4 * i + ks][0],
+                                      qb[4 * i + ks][1]);
+                        }
+                    }
+                    const int tok = row0 + hh * kPageTokens + g;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        sc[j] += sd[j];
+                        sc[j] += __shfl_xor_sync(0xffffffffu, sc[j], 2);
+                        sv[hh][j] = tok + (j >> 1) * 8 < ntok ? sc[j] * s_scale : kNegInf;
+                    }
+                }
+            }
+            float mx_a = fmaxf(fmaxf(sv[0][0], sv[0][2]), fmaxf(sv[1][0], sv[1][2]));
+            float mx_b = fmaxf(fmaxf(sv[0][1], sv[0][3]), fmaxf(sv[1][1], sv[1][3]));
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) {
+                mx_a = fmaxf(mx_a, __shfl_xor_sync(0xffffffffu, mx_a, off));
+                mx_b = fmaxf(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, off));
+            }
+            const float mn_a = fmaxf(m_a, mx_a);
+            const float mn_b = fmaxf(m_b, mx_b);
+            const int e_new = max(e_v, max(ev[0], ev[1]));
+            const float alpha_a = exp2f(m_a - mn_a);
+            const float alpha_b = exp2f(m_b - mn_b);
+            const float grow = pow2(max(e_v - e_new, -126));
+            m_a = mn_a;
+            m_b = mn_b;
+            e_v = e_new;
+            float sum_a = 0.f, sum_b = 0.f;
+            uint32_t pb[2][2];  // the weights as the second product's B fragments
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+                float p[4];
+                p[0] = exp2f(sv[hh][0] - mn_a);
+                p[1] = exp2f(sv[hh][1] - mn_b);
+                p[2] = exp2f(sv[hh][2] - mn_a);
+                p[3] = exp2f(sv[hh][3] - mn_b);
+                sum_a += p[0] + p[2];
+                sum_b += p[1] + p[3];
+                const float w = pow2(max(ev[hh] - e_new + kPShift, -126));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    p[j] *= w;
+                }
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    pb[hh][j] = transpose_8x8(lo_side ? pack_half2(f16_residual(p[2 * j]), f16_residual(p[2 * j + 1]))
+                                                      : pack_half2(p[2 * j], p[2 * j + 1]));
+                }
+            }
+            l_a = l_a * alpha_a + sum_a;
+            l_b = l_b * alpha_b + sum_b;
+#pragma unroll
+            for (int mt = 0; mt < 8; ++mt) {
+                o[mt][0] *= alpha_a * grow;
+                o[mt][1] *= alpha_b * grow;
+                o[mt][2] *= alpha_a * grow;
+                o[mt][3] *= alpha_b * grow;
+            }
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+                if (hh < cnt) {
+                    const uint32_t vt = st[hh] + kCodeBlockBytes;
+                    const int r = 2 * t;
+                    const uint4 a = ld_shared_v4(vt + r * kHeadDim + ((g ^ r) << 4));
+                    const uint4 b = ld_shared_v4(vt + (r + 1) * kHeadDim + ((g ^ (r + 1)) << 4));
+                    const uint4 c = ld_shared_v4(vt + (r + 8) * kHeadDim + ((g ^ r) << 4));
+                    const uint4 d = ld_shared_v4(vt + (r + 9) * kHeadDim + ((g ^ (r + 1)) << 4));
+                    const uint32_t va[4] = {a.x, a.y, a.z, a.w};
+                    const uint32_t vb[4] = {b.x, b.y, b.z, b.w};
+                    const uint32_t vc[4] = {c.x, c.y, c.z, c.w};
+                    const uint32_t vd[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            // dims 4w + 2 half and + 1 of the lane's 16, two rows a pair
+                            const uint32_t ab = __byte_perm(va[w], vb[w], half ? 0x7362 : 0x5140);
+                            const uint32_t cd = __byte_perm(vc[w], vd[w], half ? 0x7362 : 0x5140);
+                            mma_16816(o[2 * w + half], codes_to_half2(ab), codes_to_half2_hi(ab),
+                                      codes_to_half2(cd), codes_to_half2_hi(cd), pb[hh][0], pb[hh][1]);
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) {
+                fence_proxy_async_smem();
+                for (int hh = 0; hh < cnt; ++hh) {
+                    if (u + hh + kStages < u_end) {
+                        issue(checked_page(pool, next_page, prod.e, err), prod.h, st[hh],
+                              bar0 + 8 * ((k + hh) % kStages));
+                        advance(batch, G, prod);
+                        next_page = page_after;
+                        advance(batch, G, look);
+                        if (u + hh + kStages + 2 < u_end) {
+                            page_after = batch.pages[look.pbase + look.i];
+                        }
+                    }
+                }
+            }
+            for (int hh = 0; hh < cnt; ++hh) {
+                advance(batch, G, cons);
+            }
+            u += cnt - 1;
+            k += cnt - 1;
+            continue;
+        }
         // ---- wait for this unit's K and V head blocks
         const uint32_t bar = bar0 + 8 * s;
         const bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity));
@@ -1312,32 +1506,26 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
             return;
         }
         const uint32_t kt = stage0 + s * kStage;
-        const uint32_t vt = kt + (kE4m3 ? kCodeBlockBytes : kHeadBlockBytes);
-        const uint32_t et = kt + 2 * kCodeBlockBytes;  // exponents (8-bit format)
+        const uint32_t vt = kt + kHeadBlockBytes;
         const int row0 = cons.i * kPageTokens;
         const int valid = min(kPageTokens, ntok - row0);
         if (valid < kPageTokens) {
             // Rows past the slot's length hold whatever the page had before;
             // zero them in shared memory so 0 * garbage cannot poison PV.
-            constexpr int kRow = kE4m3 ? kHeadDim : kRowBytes;
-            for (int idx = lane; idx < (kPageTokens - valid) * (kRow / 16); idx += 32) {
-                st_shared_zero16(vt + valid * kRow + idx * 16);
+            for (int idx = lane; idx < (kPageTokens - valid) * 16; idx += 32) {
+                st_shared_zero16(vt + (valid + (idx >> 4)) * kRowBytes + (idx & 15) * 16);
             }
         }
         if (kAppend && cons.i == cons.np - 1) {
             // Fused append: this warp owns the slot's last page for this KV
             // head, so it writes the new row to HBM and into its copy of the
             // page (the copy arrived without it).
-            const int64_t row_base = (static_cast<int64_t>(seg_e) * G + seg_h) * kHeadDim;
-            const int64_t page = checked_page(pool, batch.pages[cons.pbase + cons.i], seg_e, err);
-            if constexpr (kE4m3) {
-                append_row_e4m3(pool, rope, k_new + row_base, v_new + row_base, seg_pos, layer, page, seg_h, kt,
-                                vt, et, lane);
-            } else {
             const int r = seg_pos & 15;
             const int c = lane & 15;
             const bool is_v = lane >= 16;
+            const int64_t row_base = (static_cast<int64_t>(seg_e) * G + seg_h) * kHeadDim;
             const uint4 chunk = new_row_chunk(rope, k_new + row_base, v_new + row_base, seg_pos, lane);
+            const int64_t page = checked_page(pool, batch.pages[cons.pbase + cons.i], seg_e, err);
             uint8_t *dst = pool.base +
                            head_block_index(page, layer, is_v ? 1 : 0, seg_h, pool.n_pages, G) *
                                kHeadBlockBytes +
@@ -1347,7 +1535,6 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
             asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(sdst), "r"(chunk.x),
                          "r"(chunk.y), "r"(chunk.z), "r"(chunk.w)
                          : "memory");
-            }
         }
         if (valid < kPageTokens || (kAppend && cons.i == cons.np - 1)) {
             fence_proxy_async_smem();
@@ -1396,23 +1583,6 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
         // Two accumulators (even / odd k-steps) halve the dependent mma chain.
         float sc[4] = {0.f, 0.f, 0.f, 0.f};
         float sd[4] = {0.f, 0.f, 0.f, 0.f};
-        if constexpr (kE4m3) {
-            const int g = lane >> 2;
-            const int t = lane & 3;
-            uint32_t w0[8], w1[8];  // rows g and g + 8 (the same swizzle: g + 8 = g mod 8)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint4 lo = ld_shared_v4(kt + g * kHeadDim + (((2 * t + i) ^ g) << 4));
-                const uint4 hi = ld_shared_v4(kt + (g + 8) * kHeadDim + (((2 * t + i) ^ g) << 4));
-                w0[4 * i] = lo.x; w0[4 * i + 1] = lo.y; w0[4 * i + 2] = lo.z; w0[4 * i + 3] = lo.w;
-                w1[4 * i] = hi.x; w1[4 * i + 1] = hi.y; w1[4 * i + 2] = hi.z; w1[4 * i + 3] = hi.w;
-            }
-#pragma unroll
-            for (int ks = 0; ks < 8; ++ks) {
-                mma_16816(ks & 1 ? sd : sc, codes_to_half2(w0[ks]), codes_to_half2(w1[ks]),
-                          codes_to_half2_hi(w0[ks]), codes_to_half2_hi(w1[ks]), qb[ks][0], qb[ks][1]);
-            }
-        } else {
 #pragma unroll
         for (int ks = 0; ks < 8; ks += 2) {
             uint32_t a0, a1, a2, a3, b0, b1, b2, b3;
@@ -1421,7 +1591,6 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
             mma_16816(sc, a0, a1, a2, a3, qb[ks][0], qb[ks][1]);
             mma_16816(sd, b0, b1, b2, b3, qb[ks + 1][0], qb[ks + 1][1]);
         }
-        }
 #endif
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -1429,11 +1598,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
             sc[j] += __shfl_xor_sync(0xffffffffu, sc[j], 2);
         }
         const int tok = row0 + (lane >> 2);
-        const float s_scale = kE4m3 ? scale_log2 * pow2(ld_shared_s32(et)) : scale_log2;
-        const float s0 = tok < ntok ? sc[0] * s_scale : kNegInf;      // head a, row g
-        const float s1 = tok < ntok ? sc[1] * s_scale : kNegInf;      // head b, row g
-        const float s2 = tok + 8 < ntok ? sc[2] * s_scale : kNegInf;  // head a, row g+8
-        const float s3 = tok + 8 < ntok ? sc[3] * s_scale : kNegInf;  // head b, row g+8
+        const float s0 = tok < ntok ? sc[0] * scale_log2 : kNegInf;      // head a, row g
+        const float s1 = tok < ntok ? sc[1] * scale_log2 : kNegInf;      // head b, row g
+        const float s2 = tok + 8 < ntok ? sc[2] * scale_log2 : kNegInf;  // head a, row g+8
+        const float s3 = tok + 8 < ntok ? sc[3] * scale_log2 : kNegInf;  // head b, row g+8
         float mx_a = fmaxf(s0, s2);
         float mx_b = fmaxf(s1, s3);
 #pragma unroll
@@ -1443,30 +1611,16 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
         }
         const float mn_a = fmaxf(m_a, mx_a);
         const float mn_b = fmaxf(m_b, mx_b);
-        float alpha_a = exp2f(m_a - mn_a);
-        float alpha_b = exp2f(m_b - mn_b);
-        float p0 = exp2f(s0 - mn_a);
-        float p1 = exp2f(s1 - mn_b);
-        float p2 = exp2f(s2 - mn_a);
-        float p3 = exp2f(s3 - mn_b);
+        const float alpha_a = exp2f(m_a - mn_a);
+        const float alpha_b = exp2f(m_b - mn_b);
+        const float p0 = exp2f(s0 - mn_a);
+        const float p1 = exp2f(s1 - mn_b);
+        const float p2 = exp2f(s2 - mn_a);
+        const float p3 = exp2f(s3 - mn_b);
         l_a = l_a * alpha_a + (p0 + p2);
         l_b = l_b * alpha_b + (p1 + p3);
         m_a = mn_a;
         m_b = mn_b;
-        if (kE4m3) {
-            // from here on alpha rescales o only, and p are o's weights
-            const int e_page = ld_shared_s32(et + 4);
-            const int e_new = max(e_v, e_page);
-            const float grow = pow2(max(e_v - e_new, -126));
-            const float w = pow2(max(e_page - e_new + kPShift, -126));
-            e_v = e_new;
-            alpha_a *= grow;
-            alpha_b *= grow;
-            p0 *= w;
-            p1 *= w;
-            p2 *= w;
-            p3 *= w;
-        }
 #if HKV_CUDA_CORES
         // ---- CUDA cores: p (F32) to shared memory as [token][head], then each
         // lane accumulates its 4 dims of every head over the 16 tokens.
@@ -1528,40 +1682,12 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
         ldsm_x2_trans(pbuf + (lane & 15) * 16, pb0, pb1);
 
         // ---- O^T[dim][col] += V^T[dim][token] . P^T[token][col]
-        if constexpr (kE4m3) {
-            const int g = lane >> 2;
-            const int t = lane & 3;
-            uint32_t va[4], vb[4], vc[4], vd[4];  // rows 2t, 2t + 1, 2t + 8, 2t + 9
-            {
-                const int r = 2 * t;
-                const uint4 a = ld_shared_v4(vt + r * kHeadDim + ((g ^ r) << 4));
-                const uint4 b = ld_shared_v4(vt + (r + 1) * kHeadDim + ((g ^ (r + 1)) << 4));
-                const uint4 c = ld_shared_v4(vt + (r + 8) * kHeadDim + ((g ^ r) << 4));
-                const uint4 d = ld_shared_v4(vt + (r + 9) * kHeadDim + ((g ^ (r + 1)) << 4));
-                va[0] = a.x; va[1] = a.y; va[2] = a.z; va[3] = a.w;
-                vb[0] = b.x; vb[1] = b.y; vb[2] = b.z; vb[3] = b.w;
-                vc[0] = c.x; vc[1] = c.y; vc[2] = c.z; vc[3] = c.w;
-                vd[0] = d.x; vd[1] = d.y; vd[2] = d.z; vd[3] = d.w;
-            }
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    // dims 4w + 2 half and + 1 of the lane's 16, two rows a pair
-                    const uint32_t ab = __byte_perm(va[w], vb[w], half ? 0x7362 : 0x5140);
-                    const uint32_t cd = __byte_perm(vc[w], vd[w], half ? 0x7362 : 0x5140);
-                    mma_16816(o[2 * w + half], codes_to_half2(ab), codes_to_half2_hi(ab), codes_to_half2(cd),
-                              codes_to_half2_hi(cd), pb0, pb1);
-                }
-            }
-        } else {
 #pragma unroll
         for (int mt = 0; mt < 8; ++mt) {
             uint32_t a0, a1, a2, a3;
             const int chunk = 2 * mt + v_chunk_hi;
             ldsm_x4_trans(vt + v_row_off + ((chunk ^ r7) << 4), a0, a1, a2, a3);
             mma_16816(o[mt], a0, a1, a2, a3, pb0, pb1);
-        }
         }
 #endif
         __syncwarp();
