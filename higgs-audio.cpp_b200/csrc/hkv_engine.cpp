@@ -693,7 +693,17 @@ int ensure_batch(hkv_engine *eng, int32_t n, const int32_t *slots, cudaStream_t 
         }
         C = plan_cluster(n, G, total_pages, max_warps, fit);
     }
-    const int32_t W = C > 0 ? G * C * kAttnWarps : plan_warps(total_pages * G, max_warps);
+    int32_t W = C > 0 ? G * C * kAttnWarps : plan_warps(total_pages * G, max_warps);
+    // Many segments on an 8-bit cache: the kernel variant with more warps.
+    const bool wide = C == 0 && eng->cache_type == HKV_CACHE_E4M3 &&
+                      !plan_cta_merge(static_cast<int64_t>(n) * G, W);
+    PlanRules rules;
+    if (wide) {
+        rules.cta_merge = false;
+        rules.leave_whole = 2 * kCostLeaveWhole;  // a page costs about half as much here
+        rules.leave_shared = 2 * kCostLeaveShared;
+        W = plan_wide_warps(total_pages * G, eng->num_sms);
+    }
     const size_t words = plan_words(n, G, total_pages, W);
     if (bc.consumed) {
         HKV_CUDA_TRY(eng, eng->batch_stage.mark_used(bc.consumer_stream));
@@ -703,7 +713,7 @@ int ensure_batch(hkv_engine *eng, int32_t n, const int32_t *slots, cudaStream_t 
     HKV_CUDA_TRY(eng, eng->batch_stage.begin(words * sizeof(int32_t), &host));
     const PlanSummary plan =
         C > 0 ? build_cluster_plan(static_cast<int32_t *>(host), G, pos[0], lists[0], C)
-              : build_plan(static_cast<int32_t *>(host), n, G, pos.data(), lists.data(), total_pages, W);
+              : build_plan(static_cast<int32_t *>(host), n, G, pos.data(), lists.data(), total_pages, W, rules);
     if (static_cast<int64_t>(plan.n_parts) + plan.n_groups > eng->part_cap) {
         return fail(eng, HKV_ERR_OOM, "split plan needs %d partials, capacity %lld",
                     plan.n_parts + plan.n_groups, static_cast<long long>(eng->part_cap));
@@ -712,6 +722,9 @@ int ensure_batch(hkv_engine *eng, int32_t n, const int32_t *slots, cudaStream_t 
     ++eng->enqueue_seq;
     HKV_CUDA_TRY(eng, eng->batch_stage.commit(words * sizeof(int32_t), stream, &dev));
     bc.view = bind_plan(static_cast<const int32_t *>(dev), n, G, plan, W);
+    if (wide) {
+        bc.view.cta_warps = (W + eng->num_sms - 1) / eng->num_sms;
+    }
     bc.slots.assign(slots, slots + n);
     bc.used.resize(static_cast<size_t>(n));
     for (int32_t e = 0; e < n; ++e) {
@@ -1256,7 +1269,10 @@ int hkv_engine_create_cache(const hkv_config *cfg, int32_t cache_type, hkv_engin
         // (entry, KV head) share boundary, then the group partials of the
         // two-level merge (at most one per 8 partials, rounded up).
         const int64_t segs = static_cast<int64_t>(cfg->max_slots) * cfg->n_head_kv;
-        const int64_t level1 = static_cast<int64_t>(eng->num_sms) * kAttnWarps + segs;
+        const int64_t level1 =
+            static_cast<int64_t>(eng->num_sms) *
+                (cache_type == HKV_CACHE_E4M3 ? std::max(kAttnWarps, kAttnWarpsE4m3) : kAttnWarps) +
+            segs;
         const int64_t groups = level1 / 8 + segs;
         eng->part_cap = level1 + groups;
         e = cudaMalloc(&eng->part_o, static_cast<size_t>(eng->part_cap) * kGqa * kHeadDim * 4);

@@ -92,6 +92,8 @@ struct BatchView {
     int32_t cluster;          // > 0: CTAs per thread-block cluster; cluster k holds segment
                               // k, whose CTA partials meet in the shared memory of the
                               // cluster's first CTA (plan_cluster); 0: no clusters
+    int32_t cta_warps;        // warps of a CTA where the kernel takes that from the plan
+                              // (the 8-bit cache without the CTA merge)
 };
 
 // Partials of one (entry, KV head) are merged by one warp when there are at
@@ -166,10 +168,24 @@ struct RopeView {
 #endif
 constexpr int kAttnWarps = HKV_ATTN_WARPS;    // consumer warps per CTA, one CTA per SM
 constexpr int kAttnStages = HKV_ATTN_STAGES;  // TMA ring depth per warp (K+V block per stage)
+// The 8-bit cache.  With the CTA merge: the same 8 warps, 4 stages of one page
+// (half as large) each.  Without it (many segments): up to 12 warps x 4 stages.  A
+// page costs a warp as many instructions as an F16 page and half the time on the
+// bus, so the loop is bound by latency until a scheduler has three warps: 32 slots of
+// 2k-16k positions 122 us a layer with 8 warps, 111 with 10, 100 with 12 x 4 stages,
+// 108 with 12 x 2, 106 with 16 x 2 (which spills).
 #ifndef HKV_ATTN_STAGES_E4M3
 #define HKV_ATTN_STAGES_E4M3 4
 #endif
-constexpr int kAttnStagesE4m3 = HKV_ATTN_STAGES_E4M3;  // the same for the 8-bit cache
+#ifndef HKV_ATTN_STAGES_E4M3_WIDE
+#define HKV_ATTN_STAGES_E4M3_WIDE 4
+#endif
+#ifndef HKV_ATTN_WARPS_E4M3
+#define HKV_ATTN_WARPS_E4M3 12
+#endif
+constexpr int kAttnStagesE4m3 = HKV_ATTN_STAGES_E4M3;
+constexpr int kAttnStagesE4m3Wide = HKV_ATTN_STAGES_E4M3_WIDE;
+constexpr int kAttnWarpsE4m3 = HKV_ATTN_WARPS_E4M3;
 
 void launch_append(const PoolView &pool, const RopeView &rope, const BatchView &batch, int layer,
                    const float *k, const float *v, bool apply_rope, DeviceError *err,

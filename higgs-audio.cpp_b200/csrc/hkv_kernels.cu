@@ -49,12 +49,14 @@ constexpr int kPBufBytes = 16 * 16;                // 16 tokens x 8 halves
 // and V of a page and KV head each), the staged queries, the P tile and one
 // 8-byte mbarrier per stage.  A unit of the 8-bit format is half as large, so
 // the same shared memory holds twice the stages.
-template <bool kE4m3>
+template <bool kE4m3, bool kCtaMerge>
 struct Ring {
-    static constexpr int kStages = kE4m3 ? kAttnStagesE4m3 : kAttnStages;
+    static constexpr int kStages = !kE4m3 ? kAttnStages : kCtaMerge ? kAttnStagesE4m3 : kAttnStagesE4m3Wide;
     static constexpr int kStage = kE4m3 ? kCodeUnitBytes : kStageBytes;
     static constexpr int kBarBytes = (kStages * 8 + 15) / 16 * 16;
-    static constexpr int kWarpSmem = kStages * kStage + kQcBytes + kPBufBytes + kBarBytes;
+    static constexpr int kPTile = kE4m3 ? 0 : kPBufBytes;  // the 8-bit kernel keeps P in registers
+    static constexpr int kWarpSmem = kStages * kStage + kQcBytes + kPTile + kBarBytes;
+    static constexpr int kWarps = kE4m3 && !kCtaMerge ? kAttnWarpsE4m3 : kAttnWarps;
 };
 // CTA-level partials: two slots per warp (the run a warp does not start, and
 // the run it starts), each o[4][128] + (m, l)[4]; then one ticket per run.
@@ -72,14 +74,17 @@ constexpr int kWhereGather = 3;
 constexpr int kWhereCow = 4;
 constexpr int kWhereSplitWait = 5;
 
-static_assert(Ring<false>::kWarpSmem % 16 == 0 && Ring<true>::kWarpSmem % 16 == 0,
+static_assert(Ring<false, true>::kWarpSmem % 16 == 0 && Ring<true, true>::kWarpSmem % 16 == 0,
               "per-warp shared region must keep 16-byte alignment");
-static_assert(Ring<false>::kBarBytes >= 8 * Ring<false>::kStages &&
-                  Ring<true>::kBarBytes >= 8 * Ring<true>::kStages,
+static_assert(Ring<false, true>::kBarBytes >= 8 * Ring<false, true>::kStages &&
+                  Ring<true, true>::kBarBytes >= 8 * Ring<true, true>::kStages,
               "every stage needs its mbarrier inside the warp's region");
-static_assert(kAttnWarps * Ring<false>::kWarpSmem + kCtaSmem + kClusterSmem <= 227 * 1024 &&
-                  kAttnWarps * Ring<true>::kWarpSmem + kCtaSmem + kClusterSmem <= 227 * 1024,
+static_assert(kAttnWarps * Ring<false, true>::kWarpSmem + kCtaSmem + kClusterSmem <= 227 * 1024 &&
+                  kAttnWarps * Ring<true, true>::kWarpSmem + kCtaSmem + kClusterSmem <= 227 * 1024,
               "attention CTA exceeds shared memory");
+static_assert(Ring<true, false>::kWarpSmem % 16 == 0 && Ring<true, false>::kBarBytes >= 8 * Ring<true, false>::kStages &&
+                  Ring<true, false>::kWarps * Ring<true, false>::kWarpSmem <= 227 * 1024,
+              "attention CTA of the 8-bit cache exceeds shared memory");
 static_assert(kCtaPartBytes % 16 == 0, "CTA partial slots must keep 16-byte alignment");
 static_assert(kAttnWarps <= 8, "one run ticket per warp in 32 bytes");
 
@@ -587,9 +592,10 @@ __device__ __forceinline__ void merge_partials(const float *part_o, const float 
 // batch of outputs goes out with the (m, l) loads, since the outputs do not
 // depend on the weights.  Used for the merges of a warp's last segment, after
 // its main loop, where the registers of the loop are free.
+// kBatch: partial outputs in flight per lane.
+template <int kBatch>
 __device__ __forceinline__ void merge_partials_wide(const float *part_o, const float *part_ml, int p0,
                                                int nparts, int lane, Merged &res) {
-    constexpr int kBatch = 8;  // partial outputs in flight per lane
     float4 ov[kBatch][kGqa];
     auto load_batch = [&](int t0) {
 #pragma unroll
@@ -796,22 +802,26 @@ __device__ __forceinline__ void signal_arrival(const Exchange &x, int layer, int
 // permutation of the dims if q uses the same), and dims 16g .. 16g + 15 of V
 // rows 2t, 2t + 1, 2t + 8, 2t + 9, whose bytes pair up to the A fragment of V^T.
 template <bool kAppend, bool kCtaMerge, bool kCluster, bool kE4m3>
-__global__ void __launch_bounds__(kAttnWarps * 32, 1)
+__global__ void __launch_bounds__(Ring<kE4m3, kCtaMerge>::kWarps * 32, 1)
     attention_kernel(PoolView pool, RopeView rope, BatchView batch, int layer,
                      const float *__restrict__ q, const float *__restrict__ k_new,
                      const float *__restrict__ v_new, float *__restrict__ part_o,
                      float *__restrict__ part_ml, int32_t *__restrict__ counters,
-                     float *__restrict__ out, Exchange xchg, float scale_log2, DeviceError *err) {
+                     float *__restrict__ out, Exchange xchg, float scale_log2, DeviceError *err,
+                     bool wait_first) {
     extern __shared__ __align__(1024) uint8_t smem[];
     const int lane = threadIdx.x & 31;
     const int wid = threadIdx.x >> 5;
-    const int gw = blockIdx.x * kAttnWarps + wid;
+    // the wide variant of the 8-bit kernel runs with as few warps as the plan needs
+    const int cta_warps = kE4m3 && !kCtaMerge ? static_cast<int>(blockDim.x >> 5) : kAttnWarps;
+    const int gw = blockIdx.x * cta_warps + wid;
     const int G = pool.n_head_kv;
     const int W = batch.n_warps;
     static_assert(kCtaMerge || !kCluster, "the cluster merge starts from the CTA merge");
-    constexpr int kStages = Ring<kE4m3>::kStages;
-    constexpr int kStage = Ring<kE4m3>::kStage;
-    constexpr int kWarpSmem = Ring<kE4m3>::kWarpSmem;
+    constexpr int kStages = Ring<kE4m3, kCtaMerge>::kStages;
+    constexpr int kStage = Ring<kE4m3, kCtaMerge>::kStage;
+    constexpr int kWarpSmem = Ring<kE4m3, kCtaMerge>::kWarpSmem;
+    constexpr int kMergeBatch = Ring<kE4m3, kCtaMerge>::kWarps > 8 ? 4 : 8;  // by the registers a thread has
     float *cta_slots = reinterpret_cast<float *>(smem + kAttnWarps * kWarpSmem);
     int *run_ticket = reinterpret_cast<int *>(smem + kAttnWarps * kWarpSmem + kAttnWarps * 2 * kCtaPartBytes);
     float *cl_slots = reinterpret_cast<float *>(smem + kAttnWarps * kWarpSmem + kCtaSmem);
@@ -835,6 +845,11 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
     if (gw >= W) {
         return;
     }
+    if (kE4m3 && wait_first) {
+        // launched as a dependent of a kernel that may have written the plan or
+        // this layer's pages
+        pdl_wait();
+    }
     // The plan hands each warp its share, its starting cursor and the
     // physical pages of its first units in three 16-byte records, so the
     // first copies go out without a chain of dependent loads.
@@ -849,7 +864,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
     const uint32_t stage0 = smem_u32(smem + wid * kWarpSmem);
     const uint32_t qc = stage0 + kStages * kStage;
     const uint32_t pbuf = qc + kQcBytes;
-    const uint32_t bar0 = pbuf + kPBufBytes;
+    const uint32_t bar0 = pbuf + Ring<kE4m3, kCtaMerge>::kPTile;
     const uint64_t policy = evict_first_policy();
     auto issue = [&](int64_t page, int h, uint32_t stage, uint32_t bar) {
         if constexpr (kE4m3) {
@@ -1150,7 +1165,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
             if (ticket == nparts - 1) {
                 Merged res;
                 if (after_loop) {
-                    merge_partials_wide(part_o, part_ml, p_first, nparts, lane, res);
+                    merge_partials_wide<kMergeBatch>(part_o, part_ml, p_first, nparts, lane, res);
                 } else {
                     merge_partials(part_o, part_ml, p_first, nparts, lane, res);
                 }
@@ -1173,7 +1188,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
         __threadfence();
         Merged grp;
         if (after_loop) {
-            merge_partials_wide(part_o, part_ml, p_first + g * gsz, g_size, lane, grp);
+            merge_partials_wide<kMergeBatch>(part_o, part_ml, p_first + g * gsz, g_size, lane, grp);
         } else {
             merge_partials(part_o, part_ml, p_first + g * gsz, g_size, lane, grp);
         }
@@ -1205,7 +1220,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, 1)
             __threadfence();
             Merged res;
             if (after_loop) {
-                merge_partials_wide(part_o, part_ml, batch.n_parts + batch.part2_off[eh], n_groups, lane, res);
+                merge_partials_wide<kMergeBatch>(part_o, part_ml, batch.n_parts + batch.part2_off[eh], n_groups, lane, res);
             } else {
                 merge_partials(part_o, part_ml, batch.n_parts + batch.part2_off[eh], n_groups, lane, res);
             }
@@ -1907,7 +1922,11 @@ __global__ void gather_kernel(PoolView pool, const int32_t *__restrict__ slot_pa
 }  // namespace
 
 size_t attention_smem_bytes(bool cta_merge, bool cluster, bool e4m3) {
-    return static_cast<size_t>(kAttnWarps) * (e4m3 ? Ring<true>::kWarpSmem : Ring<false>::kWarpSmem) + (cta_merge ? kCtaSmem : 0) +
+    const int warp = !e4m3 ? Ring<false, true>::kWarpSmem
+                     : cta_merge ? Ring<true, true>::kWarpSmem
+                                 : Ring<true, false>::kWarpSmem;
+    const int warps = e4m3 && !cta_merge ? kAttnWarpsE4m3 : kAttnWarps;
+    return static_cast<size_t>(warps) * warp + (cta_merge ? kCtaSmem : 0) +
            (cluster ? kClusterSmem : 0);
 }
 
@@ -2008,15 +2027,20 @@ void launch_attention_t(const PoolView &pool, const RopeView &rope, const BatchV
     int dev = 0;
     cudaGetDevice(&dev);
     configure_attention<kAppend, kCtaMerge, kCluster, kE4m3>(dev);
-    const int grid = (batch.n_warps + kAttnWarps - 1) / kAttnWarps;
+    const int warps = kE4m3 && !kCtaMerge ? batch.cta_warps : kAttnWarps;
+    const int grid = (batch.n_warps + warps - 1) / warps;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(grid));
-    cfg.blockDim = dim3(kAttnWarps * 32);
-    cfg.dynamicSmemBytes = attention_smem_bytes(kCtaMerge, kCluster, kE4m3);
+    cfg.blockDim = dim3(static_cast<unsigned>(warps) * 32);
+    cfg.dynamicSmemBytes = kE4m3 && !kCtaMerge ? static_cast<size_t>(warps) * Ring<true, false>::kWarpSmem
+                                               : attention_smem_bytes(kCtaMerge, kCluster, kE4m3);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     int n_attr = 0;
-    if (overlap_previous) {
+    // The 8-bit kernel is always launched as a dependent of the kernel before it, so
+    // that its CTAs are set up while that one ends (a batch-1 step: 10.5 -> 9.1 us), and
+    // waits at its start where it may not overlap.
+    if (overlap_previous || kE4m3) {
         attr[n_attr].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[n_attr].val.programmaticStreamSerializationAllowed = 1;
         ++n_attr;
@@ -2031,7 +2055,7 @@ void launch_attention_t(const PoolView &pool, const RopeView &rope, const BatchV
     cfg.attrs = attr;
     cfg.numAttrs = static_cast<unsigned>(n_attr);
     cudaLaunchKernelEx(&cfg, attention_kernel<kAppend, kCtaMerge, kCluster, kE4m3>, pool, rope, batch, layer, q,
-                       k_new, v_new, part_o, part_ml, counters, out, xchg, scale_log2, err);
+                       k_new, v_new, part_o, part_ml, counters, out, xchg, scale_log2, err, !overlap_previous);
     if (batch.combine && batch.split_segments > 0) {
         cudaLaunchConfig_t cc = {};
         cc.gridDim = dim3(static_cast<unsigned>(batch.n * pool.n_head_kv * kGqa));

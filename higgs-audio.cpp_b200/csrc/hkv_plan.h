@@ -57,6 +57,17 @@ inline int32_t plan_warps(int64_t total_units, int64_t max_warps) {
     return static_cast<int32_t>(total_units < max_warps ? total_units : max_warps);
 }
 
+// The same for the wide variant of the 8-bit kernel (up to kAttnWarpsE4m3 warps in a
+// CTA per SM, as few as the plan needs): three units a warp, since it takes pages
+// in pairs and every warp adds a partial to merge, but one warp an SM before any
+// has more than two units.  Measured with 1, 2, 3, 4 and 6 units a warp: 16 slots of
+// 16 rows 7.4 / 5.7 / 8.8 / 8.9 / 12.3 us (128, 128, 86 .. warps), 16 of 200 rows 13.3 /
+// 11.6 / 9.0 / 10.6 / 11.7, 32 of 300 rows 15.7 / 15.8 / 14.4 / 14.4 / 15.3.
+inline int32_t plan_wide_warps(int64_t total_units, int64_t sms) {
+    const int64_t want = std::max((total_units + 2) / 3, std::min((total_units + 1) / 2, sms));
+    return static_cast<int32_t>(std::min(want, sms * kAttnWarpsE4m3));
+}
+
 // CTA-level pre-merge pays when a segment spans many warps (a few long
 // requests); with many short segments it only adds shared-memory traffic
 // and footprint.
@@ -95,12 +106,19 @@ constexpr int64_t kCostUnit = 16;
 constexpr int64_t kCostLeaveWhole = 32;
 constexpr int64_t kCostLeaveShared = 80;
 
+// What a plan goes by, of the kernel that runs it.
+struct PlanRules {
+    int64_t leave_whole = kCostLeaveWhole;
+    int64_t leave_shared = kCostLeaveShared;
+    bool cta_merge = true;  // the kernel can merge a CTA's warps in shared memory
+};
+
 // Greedy cut of the segments (segment s has npg[s / G] units) into shares of
 // cost at most B (B >= kCostUnit, so every share holds a unit).  Returns the
 // number of shares, or max_shares + 1 as soon as more are needed; writes each
 // share's first unit to starts[] when starts is not null.
 inline int64_t plan_cut(const int32_t *npg, int32_t G, int64_t S, int64_t B, int64_t max_shares,
-                        int32_t *starts) {
+                        int32_t *starts, const PlanRules &rules = PlanRules{}) {
     int64_t k = 0, s = 0, i = 0, u = 0;  // shares, segment, unit within it, flat unit
     while (s < S) {
         if (k == max_shares) {
@@ -126,7 +144,7 @@ inline int64_t plan_cut(const int32_t *npg, int32_t G, int64_t S, int64_t B, int
             if (s == S) {
                 break;
             }
-            const int64_t leave = from_first_page ? kCostLeaveWhole : kCostLeaveShared;
+            const int64_t leave = from_first_page ? rules.leave_whole : rules.leave_shared;
             if (budget - leave < kCostUnit) {
                 break;  // the next segment opens the next share
             }
@@ -300,11 +318,12 @@ inline void fill_records(const PlanArrays &a, int32_t n, int32_t G, int32_t W,
 // Fills `w` (plan_words(...) words, 16-byte aligned).  page_lists[e] points
 // at slot e's page ids, at least pos[e] / 16 + 1 of them.
 inline PlanSummary build_plan(int32_t *w, int32_t n, int32_t G, const int32_t *pos_in,
-                              const int32_t *const *page_lists, int64_t total_pages, int32_t W) {
+                              const int32_t *const *page_lists, int64_t total_pages, int32_t W,
+                              const PlanRules &rules = PlanRules{}) {
     PlanSummary s;
     s.total_pages = total_pages;
     s.total_units = total_pages * G;
-    s.cta_merge = plan_cta_merge(static_cast<int64_t>(n) * G, W);
+    s.cta_merge = rules.cta_merge && plan_cta_merge(static_cast<int64_t>(n) * G, W);
     const int64_t U = s.total_units;
     const int64_t S = static_cast<int64_t>(n) * G;
     const PlanArrays a = plan_arrays(w, n, G, pos_in, page_lists, W);
@@ -312,13 +331,13 @@ inline PlanSummary build_plan(int32_t *w, int32_t n, int32_t G, const int32_t *p
     // ---- shares: the smallest budget that fits W warps (bisection)
     const int64_t per = (U + W - 1) / W;
     int64_t bad = kCostUnit * per - 1;  // W shares of fewer than per units cannot hold U
-    int64_t good = kCostUnit * per + kCostLeaveShared * (S + 1);
-    while (plan_cut(a.npg, G, S, good, W, nullptr) > W) {
+    int64_t good = kCostUnit * per + rules.leave_shared * (S + 1);
+    while (plan_cut(a.npg, G, S, good, W, nullptr, rules) > W) {
         good *= 2;
     }
     while (good - bad > 1) {
         const int64_t mid = bad + (good - bad) / 2;
-        if (plan_cut(a.npg, G, S, mid, W, nullptr) > W) {
+        if (plan_cut(a.npg, G, S, mid, W, nullptr, rules) > W) {
             bad = mid;
         } else {
             good = mid;
@@ -326,7 +345,7 @@ inline PlanSummary build_plan(int32_t *w, int32_t n, int32_t G, const int32_t *p
     }
     s.budget = good;
     std::vector<int32_t> starts(static_cast<size_t>(W) + 1);
-    s.shares = static_cast<int32_t>(plan_cut(a.npg, G, S, good, W, starts.data()));
+    s.shares = static_cast<int32_t>(plan_cut(a.npg, G, S, good, W, starts.data(), rules));
     for (int64_t k = s.shares; k <= W; ++k) {
         starts[k] = static_cast<int32_t>(U);
     }
@@ -385,6 +404,7 @@ inline BatchView bind_plan(const int32_t *d, int32_t n, int32_t G, const PlanSum
     b.split_segments = s.split_segments;
     b.combine = s.combine ? 1 : 0;
     b.cluster = s.cluster;
+    b.cta_warps = kAttnWarps;
     return b;
 }
 
