@@ -14,9 +14,9 @@
 // without error.
 //   warps 0-3, 4-7  softmax of M tile 0 / 1, a thread a row: S from TMEM, the
 //                   weights back into S's columns as the next product's A operand
-//   warps 8-11      loaders: 16-byte pieces of the pages to F16 operand tiles,
+//   warps 8-10      loaders: 16-byte pieces of the pages to F16 operand tiles,
 //                   through a ring of 32 KiB buffers (K and V tiles in turn)
-//   warp 12         one thread issues every product; while one tile's softmax
+//   warp 11         one thread issues every product; while one tile's softmax
 //                   runs, the other tile's products do
 // F32 tensors: q and the weights in two F16 parts each, hi + lo, which keeps 22
 // bits and doubles the products.  F16 and BF16 tensors: one part.
@@ -52,11 +52,15 @@ constexpr int kTile = 128;              // rows of an M tile: 32 tokens x 4 head
 constexpr int kTileTokens = kTile / kGqa;
 constexpr int kTileBytes = 128 * 128 * 2;
 constexpr int kSoftmaxThreads = 256;
-constexpr int kLoaderThreads = 128;
+constexpr int kLoaderThreads = 96;
+// Twelve warps: 168 registers a thread, which hold a row of 128 logits.
 constexpr int kThreads = kSoftmaxThreads + kLoaderThreads + 32;
+constexpr int kIssuer = kThreads / 32 - 1;
 constexpr int kScaleSlots = 4;          // blocks whose exponents are kept
 constexpr float kSlack = 8.f;
 constexpr int kShift = 7;               // weights enter 2^7 larger: at most 2^15 in F16
+constexpr int kNoPage = INT32_MIN;      // exponent of V where a block has no page
+constexpr int kFar = 60;                // V exponents this far below E take the slow form
 
 template <typename T>
 struct Shape {
@@ -92,6 +96,10 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t half2_sum(uint32_t a, uint32_t b) {
+    const __half2 h = __hadd2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 __device__ __forceinline__ float2 half2_floats(uint32_t u) {
@@ -161,6 +169,89 @@ __device__ float cached_value(const PoolView &pool, int64_t page, int layer, int
         *reinterpret_cast<const __half *>(b + r * kRowBytes + swizzled_chunk(r, d >> 3) * 16 + (d & 7) * 2));
 }
 
+// The issuing thread: S_i = q_i K^T and O_i += P_i V, block by block, the two M tiles
+// in turn.  nb0, nb1: blocks of each tile.
+template <typename T>
+__device__ __forceinline__ void issue_products(Control *ctl, uint8_t *q_smem, uint8_t *ring, uint32_t tmem, int nb0,
+                                               int nb1, DeviceError *err) {
+    using S = Shape<T>;
+    const int nb = max(nb0, nb1);
+    constexpr uint32_t qk_desc = f16_idesc(kTile, kKeys, false);
+    constexpr uint32_t pv_desc = f16_idesc(kTile, kHeadDim, true);
+    const uint32_t q_addr = smem_u32(q_smem);
+    const uint32_t ring_addr = smem_u32(ring);
+    auto full = [&](int seq) {
+        return wait_for(&ctl->kv_full[seq % S::kRing], (seq / S::kRing) & 1, err);
+    };
+    auto logits = [&](int i, int seq) {  // S_i = q_i K^T
+        const uint32_t kb = ring_addr + (seq % S::kRing) * kTileBytes;
+#pragma unroll
+        for (int part = 0; part < S::kParts; ++part) {
+            const uint32_t qa = q_addr + (i * S::kParts + part) * kTileBytes;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t step = (k >> 2) * (kTileBytes / 2) + (k & 3) * 32;
+                mma_ss(tmem + i * kKeys, smem_desc(qa + step, 16, 1024), smem_desc(kb + step, 16, 1024), qk_desc,
+                       part > 0 || k > 0);
+            }
+        }
+        tc_commit(smem_u32(&ctl->s_full[i]));
+    };
+    auto weigh = [&](int i, int seq, bool accumulate) {  // O_i += P_i V
+        const uint32_t vb = ring_addr + (seq % S::kRing) * kTileBytes;
+#pragma unroll
+        for (int part = 0; part < S::kParts; ++part) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t p = tmem + i * kKeys + (k >> 1) * 32 + part * 16 + (k & 1) * 8;
+                mma_ts(tmem + 256 + i * kHeadDim, p, smem_desc(vb + k * 2048, kTileBytes / 2, 1024), pv_desc,
+                       accumulate || part > 0 || k > 0);
+            }
+        }
+    };
+    const int n_blocks[2] = {nb0, nb1};
+    bool ok = nb > 0 && wait_for(&ctl->q_full, 0, err) && full(0);
+    if (ok) {
+        for (int i = 0; i < 2; ++i) {
+            if (n_blocks[i] > 0) {
+                logits(i, 0);
+            }
+        }
+        tc_commit(smem_u32(&ctl->kv_empty[0]));
+    }
+    for (int j = 0; ok && j < nb; ++j) {
+        const int v_seq = 2 * j + 1;
+        ok = full(v_seq) && (j + 1 >= nb || full(v_seq + 1));
+        for (int i = 0; ok && i < 2; ++i) {
+            if (j >= n_blocks[i]) {
+                continue;
+            }
+            ok = wait_for(&ctl->p_full[i], j & 1, err);
+            if (!ok) {
+                break;
+            }
+            tc_fence_after();
+            weigh(i, v_seq, j > 0);
+            if (j + 1 < n_blocks[i]) {
+                logits(i, v_seq + 1);
+            } else {
+                tc_commit(smem_u32(&ctl->o_full[i]));
+            }
+        }
+        if (ok) {
+            tc_commit(smem_u32(&ctl->kv_empty[v_seq % S::kRing]));
+            if (j + 1 < nb) {
+                tc_commit(smem_u32(&ctl->kv_empty[(v_seq + 1) % S::kRing]));
+            }
+        }
+    }
+    if (!ok && nb > 0) {
+        // products in flight end before the memory they use is given up
+        tc_commit(smem_u32(&ctl->drained));
+        mbar_wait_bounded(smem_u32(&ctl->drained), 0);
+    }
+}
+
 template <typename T, bool kE4m3>
 __global__ void __launch_bounds__(kThreads, 1)
     window_kernel(PoolView pool, const WindowTile *__restrict__ tiles, const int32_t *__restrict__ pages, int layer,
@@ -183,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int nb1 = n_tiles == 2 ? t.blocks : 0;
     const int nb = max(nb0, nb1);
 
-    if (warp == 12) {
+    if (warp == kIssuer) {
         tmem_alloc(smem_u32(&ctl->tmem), 512);
     }
     if (threadIdx.x == 0) {
@@ -252,37 +343,39 @@ __global__ void __launch_bounds__(kThreads, 1)
                 break;
             }
             tc_fence_after();
+            float s[kKeys];
+            tmem_load128(s_col, s);
             const float *ks = ctl->k_scale[j % kScaleSlots];
             const int *ve = ctl->v_exp[j % kScaleSlots];
-            const bool masked = j * kKeys + kKeys - 1 > first_last;
-            const int lim = my_last - j * kKeys;  // columns 0 .. lim are seen
+            if (j * kKeys + kKeys - 1 > first_last) {
+                const int lim = my_last - j * kKeys;  // columns 0 .. lim are seen
+#pragma unroll
+                for (int k = 0; k < kKeys; ++k) {
+                    s[k] = k <= lim ? s[k] : -INFINITY;
+                }
+            }
             float mx = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                float s[32];
-                tmem_load32(s_col + 32 * c, s);
-                if (masked) {
+            for (int p = 0; p < kBlockPages; ++p) {
+                float a = s[16 * p], b = s[16 * p + 1];
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) {
-                        s[k] = 32 * c + k <= lim ? s[k] : -INFINITY;
-                    }
+                for (int k = 2; k < 16; k += 2) {
+                    a = fmaxf(a, s[16 * p + k]);
+                    b = fmaxf(b, s[16 * p + k + 1]);
                 }
-#pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    float a = s[16 * p];
-#pragma unroll
-                    for (int k = 1; k < 16; ++k) {
-                        a = fmaxf(a, s[16 * p + k]);
-                    }
-                    mx = fmaxf(mx, a * ks[2 * c + p]);
-                }
+                mx = fmaxf(mx, fmaxf(a, b) * ks[p]);
             }
             // the bound and E move (o has to follow) only when they must
             int e_new = e_v;
+            bool far = false;
             if (kE4m3) {
 #pragma unroll
                 for (int p = 0; p < kBlockPages; ++p) {
                     e_new = max(e_new, ve[p]);
+                }
+#pragma unroll
+                for (int p = 0; p < kBlockPages; ++p) {
+                    far = far || (ve[p] != kNoPage && ve[p] < e_new - kFar);
                 }
             }
             const bool move = mx > m + kSlack || e_new > e_v;
@@ -294,52 +387,65 @@ __global__ void __launch_bounds__(kThreads, 1)
                 e_v = e_new;
                 l *= corr;
                 if (j > 0) {
-                    for (int c = 0; c < 4; ++c) {
-                        float o[32];
-                        tmem_load32(o_col + 32 * c, o);
+#pragma unroll 1
+                    for (int c = 0; c < kHeadDim; c += 16) {
+                        float o[16];
+                        tmem_load16(o_col + c, o);
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) {
+                        for (int k = 0; k < 16; ++k) {
                             o[k] *= o_corr;
                         }
-                        tmem_store32(o_col + 32 * c, o);
+                        tmem_store16(o_col + c, reinterpret_cast<const uint32_t (&)[16]>(o));
                     }
                 }
             }
             const float bound = (m == -INFINITY ? 0.f : m) - kShift;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                float s[32];
-                tmem_load32(s_col + 32 * c, s);
-                if (masked) {
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) {
-                        s[k] = 32 * c + k <= lim ? s[k] : -INFINITY;
-                    }
-                }
                 uint32_t hi[16], lo[16];
 #pragma unroll
                 for (int p = 0; p < 2; ++p) {
-                    const float scale = ks[2 * c + p];
-                    const float weigh = kE4m3 ? pow2(max(ve[2 * c + p] - e_v, -126)) : 1.f;
-                    float sum = 0.f;
+                    // 2^(eV - E) belongs to the weight and not to l: in the exponent, and
+                    // taken out of the page's sum again; where that could underflow
+                    // (V pages 2^60 apart), by a product instead
+                    const int page = 2 * c + p;
+                    const float scale = ks[page];
+                    const int d = kE4m3 && ve[page] != kNoPage ? ve[page] - e_v : 0;
+                    const float off = (kE4m3 && !far ? static_cast<float>(d) : 0.f) - bound;
+                    float *x = s + 16 * page;
+                    float sum = 0.f, sum2 = 0.f;
+#pragma unroll
+                    for (int k = 0; k < 16; k += 2) {
+                        x[k] = exp2_fast(fmaf(x[k], scale, off));
+                        x[k + 1] = exp2_fast(fmaf(x[k + 1], scale, off));
+                        sum += x[k];
+                        sum2 += x[k + 1];
+                    }
+                    sum += sum2;
+                    if (kE4m3) {
+                        if (far) {
+                            const float w = pow2(max(d, -126));
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) {
+                                x[k] *= w;
+                            }
+                            l += sum;
+                        } else {
+                            l = fmaf(sum, pow2(-d), l);
+                        }
+                    } else {
+                        l += sum;
+                    }
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
-                        float a = exp2_fast(fmaf(s[16 * p + 2 * k], scale, -bound));
-                        float b = exp2_fast(fmaf(s[16 * p + 2 * k + 1], scale, -bound));
-                        sum += a + b;
-                        if (kE4m3) {
-                            a *= weigh;
-                            b *= weigh;
-                        }
-                        hi[8 * p + k] = half2_bits(a, b);
+                        hi[8 * p + k] = half2_bits(x[2 * k], x[2 * k + 1]);
                         if (S::kSplit) {
                             const float2 f = half2_floats(hi[8 * p + k]);
-                            lo[8 * p + k] = half2_bits(a - f.x, b - f.y);
+                            lo[8 * p + k] = half2_bits(x[2 * k] - f.x, x[2 * k + 1] - f.y);
                         }
                     }
-                    l += sum;
                 }
-                // in place of the columns just read: 16 columns of hi, 16 of lo
+                // in place of the logits: 16 columns of hi, 16 of lo per 32 keys
                 tmem_store16(s_col + 32 * c, hi);
                 if (S::kSplit) {
                     tmem_store16(s_col + 32 * c + 16, lo);
@@ -409,219 +515,173 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             tc_fence_before();
         }
-    } else if (warp < 12) {
+    } else if (warp < kIssuer) {
         // ------------------------------------------------------------ loaders
         const int tid = threadIdx.x - kSoftmaxThreads;
         const int n_pages = (t.pos0 + t.tokens - 1) / kPageTokens + 1;  // of the slot, up to its last key here
-        constexpr int kPieces = kE4m3 ? kBlockPages : 2 * kBlockPages;  // 16-byte pieces per thread and tile
-        uint4 raw[kPieces];
-        // Piece p of tile `seq` (K of block seq / 2, or V): E4M3, 16 codes of row
-        // tid / 8 of page p; F16, 8 values of row tid / 16 (+ 8) of page p / 2.
-        auto fetch = [&](int seq) {
-            const int first = (t.key0 + (seq >> 1) * kKeys) / kPageTokens;
-            const int kv = seq & 1;
+        // A block is filled in steps of 1024 16-byte pieces: K, V (8-bit cache) or the
+        // two halves of K, then of V (F16).  Two steps' pieces are in registers: a
+        // step's loads go out when the step two before it is stored.  A piece: 8 bits,
+        // 16 dims of a row of one of 8 pages; F16, 8 dims of a row of one of 4.
+        // Eight consecutive threads store to eight different bank groups: 8 bits, dims
+        // 0-63 or 64-127 of two neighbouring rows (an even and an odd row's swizzles
+        // interleave); F16, half a row.
+        constexpr int kSteps = kE4m3 ? 2 : 4;
+        constexpr int kAhead = 2;
+        constexpr int kPieces = 1024;
+        constexpr int kEach = (kPieces + kLoaderThreads - 1) / kLoaderThreads;
+        static_assert(kLoaderThreads % 16 == 0, "a thread keeps its place in the row");
+        const int c = kE4m3 ? ((tid >> 3) & 1) * 4 + (tid & 3) : tid & 15;  // piece of the row
+        const int row0 = kE4m3 ? 2 * (tid >> 4) + ((tid >> 2) & 1) : tid >> 4;
+        constexpr int kRowStep = (kE4m3 ? 2 : 1) * kLoaderThreads / 16;
+        const int64_t page_stride = static_cast<int64_t>(G) * cache_unit_bytes(pool.format);
+        const uint8_t *base = pool.base + static_cast<int64_t>(layer) * pool.n_pages * page_stride +
+                              h * (kE4m3 ? kCodeUnitBytes : kHeadBlockBytes);
+        const int64_t v_off = kE4m3 ? kCodeBlockBytes : static_cast<int64_t>(G) * kHeadBlockBytes;
+        const int32_t *list = pages + t.page_off + t.key0 / kPageTokens;
+        const int last_page = n_pages - 1 - t.key0 / kPageTokens;
+        int bad = -1;
+        // Past the slot's pages its last one is read again: K there is masked, V zeroed.
+        auto page_at = [&](int index) {
+            int page = list[min(index, last_page)];
+            if (page >= pool.n_pages || page < 0) {
+                bad = index;
+                page = 0;
+            }
+            return page;
+        };
+        uint4 raw[kAhead][kEach];
+        auto fetch = [&](int j, int step, uint4 (&to)[kEach]) {
+            const uint8_t *from = base + (step * 2 / kSteps == 1 ? v_off : 0);
+            const int first = j * kBlockPages + (kE4m3 ? 0 : (step & 1) * 4);
+            int page[kEach];
 #pragma unroll
-            for (int p = 0; p < kBlockPages; ++p) {
-                int64_t page = -1;
-                if (first + p < n_pages) {
-                    page = pages[t.page_off + first + p];
-                    if (page < 0 || page >= pool.n_pages) {
-                        record(err, kErrBadIndex, static_cast<int>(page), first + p);
-                        page = -1;
-                    }
-                }
-                if (kE4m3) {
-                    raw[p] = make_uint4(0, 0, 0, 0);
-                    if (page >= 0) {
-                        const uint8_t *unit =
-                            pool.base + code_unit_index(page, layer, h, pool.n_pages, G) * kCodeUnitBytes;
-                        raw[p] = *reinterpret_cast<const uint4 *>(unit + kv * kCodeBlockBytes + tid * 16);
-                    }
-                } else {
-                    const uint8_t *b =
-                        pool.base + head_block_index(page, layer, kv, h, pool.n_pages, G) * kHeadBlockBytes;
-                    raw[2 * p] = raw[2 * p + 1] = make_uint4(0, 0, 0, 0);
-                    if (page >= 0) {
-                        raw[2 * p] = *reinterpret_cast<const uint4 *>(b + tid * 16);
-                        raw[2 * p + 1] = *reinterpret_cast<const uint4 *>(b + kHeadBlockBytes / 2 + tid * 16);
-                    }
-                }
+            for (int i = 0; i < kEach; ++i) {
+                page[i] = page_at(first + ((row0 + i * kRowStep) >> 4));
+            }
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const int row = (row0 + i * kRowStep) & 15;
+                to[i] = *reinterpret_cast<const uint4 *>(from + page[i] * page_stride +
+                                                         row * (kE4m3 ? kHeadDim : kRowBytes) +
+                                                         ((c ^ (row & 7)) << 4));
             }
         };
         const int last_key = t.pos0 + t.tokens - 1 - t.key0;
-        bool odd = false;
-        fetch(0);
-        for (int seq = 0; seq < 2 * nb; ++seq) {
-            const int slot = seq % S::kRing;
-            const bool is_v = (seq & 1) != 0;
-            if (seq >= S::kRing && !wait_for(&ctl->kv_empty[slot], (seq / S::kRing - 1) & 1, err)) {
-                break;
-            }
-            const uint32_t buf = smem_u32(ring) + slot * kTileBytes;
-            if (!is_v && tid < kBlockPages) {
-                // the exponents of both K and V of the block, with the K tile
-                const int j = seq >> 1;
-                const int first = (t.key0 + j * kKeys) / kPageTokens + tid;
-                int ek = 0, ev = kE4m3 ? kExpMin : 0;
-                if (kE4m3 && first < n_pages) {
-                    const int64_t page = pages[t.page_off + first];
-                    if (page >= 0 && page < pool.n_pages) {
-                        const int *e = reinterpret_cast<const int *>(
-                            pool.base + code_unit_index(page, layer, h, pool.n_pages, G) * kCodeUnitBytes +
-                            2 * kCodeBlockBytes);
-                        ek = e[0];
-                        ev = e[1];
-                    }
+        auto put = [&](int j, int step, const uint4 (&from)[kEach], uint32_t buf) {
+            const bool is_v = step * 2 / kSteps == 1;
+            const bool tail = is_v && j * kKeys + kKeys - 1 > last_key;
+            bool odd = false;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const int row = (kE4m3 ? 0 : 64 * (step & 1)) + row0 + i * kRowStep;
+                if (i == kEach - 1 && tid + i * kLoaderThreads >= kPieces) {
+                    break;
                 }
-                ctl->k_scale[j % kScaleSlots][tid] = scale_log2 * pow2(ek);
-                ctl->v_exp[j % kScaleSlots][tid] = ev;
-            }
+                uint32_t w[4] = {from[i].x, from[i].y, from[i].z, from[i].w};
+                // rows past the last key hold whatever the page had before
+                if (tail && j * kKeys + row > last_key) {
+                    w[0] = w[1] = w[2] = w[3] = 0;
+                }
+                uint32_t x[kE4m3 ? 8 : 4];
 #pragma unroll
-            for (int p = 0; p < kPieces; ++p) {
-                uint32_t w[4] = {raw[p].x, raw[p].y, raw[p].z, raw[p].w};
-                if (kE4m3) {
-                    const int r = tid >> 3;
-                    const int c = (tid & 7) ^ (r & 7);  // dims 16c .. 16c + 15
-                    if (is_v) {
-                        // rows past the last key held whatever the page had before
-                        if ((seq >> 1) * kKeys + 16 * p + r > last_key) {
-                            w[0] = w[1] = w[2] = w[3] = 0;
-                        }
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const uint32_t nan = ((w[k] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-                            if (nan != 0) {
-                                w[k] &= ~((nan >> 7) * 0xffu);
-                                odd = true;
-                            }
-                        }
-                    }
-                    uint32_t x[8];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
+                for (int k = 0; k < 4; ++k) {
+                    if (kE4m3) {
                         x[2 * k] = codes_to_half2(w[k]);
                         x[2 * k + 1] = codes_to_half2_hi(w[k]);
+                    } else {
+                        x[k] = w[k];
                     }
-                    const int row = 16 * p + r;
-                    const uint32_t a = buf + tile_offset(kKeys, row, 2 * c);
-                    const uint32_t b = buf + tile_offset(kKeys, row, 2 * c + 1);
-                    // the two halves of the tile share their banks: the lanes of the
-                    // upper one store their pieces in the other order
-                    const bool swap = c >= 4;
-                    st_shared16(swap ? b : a, swap ? x[4] : x[0], swap ? x[5] : x[1], swap ? x[6] : x[2],
-                                swap ? x[7] : x[3]);
-                    st_shared16(swap ? a : b, swap ? x[0] : x[4], swap ? x[1] : x[5], swap ? x[2] : x[6],
-                                swap ? x[3] : x[7]);
-                } else {
-                    const int r = (tid >> 4) + (p & 1) * 8;
-                    const int c = (tid & 15) ^ (r & 7);
-                    const int row = 16 * (p >> 1) + r;
-                    if (is_v) {
-                        if ((seq >> 1) * kKeys + row > last_key) {
-                            w[0] = w[1] = w[2] = w[3] = 0;
-                        }
+                }
+                if (is_v) {
+                    // a sum that is not finite: look at each (an F16 sum may overflow)
+                    uint32_t sum = x[0];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const uint32_t bad = ((w[k] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
-                            if (bad != 0) {
-                                w[k] &= ~((bad >> 15) * 0xffffu);
-                                odd = true;
-                            }
+                    for (int k = 1; k < (kE4m3 ? 8 : 4); ++k) {
+                        sum = half2_sum(sum, x[k]);
+                    }
+                    if ((((sum & 0x7c007c00u) + 0x04000400u) & 0x80008000u) != 0) {
+#pragma unroll
+                        for (int k = 0; k < (kE4m3 ? 8 : 4); ++k) {
+                            const uint32_t out = ((x[k] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+                            odd = odd || out != 0;
+                            x[k] &= ~((out >> 15) * 0xffffu);
                         }
                     }
-                    st_shared16(buf + tile_offset(kKeys, row, c), w[0], w[1], w[2], w[3]);
+                }
+                if (kE4m3) {
+                    st_shared16(buf + tile_offset(kKeys, row, 2 * c), x[0], x[1], x[2], x[3]);
+                    st_shared16(buf + tile_offset(kKeys, row, 2 * c + 1), x[kE4m3 ? 4 : 0], x[kE4m3 ? 5 : 0],
+                                x[kE4m3 ? 6 : 0], x[kE4m3 ? 7 : 0]);
+                } else {
+                    st_shared16(buf + tile_offset(kKeys, row, c), x[0], x[1], x[2], x[3]);
                 }
             }
             if (odd) {
                 *reinterpret_cast<volatile int *>(&ctl->odd_v) = 1;
             }
-            if (seq + 1 < 2 * nb) {
-                fetch(seq + 1);
-            }
-            fence_proxy_async_smem();
-            mbar_arrive(smem_u32(&ctl->kv_full[slot]));
-        }
-    } else if (lane == 0) {
-        // ----------------------------------------------------------- products
-        constexpr uint32_t qk_desc = f16_idesc(kTile, kKeys, false);
-        constexpr uint32_t pv_desc = f16_idesc(kTile, kHeadDim, true);
-        const uint32_t q_addr = smem_u32(q_smem);
-        const uint32_t ring_addr = smem_u32(ring);
-        auto full = [&](int seq) {
-            return wait_for(&ctl->kv_full[seq % S::kRing], (seq / S::kRing) & 1, err);
         };
-        auto logits = [&](int i, int seq) {  // S_i = q_i K^T
-            const uint32_t kb = ring_addr + (seq % S::kRing) * kTileBytes;
-#pragma unroll
-            for (int part = 0; part < S::kParts; ++part) {
-                const uint32_t qa = q_addr + (i * S::kParts + part) * kTileBytes;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const uint32_t step = (k >> 2) * (kTileBytes / 2) + (k & 3) * 32;
-                    mma_ss(tmem + i * kKeys, smem_desc(qa + step, 16, 1024), smem_desc(kb + step, 16, 1024), qk_desc,
-                           part > 0 || k > 0);
-                }
-            }
-            tc_commit(smem_u32(&ctl->s_full[i]));
-        };
-        auto weigh = [&](int i, int seq, bool accumulate) {  // O_i += P_i V
-            const uint32_t vb = ring_addr + (seq % S::kRing) * kTileBytes;
-#pragma unroll
-            for (int part = 0; part < S::kParts; ++part) {
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const uint32_t p = tmem + i * kKeys + (k >> 1) * 32 + part * 16 + (k & 1) * 8;
-                    mma_ts(tmem + 256 + i * kHeadDim, p, smem_desc(vb + k * 2048, kTileBytes / 2, 1024), pv_desc,
-                           accumulate || part > 0 || k > 0);
+        // The exponents of a block's K and V, with its K tile: thread p takes page p's.
+        int2 exps = make_int2(0, kNoPage);
+        auto fetch_exponents = [&](int j) {
+            if (kE4m3 && tid < kBlockPages) {
+                const int index = j * kBlockPages + tid;
+                exps = *reinterpret_cast<const int2 *>(base + page_at(index) * page_stride + 2 * kCodeBlockBytes);
+                if (index > last_page) {
+                    exps.y = kNoPage;
                 }
             }
         };
-        const int n_blocks[2] = {nb0, nb1};
-        bool ok = nb > 0 && wait_for(&ctl->q_full, 0, err) && full(0);
-        if (ok) {
-            for (int i = 0; i < 2; ++i) {
-                if (n_blocks[i] > 0) {
-                    logits(i, 0);
-                }
-            }
-            tc_commit(smem_u32(&ctl->kv_empty[0]));
-        }
+        fetch(0, 0, raw[0]);
+        fetch(0, 1, raw[1]);
+        fetch_exponents(0);
+        bool ok = true;
         for (int j = 0; ok && j < nb; ++j) {
-            const int v_seq = 2 * j + 1;
-            ok = full(v_seq) && (j + 1 >= nb || full(v_seq + 1));
-            for (int i = 0; ok && i < 2; ++i) {
-                if (j >= n_blocks[i]) {
-                    continue;
+#pragma unroll
+            for (int step = 0; step < kSteps; ++step) {
+                const int seq = 2 * j + step * 2 / kSteps;  // the operand tile
+                const int slot = seq % S::kRing;
+                const bool first_step = step % (kSteps / 2) == 0;
+                const bool last_step = (step + 1) % (kSteps / 2) == 0;
+                if (first_step && seq >= S::kRing) {
+                    ok = ok && wait_for(&ctl->kv_empty[slot], (seq / S::kRing - 1) & 1, err);
                 }
-                ok = wait_for(&ctl->p_full[i], j & 1, err);
                 if (!ok) {
                     break;
                 }
-                tc_fence_after();
-                weigh(i, v_seq, j > 0);
-                if (j + 1 < n_blocks[i]) {
-                    logits(i, v_seq + 1);
-                } else {
-                    tc_commit(smem_u32(&ctl->o_full[i]));
+                if (step == 0 && tid < kBlockPages) {
+                    ctl->k_scale[j % kScaleSlots][tid] = scale_log2 * pow2(exps.x);
+                    ctl->v_exp[j % kScaleSlots][tid] = exps.y;
                 }
-            }
-            if (ok) {
-                tc_commit(smem_u32(&ctl->kv_empty[v_seq % S::kRing]));
-                if (j + 1 < nb) {
-                    tc_commit(smem_u32(&ctl->kv_empty[(v_seq + 1) % S::kRing]));
+                put(j, step, raw[step % kAhead], smem_u32(ring) + slot * kTileBytes);
+                if (last_step) {
+                    fence_proxy_async_smem();
+                    mbar_arrive(smem_u32(&ctl->kv_full[slot]));
+                }
+                if (step + kAhead < kSteps) {
+                    fetch(j, step + kAhead, raw[step % kAhead]);
+                } else if (j + 1 < nb) {
+                    fetch(j + 1, step + kAhead - kSteps, raw[step % kAhead]);
+                    if (step + kAhead == kSteps) {
+                        fetch_exponents(j + 1);
+                    }
                 }
             }
         }
-        if (!ok && nb > 0) {
-            // products in flight end before the memory they use is given up
-            tc_commit(smem_u32(&ctl->drained));
-            mbar_wait_bounded(smem_u32(&ctl->drained), 0);
+        if (bad >= 0) {
+            record(err, kErrBadIndex, list[min(bad, last_page)], bad);
+        }
+    } else {
+        // ----------------------------------------------------------- products
+        if (lane == 0) {
+            issue_products<T>(ctl, q_smem, ring, tmem, nb0, nb1, err);
         }
     }
+
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 12) {
+    if (warp == kIssuer) {
         __syncwarp();
         tmem_free(tmem, 512);
     }
