@@ -14,10 +14,15 @@
 // without error.
 //   warps 0-3, 4-7  softmax of M tile 0 / 1, a thread a row: S from TMEM, the
 //                   weights back into S's columns as the next product's A operand
-//   warps 8-10      loaders: 16-byte pieces of the pages to F16 operand tiles,
-//                   through a ring of 32 KiB buffers (K and V tiles in turn)
-//   warp 11         one thread issues every product; while one tile's softmax
+//   warps 8-13      converters: 16-byte pieces of the pages to F16 operand tiles
+//   warp 14         exponents of each block, and K as it is where q is in E4M3 parts
+//   warp 15         one thread issues every product; while one tile's softmax
 //                   runs, the other tile's products do
+//
+// BF16 tensors on an 8-bit cache: q has 8 significant bits, two E4M3 numbers of 4
+// (with a power of two per row), so q K^T is two E4M3 products at twice the F16 rate
+// and K goes from its pages to shared memory by bulk copies, unconverted: a page's
+// code block is the 128-byte-swizzled operand tile already.
 // F32 tensors: q and the weights in two F16 parts each, hi + lo, which keeps 22
 // bits and doubles the products.  F16 and BF16 tensors: one part.
 //
@@ -31,6 +36,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "hkv_device.cuh"
 #include "hkv_e4m3.cuh"
@@ -46,40 +53,68 @@ constexpr int kWhereWindow = 8;
 constexpr int kDtypeF32 = 0;
 constexpr int kDtypeF16 = 1;
 
-constexpr int kKeys = 128;              // keys of a block
+constexpr int kKeys = kWindowKeys;      // keys of a block
 constexpr int kBlockPages = kKeys / kPageTokens;
 constexpr int kTile = 128;              // rows of an M tile: 32 tokens x 4 heads
 constexpr int kTileTokens = kTile / kGqa;
-constexpr int kTileBytes = 128 * 128 * 2;
+constexpr int kTileBytes = 128 * 128 * 2;   // an F16 operand tile (q rows, keys)
+constexpr int kCodeTileBytes = 128 * 128;   // an E4M3 one
+static_assert(kKeys == 128 && kTile == 128, "operand tiles are 128 x 128");
 constexpr int kSoftmaxThreads = 256;
-constexpr int kLoaderThreads = 96;
-// Twelve warps: 168 registers a thread, which hold a row of 128 logits.
-constexpr int kThreads = kSoftmaxThreads + kLoaderThreads + 32;
-constexpr int kIssuer = kThreads / 32 - 1;
-constexpr int kScaleSlots = 4;          // blocks whose exponents are kept
+constexpr int kConvertThreads = 192;
+constexpr int kScaleWarp = 14;
+constexpr int kIssuer = 15;
+constexpr int kThreads = 512;
+// Registers of a thread: the launch gives 128 to each, the softmax, which holds a
+// row of 128 logits, takes what the other two warpgroups leave.  (184 / 72: the
+// converters spill what they prefetch and bound the kernel, 1.09 ms at 8,100 tokens;
+// 176 / 80 0.87; 168 / 88 0.81; 160 / 96 0.80.)
+constexpr int kSoftmaxRegs = 160;
+constexpr int kOtherRegs = 96;
+static_assert(2 * kSoftmaxRegs + 2 * kOtherRegs == 4 * 128, "the shares add up to the launch's registers");
+// Blocks whose scales are kept.  Those of block j are written once the products of
+// q and K of block j - kKSlots (at most 4) are done, when a softmax may still be at
+// that block.
+constexpr int kScaleSlots = 8;
 constexpr float kSlack = 8.f;
 constexpr int kShift = 7;               // weights enter 2^7 larger: at most 2^15 in F16
-constexpr int kNoPage = INT32_MIN;      // exponent of V where a block has no page
 constexpr int kFar = 60;                // V exponents this far below E take the slow form
 
-template <typename T>
+template <typename T, bool kE4m3>
 struct Shape {
     static constexpr bool kSplit = sizeof(T) == 4;
-    static constexpr int kParts = kSplit ? 2 : 1;  // F16 parts of q and of the weights
-    static constexpr int kRing = kSplit ? 3 : 5;   // operand tiles beside q in 224 KiB
-    static constexpr int kQBytes = 2 * kParts * kTileBytes;
-    static constexpr int kSmem = kQBytes + kRing * kTileBytes + 1024;
+    static constexpr bool kCodeK = kE4m3 && std::is_same<T, __nv_bfloat16>::value;
+    static constexpr int kParts = kSplit || kCodeK ? 2 : 1;  // of q
+    static constexpr int kQPart = kCodeK ? kCodeTileBytes : kTileBytes;
+    static constexpr int kKTile = kCodeK ? kCodeTileBytes : kTileBytes;
+    static constexpr int kKSlots = kSplit ? 1 : kCodeK ? 4 : 2;
+    static constexpr int kVSlots = kSplit ? 2 : 3;
+    static constexpr int kQBytes = 2 * kParts * kQPart;
+    static constexpr int kSmem = kQBytes + kKSlots * kKTile + kVSlots * kTileBytes + 3072;
+    static_assert(kSmem <= 227 * 1024, "operands exceed shared memory");
+};
+
+// What the softmax needs of a block's pages.
+struct BlockScale {
+    float k_scale[kBlockPages];  // scale * log2(e) * 2^eK
+    float shift[kBlockPages];    // of the exponent: kShift + eV - E
+    float back[kBlockPages];     // 2^(E - eV): takes eV - E out of the sum of the weights again
+    float grow;                  // 2^(E before - E)
+    int e;                       // E: the largest eV of the CTA's blocks so far
+    int far;                     // some eV - E < -kFar: shift is kShift, the weights times 1 / back
+    int unused;
 };
 
 struct Control {
-    uint64_t q_full, s_full[2], p_full[2], o_full[2], kv_full[5], kv_empty[5];
+    uint64_t q_full, s_full[2], p_full[2], o_full[2];
+    uint64_t k_full[4], k_empty[4], v_full[3], v_empty[3];
     uint64_t drained;                           // after a wait that ran out: no product in flight
     uint32_t tmem;
     int odd_v;                                  // a V value that is not finite was met
-    float k_scale[kScaleSlots][kBlockPages];    // scale * log2(e) * 2^eK
-    int v_exp[kScaleSlots][kBlockPages];
+    BlockScale scale[kScaleSlots];
+    int q_exp[2][kTile];                        // of a row of q in E4M3 parts
 };
-static_assert(sizeof(Control) <= 1024, "the control block has 1 KiB");
+static_assert(sizeof(Control) <= 3072, "the control block has 3 KiB");
 
 __device__ __forceinline__ void record(DeviceError *err, int code, int a, int b) {
     if (atomicCAS(&err->code, 0, code) == 0) {
@@ -107,6 +142,15 @@ __device__ __forceinline__ float2 half2_floats(uint32_t u) {
 }
 __device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ void st_shared8(uint32_t addr, uint32_t a, uint32_t b) {
+    asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(addr), "r"(a), "r"(b) : "memory");
+}
+// L2 policy of K, which the CTAs of other query tiles read again.
+__device__ __forceinline__ uint64_t keep_policy() {
+    uint64_t policy;
+    asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
+    return policy;
 }
 __device__ __forceinline__ void load8(const float *p, float (&x)[8]) {
     const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
@@ -146,9 +190,29 @@ __device__ __forceinline__ void store4(__nv_bfloat16 *p, const float *x) {
 
 // A wait of one role.  One that runs out is recorded and ends its role; the waits
 // that depend on it run out in turn, and the CTA leaves.
+// The threads sleep in try_wait (20 us at a time), so that they leave the issue
+// slots to the warps that work.
+__device__ __forceinline__ bool try_wait_long(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(20000u)
+        : "memory");
+    return ok != 0;
+}
 __device__ __forceinline__ bool wait_for(uint64_t *bar, uint32_t parity, DeviceError *err) {
-    if (mbar_wait_bounded(smem_u32(bar), parity)) {
+    const uint32_t at = smem_u32(bar);
+    if (try_wait_long(at, parity)) {
         return true;
+    }
+    const long long t0 = clock64();
+    while (clock64() - t0 < kWaitBudgetCycles) {
+        if (try_wait_long(at, parity)) {
+            return true;
+        }
     }
     record(err, kErrTimeout, static_cast<int>(blockIdx.x), static_cast<int>(threadIdx.x));
     return false;
@@ -169,59 +233,82 @@ __device__ float cached_value(const PoolView &pool, int64_t page, int layer, int
         *reinterpret_cast<const __half *>(b + r * kRowBytes + swizzled_chunk(r, d >> 3) * 16 + (d & 7) * 2));
 }
 
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(d)
+        : "l"(*reinterpret_cast<const uint64_t *>(&a)), "l"(*reinterpret_cast<const uint64_t *>(&b)),
+          "l"(*reinterpret_cast<const uint64_t *>(&c)));
+    return *reinterpret_cast<const float2 *>(&d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(d)
+        : "l"(*reinterpret_cast<const uint64_t *>(&a)), "l"(*reinterpret_cast<const uint64_t *>(&b)));
+    return *reinterpret_cast<const float2 *>(&d);
+}
+
 // The issuing thread: S_i = q_i K^T and O_i += P_i V, block by block, the two M tiles
 // in turn.  nb0, nb1: blocks of each tile.
-template <typename T>
-__device__ __forceinline__ void issue_products(Control *ctl, uint8_t *q_smem, uint8_t *ring, uint32_t tmem, int nb0,
-                                               int nb1, DeviceError *err) {
-    using S = Shape<T>;
+template <class S>
+__device__ __forceinline__ void issue_products(Control *ctl, uint32_t q_addr, uint32_t k_ring, uint32_t v_ring,
+                                               uint32_t tmem, int nb0, int nb1, DeviceError *err) {
     const int nb = max(nb0, nb1);
-    constexpr uint32_t qk_desc = f16_idesc(kTile, kKeys, false);
-    constexpr uint32_t pv_desc = f16_idesc(kTile, kHeadDim, true);
-    const uint32_t q_addr = smem_u32(q_smem);
-    const uint32_t ring_addr = smem_u32(ring);
-    auto full = [&](int seq) {
-        return wait_for(&ctl->kv_full[seq % S::kRing], (seq / S::kRing) & 1, err);
+    constexpr uint32_t qk_desc = mma_idesc(kTile, kKeys, false);
+    constexpr uint32_t pv_desc = mma_idesc(kTile, kHeadDim, true);
+    auto k_ready = [&](int j) {
+        return wait_for(&ctl->k_full[j % S::kKSlots], (j / S::kKSlots) & 1, err);
     };
-    auto logits = [&](int i, int seq) {  // S_i = q_i K^T
-        const uint32_t kb = ring_addr + (seq % S::kRing) * kTileBytes;
+    auto v_ready = [&](int j) {
+        return wait_for(&ctl->v_full[j % S::kVSlots], (j / S::kVSlots) & 1, err);
+    };
+    auto logits = [&](int i, int j) {  // S_i of block j
+        const uint32_t kb = k_ring + (j % S::kKSlots) * S::kKTile;
 #pragma unroll
         for (int part = 0; part < S::kParts; ++part) {
-            const uint32_t qa = q_addr + (i * S::kParts + part) * kTileBytes;
+            const uint32_t qa = q_addr + (i * S::kParts + part) * S::kQPart;
+            if (S::kCodeK) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const uint32_t step = (k >> 2) * (kTileBytes / 2) + (k & 3) * 32;
-                mma_ss(tmem + i * kKeys, smem_desc(qa + step, 16, 1024), smem_desc(kb + step, 16, 1024), qk_desc,
-                       part > 0 || k > 0);
+                for (int k = 0; k < 4; ++k) {
+                    mma_ss_e4m3(tmem + i * kKeys, smem_desc(qa + k * 32, 16, 1024), smem_desc(kb + k * 32, 16, 1024),
+                                qk_desc, part > 0 || k > 0);
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const uint32_t step = (k >> 2) * (kTileBytes / 2) + (k & 3) * 32;
+                    mma_ss(tmem + i * kKeys, smem_desc(qa + step, 16, 1024), smem_desc(kb + step, 16, 1024), qk_desc,
+                           part > 0 || k > 0);
+                }
             }
         }
         tc_commit(smem_u32(&ctl->s_full[i]));
     };
-    auto weigh = [&](int i, int seq, bool accumulate) {  // O_i += P_i V
-        const uint32_t vb = ring_addr + (seq % S::kRing) * kTileBytes;
+    auto weigh = [&](int i, int j) {  // O_i += P_i V of block j
+        const uint32_t vb = v_ring + (j % S::kVSlots) * kTileBytes;
 #pragma unroll
-        for (int part = 0; part < S::kParts; ++part) {
+        for (int part = 0; part < (S::kSplit ? 2 : 1); ++part) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 const uint32_t p = tmem + i * kKeys + (k >> 1) * 32 + part * 16 + (k & 1) * 8;
                 mma_ts(tmem + 256 + i * kHeadDim, p, smem_desc(vb + k * 2048, kTileBytes / 2, 1024), pv_desc,
-                       accumulate || part > 0 || k > 0);
+                       j > 0 || part > 0 || k > 0);
             }
         }
     };
     const int n_blocks[2] = {nb0, nb1};
-    bool ok = nb > 0 && wait_for(&ctl->q_full, 0, err) && full(0);
+    bool ok = nb > 0 && wait_for(&ctl->q_full, 0, err) && k_ready(0);
     if (ok) {
         for (int i = 0; i < 2; ++i) {
             if (n_blocks[i] > 0) {
                 logits(i, 0);
             }
         }
-        tc_commit(smem_u32(&ctl->kv_empty[0]));
+        tc_commit(smem_u32(&ctl->k_empty[0]));
     }
     for (int j = 0; ok && j < nb; ++j) {
-        const int v_seq = 2 * j + 1;
-        ok = full(v_seq) && (j + 1 >= nb || full(v_seq + 1));
+        ok = v_ready(j);
         for (int i = 0; ok && i < 2; ++i) {
             if (j >= n_blocks[i]) {
                 continue;
@@ -231,17 +318,20 @@ __device__ __forceinline__ void issue_products(Control *ctl, uint8_t *q_smem, ui
                 break;
             }
             tc_fence_after();
-            weigh(i, v_seq, j > 0);
+            weigh(i, j);
             if (j + 1 < n_blocks[i]) {
-                logits(i, v_seq + 1);
+                ok = k_ready(j + 1);
+                if (ok) {
+                    logits(i, j + 1);
+                }
             } else {
                 tc_commit(smem_u32(&ctl->o_full[i]));
             }
         }
         if (ok) {
-            tc_commit(smem_u32(&ctl->kv_empty[v_seq % S::kRing]));
+            tc_commit(smem_u32(&ctl->v_empty[j % S::kVSlots]));
             if (j + 1 < nb) {
-                tc_commit(smem_u32(&ctl->kv_empty[(v_seq + 1) % S::kRing]));
+                tc_commit(smem_u32(&ctl->k_empty[(j + 1) % S::kKSlots]));
             }
         }
     }
@@ -257,18 +347,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     window_kernel(PoolView pool, const WindowTile *__restrict__ tiles, const int32_t *__restrict__ pages, int layer,
                   const T *__restrict__ q, int64_t q_stride, T *__restrict__ out, int64_t out_stride,
                   float *__restrict__ work, float scale_log2, DeviceError *err) {
-    using S = Shape<T>;
+    using S = Shape<T, kE4m3>;
     extern __shared__ __align__(1024) uint8_t smem[];
-    uint8_t *q_smem = smem;
-    uint8_t *ring = smem + S::kQBytes;
-    Control *ctl = reinterpret_cast<Control *>(smem + S::kQBytes + S::kRing * kTileBytes);
+    const uint32_t q_smem = smem_u32(smem);
+    const uint32_t k_ring = q_smem + S::kQBytes;
+    const uint32_t v_ring = k_ring + S::kKSlots * S::kKTile;
+    Control *ctl = reinterpret_cast<Control *>(smem + S::kQBytes + S::kKSlots * S::kKTile + S::kVSlots * kTileBytes);
     const WindowTile t = tiles[blockIdx.x];
     const int h = blockIdx.y;
     const int G = pool.n_head_kv;
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     const int n_tiles = t.tokens > kTileTokens ? 2 : 1;
-    // 128-key blocks of each M tile: up to the last key that its last token sees
+    // blocks of each M tile: up to the last key that its last token sees
     const int key_end0 = t.pos0 + min(t.tokens, kTileTokens) - t.key0;
     const int nb0 = min(t.blocks, max(0, (key_end0 + kKeys - 1) / kKeys));
     const int nb1 = n_tiles == 2 ? t.blocks : 0;
@@ -284,9 +375,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(smem_u32(&ctl->p_full[i]), kTile);
             mbar_init(smem_u32(&ctl->o_full[i]), 1);
         }
-        for (int i = 0; i < S::kRing; ++i) {
-            mbar_init(smem_u32(&ctl->kv_full[i]), kLoaderThreads);
-            mbar_init(smem_u32(&ctl->kv_empty[i]), 1);
+        for (int i = 0; i < S::kKSlots; ++i) {
+            mbar_init(smem_u32(&ctl->k_full[i]), S::kCodeK ? 1 : kConvertThreads + 1);
+            mbar_init(smem_u32(&ctl->k_empty[i]), 1);
+        }
+        for (int i = 0; i < S::kVSlots; ++i) {
+            mbar_init(smem_u32(&ctl->v_full[i]), kConvertThreads);
+            mbar_init(smem_u32(&ctl->v_empty[i]), 1);
         }
         mbar_init(smem_u32(&ctl->drained), 1);
         ctl->odd_v = 0;
@@ -297,14 +392,34 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     const uint32_t tmem = ctl->tmem;
 
+    // The slot's pages from the CTA's first key on.  Past its last one that one is
+    // read again: K there is masked, V zeroed.
+    const int32_t *list = pages + t.page_off + t.key0 / kPageTokens;
+    const int last_page = (t.pos0 + t.tokens - 1 - t.key0) / kPageTokens;
+    const int last_key = t.pos0 + t.tokens - 1 - t.key0;
+    const int64_t page_stride = static_cast<int64_t>(G) * cache_unit_bytes(kE4m3 ? kCacheE4m3 : kCacheF16);
+    const uint8_t *head_base = pool.base + static_cast<int64_t>(layer) * pool.n_pages * page_stride +
+                               h * (kE4m3 ? kCodeUnitBytes : kHeadBlockBytes);
+    int bad = -1;  // index of a page id outside the pool
+    auto page_at = [&](int index) {
+        int page = list[min(index, last_page)];
+        if (page >= pool.n_pages || page < 0) {
+            bad = index;
+            page = 0;
+        }
+        return page;
+    };
+
     if (warp < 8) {
         // ------------------------------------------------------------ softmax
+        take_registers<kSoftmaxRegs>();
         const int i = warp >> 2;                      // M tile
         const int row = (warp & 3) * 32 + lane;       // = 4 token + head
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_col = tmem + lanes + i * kKeys;
         const uint32_t o_col = tmem + lanes + 256 + i * kHeadDim;
-        // q: rows past the last token are zeros
+        // q: sixteen lanes hold a row, 8 dims each; rows past the last token are zeros
+#pragma unroll 4
         for (int it = 0; it < 16; ++it) {
             const int idx = it * kTile + row;
             const int r = idx >> 4;
@@ -314,28 +429,68 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (tok < t.tokens) {
                 load8(q + (static_cast<int64_t>(t.row0) + tok) * q_stride + (kGqa * h + (r & 3)) * kHeadDim + c * 8, x);
             }
-            uint32_t hi[4], lo[4];
+            const uint32_t part0 = q_smem + i * S::kParts * S::kQPart;
+            if (S::kCodeK) {
+                float amax = 0.f;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                hi[k] = half2_bits(x[2 * k], x[2 * k + 1]);
-                const float2 f = half2_floats(hi[k]);
-                lo[k] = half2_bits(__fsub_rn(x[2 * k], f.x), __fsub_rn(x[2 * k + 1], f.y));
-            }
-            const uint32_t at = smem_u32(q_smem) + i * S::kParts * kTileBytes + tile_offset(kTile, r, c);
-            st_shared16(at, hi[0], hi[1], hi[2], hi[3]);
-            if (S::kSplit) {
-                st_shared16(at + kTileBytes, lo[0], lo[1], lo[2], lo[3]);
+                for (int k = 0; k < 8; ++k) {
+                    amax = fmaxf(amax, finite_abs(x[k]));
+                }
+#pragma unroll
+                for (int off = 8; off > 0; off >>= 1) {
+                    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+                }
+                const int e = block_exponent(amax);
+                if (c == 0) {
+                    ctl->q_exp[i][r] = e;
+                }
+                const float inv = pow2(-e);
+                uint32_t hi[2], lo[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const float4 y = make_float4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
+                    hi[k] = to_codes4(y, inv);
+                    const float4 f = codes_to_float4(hi[k]);
+                    lo[k] = to_codes4(make_float4(fmaf(y.x, inv, -f.x), fmaf(y.y, inv, -f.y), fmaf(y.z, inv, -f.z),
+                                                  fmaf(y.w, inv, -f.w)),
+                                      1.f);
+                }
+                const uint32_t at = part0 + r * kHeadDim + (((c >> 1) ^ (r & 7)) << 4) + (c & 1) * 8;
+                st_shared8(at, hi[0], hi[1]);
+                st_shared8(at + S::kQPart, lo[0], lo[1]);
+            } else {
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    hi[k] = half2_bits(x[2 * k], x[2 * k + 1]);
+                    const float2 f = half2_floats(hi[k]);
+                    lo[k] = half2_bits(__fsub_rn(x[2 * k], f.x), __fsub_rn(x[2 * k + 1], f.y));
+                }
+                const uint32_t at = part0 + tile_offset(kTile, r, c);
+                st_shared16(at, hi[0], hi[1], hi[2], hi[3]);
+                if (S::kSplit) {
+                    st_shared16(at + S::kQPart, lo[0], lo[1], lo[2], lo[3]);
+                }
             }
         }
         fence_proxy_async_smem();
         mbar_arrive(smem_u32(&ctl->q_full));
+        float q_scale = 1.f;
+        if (S::kCodeK) {
+            if (i == 0) {  // q_exp of the tile's rows
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+            } else {
+                asm volatile("bar.sync 2, 128;" ::: "memory");
+            }
+            q_scale = pow2(ctl->q_exp[i][row]);
+        }
 
         const int my_tok = i * kTileTokens + (row >> 2);
         const int my_last = t.pos0 + min(my_tok, t.tokens - 1) - t.key0;  // last key this row sees
         const int first_last = t.pos0 + i * kTileTokens - t.key0;         // and the tile's first row
         const int blocks = i == 0 ? nb0 : nb1;
         float m = -INFINITY, l = 0.f;
-        int e_v = kE4m3 ? kExpMin : 0;
+        int e_v = 0;
         bool ok = true;
         for (int j = 0; j < blocks; ++j) {
             if (!__all_sync(0xffffffffu, wait_for(&ctl->s_full[i], j & 1, err))) {
@@ -344,9 +499,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             tc_fence_after();
             float s[kKeys];
-            tmem_load128(s_col, s);
-            const float *ks = ctl->k_scale[j % kScaleSlots];
-            const int *ve = ctl->v_exp[j % kScaleSlots];
+            tmem_load64(s_col, s);
+            tmem_load64(s_col + 64, s + 64);
+            const BlockScale &b = ctl->scale[j % kScaleSlots];
             if (j * kKeys + kKeys - 1 > first_last) {
                 const int lim = my_last - j * kKeys;  // columns 0 .. lim are seen
 #pragma unroll
@@ -357,34 +512,21 @@ __global__ void __launch_bounds__(kThreads, 1)
             float mx = -INFINITY;
 #pragma unroll
             for (int p = 0; p < kBlockPages; ++p) {
-                float a = s[16 * p], b = s[16 * p + 1];
+                float a = s[16 * p], c = s[16 * p + 1];
 #pragma unroll
                 for (int k = 2; k < 16; k += 2) {
                     a = fmaxf(a, s[16 * p + k]);
-                    b = fmaxf(b, s[16 * p + k + 1]);
+                    c = fmaxf(c, s[16 * p + k + 1]);
                 }
-                mx = fmaxf(mx, fmaxf(a, b) * ks[p]);
+                mx = fmaxf(mx, fmaxf(a, c) * b.k_scale[p]);
             }
+            mx *= q_scale;
             // the bound and E move (o has to follow) only when they must
-            int e_new = e_v;
-            bool far = false;
-            if (kE4m3) {
-#pragma unroll
-                for (int p = 0; p < kBlockPages; ++p) {
-                    e_new = max(e_new, ve[p]);
-                }
-#pragma unroll
-                for (int p = 0; p < kBlockPages; ++p) {
-                    far = far || (ve[p] != kNoPage && ve[p] < e_new - kFar);
-                }
-            }
-            const bool move = mx > m + kSlack || e_new > e_v;
-            if (__any_sync(0xffffffffu, move)) {
+            if (__any_sync(0xffffffffu, mx > m + kSlack || b.grow < 1.f)) {
                 const float m_new = fmaxf(m, mx);
                 const float corr = (m_new == -INFINITY ? 1.f : exp2_fast(m - m_new));
-                const float o_corr = corr * pow2(max(e_v - e_new, -126));
+                const float o_corr = corr * b.grow;
                 m = m_new;
-                e_v = e_new;
                 l *= corr;
                 if (j > 0) {
 #pragma unroll 1
@@ -399,7 +541,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             }
-            const float bound = (m == -INFINITY ? 0.f : m) - kShift;
+            e_v = b.e;
+            const bool far = kE4m3 && b.far != 0;
+            const float bound = m == -INFINITY ? 0.f : m;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 uint32_t hi[16], lo[16];
@@ -409,39 +553,34 @@ __global__ void __launch_bounds__(kThreads, 1)
                     // taken out of the page's sum again; where that could underflow
                     // (V pages 2^60 apart), by a product instead
                     const int page = 2 * c + p;
-                    const float scale = ks[page];
-                    const int d = kE4m3 && ve[page] != kNoPage ? ve[page] - e_v : 0;
-                    const float off = (kE4m3 && !far ? static_cast<float>(d) : 0.f) - bound;
-                    float *x = s + 16 * page;
-                    float sum = 0.f, sum2 = 0.f;
+                    const float sc = b.k_scale[page] * q_scale;
+                    const float sh = b.shift[page] - bound;
+                    const float back = b.back[page];
+                    const float2 scale = make_float2(sc, sc), off = make_float2(sh, sh);
+                    float2 *x = reinterpret_cast<float2 *>(s + 16 * page);
+                    float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-                    for (int k = 0; k < 16; k += 2) {
-                        x[k] = exp2_fast(fmaf(x[k], scale, off));
-                        x[k + 1] = exp2_fast(fmaf(x[k + 1], scale, off));
-                        sum += x[k];
-                        sum2 += x[k + 1];
+                    for (int k = 0; k < 8; ++k) {
+                        const float2 e = fma2(x[k], scale, off);
+                        x[k] = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+                        sum = add2(sum, x[k]);
                     }
-                    sum += sum2;
-                    if (kE4m3) {
-                        if (far) {
-                            const float w = pow2(max(d, -126));
+                    if (far) {
+                        const float w = 1.f / back;
 #pragma unroll
-                            for (int k = 0; k < 16; ++k) {
-                                x[k] *= w;
-                            }
-                            l += sum;
-                        } else {
-                            l = fmaf(sum, pow2(-d), l);
+                        for (int k = 0; k < 8; ++k) {
+                            x[k] = make_float2(x[k].x * w, x[k].y * w);
                         }
+                        l += sum.x + sum.y;
                     } else {
-                        l += sum;
+                        l = fmaf(sum.x + sum.y, back, l);
                     }
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
-                        hi[8 * p + k] = half2_bits(x[2 * k], x[2 * k + 1]);
+                        hi[8 * p + k] = half2_bits(x[k].x, x[k].y);
                         if (S::kSplit) {
                             const float2 f = half2_floats(hi[8 * p + k]);
-                            lo[8 * p + k] = half2_bits(x[2 * k] - f.x, x[2 * k + 1] - f.y);
+                            lo[8 * p + k] = half2_bits(x[k].x - f.x, x[k].y - f.y);
                         }
                     }
                 }
@@ -515,169 +654,206 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             tc_fence_before();
         }
-    } else if (warp < kIssuer) {
-        // ------------------------------------------------------------ loaders
-        const int tid = threadIdx.x - kSoftmaxThreads;
-        const int n_pages = (t.pos0 + t.tokens - 1) / kPageTokens + 1;  // of the slot, up to its last key here
-        // A block is filled in steps of 1024 16-byte pieces: K, V (8-bit cache) or the
-        // two halves of K, then of V (F16).  Two steps' pieces are in registers: a
-        // step's loads go out when the step two before it is stored.  A piece: 8 bits,
-        // 16 dims of a row of one of 8 pages; F16, 8 dims of a row of one of 4.
-        // Eight consecutive threads store to eight different bank groups: 8 bits, dims
-        // 0-63 or 64-127 of two neighbouring rows (an even and an odd row's swizzles
-        // interleave); F16, half a row.
-        constexpr int kSteps = kE4m3 ? 2 : 4;
-        constexpr int kAhead = 2;
-        constexpr int kPieces = 1024;
-        constexpr int kEach = (kPieces + kLoaderThreads - 1) / kLoaderThreads;
-        static_assert(kLoaderThreads % 16 == 0, "a thread keeps its place in the row");
-        const int c = kE4m3 ? ((tid >> 3) & 1) * 4 + (tid & 3) : tid & 15;  // piece of the row
-        const int row0 = kE4m3 ? 2 * (tid >> 4) + ((tid >> 2) & 1) : tid >> 4;
-        constexpr int kRowStep = (kE4m3 ? 2 : 1) * kLoaderThreads / 16;
-        const int64_t page_stride = static_cast<int64_t>(G) * cache_unit_bytes(pool.format);
-        const uint8_t *base = pool.base + static_cast<int64_t>(layer) * pool.n_pages * page_stride +
-                              h * (kE4m3 ? kCodeUnitBytes : kHeadBlockBytes);
-        const int64_t v_off = kE4m3 ? kCodeBlockBytes : static_cast<int64_t>(G) * kHeadBlockBytes;
-        const int32_t *list = pages + t.page_off + t.key0 / kPageTokens;
-        const int last_page = n_pages - 1 - t.key0 / kPageTokens;
-        int bad = -1;
-        // Past the slot's pages its last one is read again: K there is masked, V zeroed.
-        auto page_at = [&](int index) {
-            int page = list[min(index, last_page)];
-            if (page >= pool.n_pages || page < 0) {
-                bad = index;
-                page = 0;
-            }
-            return page;
-        };
-        uint4 raw[kAhead][kEach];
-        auto fetch = [&](int j, int step, uint4 (&to)[kEach]) {
-            const uint8_t *from = base + (step * 2 / kSteps == 1 ? v_off : 0);
-            const int first = j * kBlockPages + (kE4m3 ? 0 : (step & 1) * 4);
-            int page[kEach];
+    } else {
+        give_registers<kOtherRegs>();
+        if (warp < kScaleWarp) {
+            // -------------------------------------------------------- converters
+            const int tid = threadIdx.x - kSoftmaxThreads;
+            // A half tile is 1024 (F16: a quarter, 512 x 2) 16-byte pieces: 8 bits, 16 dims of a
+            // row; F16, 8 dims.  Steps of 1024 pieces, K (where it is converted) then V of
+            // each block; the pieces of kAhead steps are in registers: a step's loads go
+            // out when the step kAhead before it is stored.
+            // Eight consecutive threads store to eight different bank groups: 8 bits, dims
+            // 0-63 or 64-127 of two neighbouring rows (an even and an odd row's swizzles
+            // interleave); F16, half a row.
+            constexpr int kTileSteps = kE4m3 ? 1 : 2;
+            constexpr int kSteps = (S::kCodeK ? 1 : 2) * kTileSteps;
+            constexpr int kAhead = 2;
+            constexpr int kPieces = 1024;
+            constexpr int kEach = (kPieces + kConvertThreads - 1) / kConvertThreads;
+            static_assert(kConvertThreads % 16 == 0, "a thread keeps its place in the row");
+            static_assert(kSteps <= kAhead || kSteps % kAhead == 0, "steps keep their registers");
+            const int c = kE4m3 ? ((tid >> 3) & 1) * 4 + (tid & 3) : tid & 15;  // piece of the row
+            const int row0 = kE4m3 ? 2 * (tid >> 4) + ((tid >> 2) & 1) : tid >> 4;
+            constexpr int kRowStep = (kE4m3 ? 2 : 1) * kConvertThreads / 16;
+            const int64_t v_off = kE4m3 ? kCodeBlockBytes : static_cast<int64_t>(G) * kHeadBlockBytes;
+            auto step_is_v = [](int step) { return S::kCodeK || step >= kTileSteps; };
+            uint4 raw[kAhead][kEach];
+            auto fetch = [&](int j, int step, uint4 (&to)[kEach]) {
+                const uint8_t *from = head_base + (step_is_v(step) ? v_off : 0);
+                const int first = j * kBlockPages + (kE4m3 ? 0 : (step & 1) * 4);
+                int page[kEach];
 #pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                page[i] = page_at(first + ((row0 + i * kRowStep) >> 4));
-            }
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                const int row = (row0 + i * kRowStep) & 15;
-                to[i] = *reinterpret_cast<const uint4 *>(from + page[i] * page_stride +
-                                                         row * (kE4m3 ? kHeadDim : kRowBytes) +
-                                                         ((c ^ (row & 7)) << 4));
-            }
-        };
-        const int last_key = t.pos0 + t.tokens - 1 - t.key0;
-        auto put = [&](int j, int step, const uint4 (&from)[kEach], uint32_t buf) {
-            const bool is_v = step * 2 / kSteps == 1;
-            const bool tail = is_v && j * kKeys + kKeys - 1 > last_key;
-            bool odd = false;
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                const int row = (kE4m3 ? 0 : 64 * (step & 1)) + row0 + i * kRowStep;
-                if (i == kEach - 1 && tid + i * kLoaderThreads >= kPieces) {
-                    break;
+                for (int i = 0; i < kEach; ++i) {
+                    page[i] = page_at(first + ((row0 + i * kRowStep) >> 4));
                 }
-                uint32_t w[4] = {from[i].x, from[i].y, from[i].z, from[i].w};
-                // rows past the last key hold whatever the page had before
-                if (tail && j * kKeys + row > last_key) {
-                    w[0] = w[1] = w[2] = w[3] = 0;
-                }
-                uint32_t x[kE4m3 ? 8 : 4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    if (kE4m3) {
-                        x[2 * k] = codes_to_half2(w[k]);
-                        x[2 * k + 1] = codes_to_half2_hi(w[k]);
-                    } else {
-                        x[k] = w[k];
+                for (int i = 0; i < kEach; ++i) {
+                    const int row = (row0 + i * kRowStep) & 15;
+                    to[i] = *reinterpret_cast<const uint4 *>(from + page[i] * page_stride +
+                                                             row * (kE4m3 ? kHeadDim : kRowBytes) +
+                                                             ((c ^ (row & 7)) << 4));
+                }
+            };
+            auto put = [&](int j, int step, const uint4 (&from)[kEach], uint32_t buf) {
+                const bool is_v = step_is_v(step);
+                const bool tail = is_v && j * kKeys + kKeys - 1 > last_key;
+                bool odd = false;
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) {
+                    const int row = (kE4m3 ? 0 : 64 * (step & 1)) + row0 + i * kRowStep;
+                    if (i == kEach - 1 && tid + i * kConvertThreads >= kPieces) {
+                        break;
                     }
-                }
-                if (is_v) {
-                    // a sum that is not finite: look at each (an F16 sum may overflow)
-                    uint32_t sum = x[0];
-#pragma unroll
-                    for (int k = 1; k < (kE4m3 ? 8 : 4); ++k) {
-                        sum = half2_sum(sum, x[k]);
+                    uint32_t w[4] = {from[i].x, from[i].y, from[i].z, from[i].w};
+                    // rows past the last key hold whatever the page had before
+                    if (tail && j * kKeys + row > last_key) {
+                        w[0] = w[1] = w[2] = w[3] = 0;
                     }
-                    if ((((sum & 0x7c007c00u) + 0x04000400u) & 0x80008000u) != 0) {
+                    uint32_t x[kE4m3 ? 8 : 4];
 #pragma unroll
-                        for (int k = 0; k < (kE4m3 ? 8 : 4); ++k) {
-                            const uint32_t out = ((x[k] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
-                            odd = odd || out != 0;
-                            x[k] &= ~((out >> 15) * 0xffffu);
+                    for (int k = 0; k < 4; ++k) {
+                        if (kE4m3) {
+                            x[2 * k] = codes_to_half2(w[k]);
+                            x[2 * k + 1] = codes_to_half2_hi(w[k]);
+                        } else {
+                            x[k] = w[k];
                         }
                     }
-                }
-                if (kE4m3) {
-                    st_shared16(buf + tile_offset(kKeys, row, 2 * c), x[0], x[1], x[2], x[3]);
-                    st_shared16(buf + tile_offset(kKeys, row, 2 * c + 1), x[kE4m3 ? 4 : 0], x[kE4m3 ? 5 : 0],
-                                x[kE4m3 ? 6 : 0], x[kE4m3 ? 7 : 0]);
-                } else {
-                    st_shared16(buf + tile_offset(kKeys, row, c), x[0], x[1], x[2], x[3]);
-                }
-            }
-            if (odd) {
-                *reinterpret_cast<volatile int *>(&ctl->odd_v) = 1;
-            }
-        };
-        // The exponents of a block's K and V, with its K tile: thread p takes page p's.
-        int2 exps = make_int2(0, kNoPage);
-        auto fetch_exponents = [&](int j) {
-            if (kE4m3 && tid < kBlockPages) {
-                const int index = j * kBlockPages + tid;
-                exps = *reinterpret_cast<const int2 *>(base + page_at(index) * page_stride + 2 * kCodeBlockBytes);
-                if (index > last_page) {
-                    exps.y = kNoPage;
-                }
-            }
-        };
-        fetch(0, 0, raw[0]);
-        fetch(0, 1, raw[1]);
-        fetch_exponents(0);
-        bool ok = true;
-        for (int j = 0; ok && j < nb; ++j) {
+                    if (is_v) {
+                        // a sum that is not finite: look at each (an F16 sum may overflow)
+                        uint32_t sum = x[0];
 #pragma unroll
-            for (int step = 0; step < kSteps; ++step) {
-                const int seq = 2 * j + step * 2 / kSteps;  // the operand tile
-                const int slot = seq % S::kRing;
-                const bool first_step = step % (kSteps / 2) == 0;
-                const bool last_step = (step + 1) % (kSteps / 2) == 0;
-                if (first_step && seq >= S::kRing) {
-                    ok = ok && wait_for(&ctl->kv_empty[slot], (seq / S::kRing - 1) & 1, err);
+                        for (int k = 1; k < (kE4m3 ? 8 : 4); ++k) {
+                            sum = half2_sum(sum, x[k]);
+                        }
+                        if ((((sum & 0x7c007c00u) + 0x04000400u) & 0x80008000u) != 0) {
+#pragma unroll
+                            for (int k = 0; k < (kE4m3 ? 8 : 4); ++k) {
+                                const uint32_t out = ((x[k] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+                                odd = odd || out != 0;
+                                x[k] &= ~((out >> 15) * 0xffffu);
+                            }
+                        }
+                    }
+                    if (kE4m3) {
+                        st_shared16(buf + tile_offset(kKeys, row, 2 * c), x[0], x[1], x[2], x[3]);
+                        st_shared16(buf + tile_offset(kKeys, row, 2 * c + 1), x[kE4m3 ? 4 : 0], x[kE4m3 ? 5 : 0],
+                                    x[kE4m3 ? 6 : 0], x[kE4m3 ? 7 : 0]);
+                    } else {
+                        st_shared16(buf + tile_offset(kKeys, row, c), x[0], x[1], x[2], x[3]);
+                    }
                 }
-                if (!ok) {
-                    break;
+                if (odd) {
+                    *reinterpret_cast<volatile int *>(&ctl->odd_v) = 1;
                 }
-                if (step == 0 && tid < kBlockPages) {
-                    ctl->k_scale[j % kScaleSlots][tid] = scale_log2 * pow2(exps.x);
-                    ctl->v_exp[j % kScaleSlots][tid] = exps.y;
+            };
+            // steps in one line, step s of block j being j * kSteps + s
+            const int all = nb * kSteps;
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a) {
+                if (a < all) {
+                    fetch(a / kSteps, a % kSteps, raw[a]);
                 }
-                put(j, step, raw[step % kAhead], smem_u32(ring) + slot * kTileBytes);
-                if (last_step) {
-                    fence_proxy_async_smem();
-                    mbar_arrive(smem_u32(&ctl->kv_full[slot]));
-                }
-                if (step + kAhead < kSteps) {
-                    fetch(j, step + kAhead, raw[step % kAhead]);
-                } else if (j + 1 < nb) {
-                    fetch(j + 1, step + kAhead - kSteps, raw[step % kAhead]);
-                    if (step + kAhead == kSteps) {
-                        fetch_exponents(j + 1);
+            }
+            bool ok = true;
+            for (int first = 0; ok && first < all; first += kAhead) {
+#pragma unroll
+                for (int a = 0; a < kAhead; ++a) {
+                    const int at = first + a;
+                    if (at >= all) {
+                        break;
+                    }
+                    const int j = at / kSteps;
+                    const int step = at % kSteps;
+                    const bool is_v = step_is_v(step);
+                    const int slot = is_v ? j % S::kVSlots : j % S::kKSlots;
+                    if (step % kTileSteps == 0) {
+                        const int n = is_v ? S::kVSlots : S::kKSlots;
+                        if (j >= n && !wait_for(is_v ? &ctl->v_empty[slot] : &ctl->k_empty[slot], (j / n - 1) & 1, err)) {
+                            ok = false;
+                            break;
+                        }
+                    }
+                    put(j, step, raw[a], is_v ? v_ring + slot * kTileBytes : k_ring + slot * S::kKTile);
+                    if (step % kTileSteps == kTileSteps - 1) {
+                        fence_proxy_async_smem();
+                        mbar_arrive(smem_u32(is_v ? &ctl->v_full[slot] : &ctl->k_full[slot]));
+                    }
+                    if (at + kAhead < all) {
+                        fetch((at + kAhead) / kSteps, (at + kAhead) % kSteps, raw[a]);
                     }
                 }
             }
-        }
-        if (bad >= 0) {
-            record(err, kErrBadIndex, list[min(bad, last_page)], bad);
-        }
-    } else {
-        // ----------------------------------------------------------- products
-        if (lane == 0) {
-            issue_products<T>(ctl, q_smem, ring, tmem, nb0, nb1, err);
+        } else if (warp == kScaleWarp) {
+            // ------------------------------------------- exponents, and K's codes
+            int e = INT32_MIN;  // E
+            bool ok = true;
+            for (int j = 0; ok && j < nb; ++j) {
+                const int slot = j % S::kKSlots;
+                const int index = j * kBlockPages + (lane & 7);
+                const int64_t page = page_at(index);
+                const uint8_t *unit = head_base + page * page_stride;
+                int2 exps = make_int2(0, 0);
+                if (kE4m3) {
+                    exps = *reinterpret_cast<const int2 *>(unit + 2 * kCodeBlockBytes);
+                }
+                const bool there = index <= last_page;
+                int top = there ? exps.y : INT32_MIN;
+#pragma unroll
+                for (int off = 4; off > 0; off >>= 1) {
+                    top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
+                }
+                const int e_new = max(e, top);
+                const int d = there ? exps.y - e_new : 0;
+                const bool far = __any_sync(0xffffffffu, d < -kFar);
+                if (j >= S::kKSlots) {
+                    ok = __all_sync(0xffffffffu, wait_for(&ctl->k_empty[slot], (j / S::kKSlots - 1) & 1, err));
+                    if (!ok) {
+                        break;
+                    }
+                }
+                BlockScale &b = ctl->scale[j % kScaleSlots];
+                if (lane < kBlockPages) {
+                    b.k_scale[lane] = scale_log2 * pow2(exps.x);
+                    b.shift[lane] = static_cast<float>(kShift + (far ? 0 : d));
+                    b.back[lane] = pow2(min(-d, 126));
+                }
+                if (lane == 0) {
+                    b.grow = j == 0 ? 1.f : pow2(max(e - e_new, -126));
+                    b.e = e_new;
+                    b.far = far ? 1 : 0;
+                }
+                e = e_new;
+                __syncwarp();
+                const uint32_t bar = smem_u32(&ctl->k_full[slot]);
+                if (S::kCodeK) {
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(bar, kCodeTileBytes);
+                    }
+                    __syncwarp();
+                    if (lane < kBlockPages) {
+                        bulk_load(k_ring + slot * S::kKTile + lane * kCodeBlockBytes, unit, kCodeBlockBytes, bar,
+                                  keep_policy());
+                    }
+                } else if (lane == 0) {
+                    mbar_arrive(bar);
+                }
+            }
+            if (S::kCodeK) {
+                // copies that no product waited for end before the CTA does
+                for (int j = max(0, nb - S::kKSlots); j < nb; ++j) {
+                    mbar_wait_bounded(smem_u32(&ctl->k_full[j % S::kKSlots]), (j / S::kKSlots) & 1);
+                }
+            }
+        } else if (lane == 0) {
+            // ---------------------------------------------------------- products
+            issue_products<S>(ctl, q_smem, k_ring, v_ring, tmem, nb0, nb1, err);
         }
     }
-
+    if (bad >= 0) {
+        record(err, kErrBadIndex, list[min(bad, last_page)], bad);
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -732,14 +908,14 @@ void launch_window_t(const PoolView &pool, const WindowArgs &a, DeviceError *err
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64 || !configured[dev]) {
-        cudaFuncSetAttribute(window_kernel<T, kE4m3>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<T>::kSmem);
+        cudaFuncSetAttribute(window_kernel<T, kE4m3>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<T, kE4m3>::kSmem);
         if (dev >= 0 && dev < 64) {
             configured[dev] = true;
         }
     }
     const unsigned G = static_cast<unsigned>(pool.n_head_kv);
     T *out = static_cast<T *>(a.out);
-    window_kernel<T, kE4m3><<<dim3(static_cast<unsigned>(a.n_tiles), G), kThreads, Shape<T>::kSmem, stream>>>(
+    window_kernel<T, kE4m3><<<dim3(static_cast<unsigned>(a.n_tiles), G), kThreads, Shape<T, kE4m3>::kSmem, stream>>>(
         pool, a.tiles, a.pages, a.layer, static_cast<const T *>(a.q), a.q_stride, out, a.out_stride, a.work,
         a.scale_log2, err);
     if (a.n_merges > 0) {

@@ -18,14 +18,19 @@ HALF = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
 DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 
 
-def tolerance(name, big, n_rows, vmax, want):
-    """F32: attention_tolerance().  F16 and BF16: q enters exactly; the weights are
-    rounded to F16 (2^-11 relative, on top of the F32 path's) and the output once to its type;
-    F16 outputs below 2^-14 have steps of 2^-24."""
+def tolerance(name, big, n_rows, vmax, want, q, k):
+    """F32: attention_tolerance().  F16 and BF16: the weights are rounded to F16 (2^-11
+    relative, on top of the F32 path's) and the output once to its type; F16 outputs
+    below 2^-14 have steps of 2^-24.  F16 q enters exactly.  BF16 q (8 bits) enters as two
+    E4M3 numbers of 4 bits, scaled so that the row's largest value is at least 224: exact
+    down to 2^-2 (the second part is a multiple of 2^-9), off by at most 2^-10 below that, which
+    is 2^-10 / 224 of the row's largest value for each dim, and moves every weight by twice that."""
     t = attention_tolerance(big, n_rows, vmax)
     if name == "f32":
         return t
     t += vmax * 2.0 ** -11
+    if name == "bf16":
+        t += 2 * vmax * np.abs(q).max() * 2.0 ** -10 / 224 * np.abs(k).sum(-1).max() / np.sqrt(128.0)
     return t + HALF[name] * (np.abs(want) + t) + (2.0 ** -25 if name == "f16" else 0.0)
 
 
@@ -52,7 +57,7 @@ def check(eng, hkv, slots, new, q, out, name, layer=0):
         torch.cuda.synchronize()
         k, v = k.cpu().numpy(), v.cpu().numpy()
         want, big = attention(q64[at:at + n], k, v, p)
-        tol = tolerance(name, big, p + n, np.abs(v).max(), want)
+        tol = tolerance(name, big, p + n, np.abs(v).max(), want, q64[at:at + n], k)
         over = float((np.abs(got[at:at + n] - want) - tol).max())
         assert over <= 0, (s, p, n, over, float(np.abs(got[at:at + n] - want).max()))
         at += n
@@ -135,7 +140,7 @@ def test_window_exponents_far_apart(hkv_lib, name):
         got = out.double().cpu().numpy().reshape(200, 4, D)
         for i in range(0, 200, 3):
             want, big = attention(q64[i:i + 1], kk[:i + 1], vv[:i + 1], i)
-            tol = tolerance(name, big, i + 1, np.abs(vv[:i + 1]).max(), want)
+            tol = tolerance(name, big, i + 1, np.abs(vv[:i + 1]).max(), want, q64[i], kk[:i + 1])
             assert float((np.abs(got[i] - want[0]) - tol).max()) <= 0, i
     eng.close()
 
