@@ -12,12 +12,13 @@
 // rows, and a run of 128-key blocks.  Both products run on the tensor cores
 // (tcgen05, F32 accumulators in TMEM); codes are exact in F16, so K and V enter
 // without error.
-//   warps 0-3, 4-7  softmax of M tile 0 / 1, a thread a row: S from TMEM, the
-//                   weights back into S's columns as the next product's A operand
-//   warps 8-13      converters: 16-byte pieces of the pages to F16 operand tiles
-//   warp 14         exponents of each block, and K as it is where q is in E4M3 parts
-//   warp 15         one thread issues every product; while one tile's softmax
-//                   runs, the other tile's products do
+//   warps 0-7, 8-15 softmax of M tile 0 / 1, two threads a row (64 of a block's keys
+//                   each): S from TMEM, the weights back into S's columns as the next
+//                   product's A operand
+//   warps 16-20     converters: 16-byte pieces of the pages to F16 operand tiles
+//   warp 21         exponents of each block, and K as it is where q is in E4M3 parts
+//   warps 22, 23    one thread each issues the products of an M tile; while one tile's
+//                   softmax runs, the other tile's products do
 //
 // BF16 tensors on an 8-bit cache: q has 8 significant bits, two E4M3 numbers of 4
 // (with a power of two per row), so q K^T is two E4M3 products at twice the F16 rate
@@ -60,39 +61,20 @@ constexpr int kTileTokens = kTile / kGqa;
 constexpr int kTileBytes = 128 * 128 * 2;   // an F16 operand tile (q rows, keys)
 constexpr int kCodeTileBytes = 128 * 128;   // an E4M3 one
 static_assert(kKeys == 128 && kTile == 128, "operand tiles are 128 x 128");
-constexpr int kSoftmaxThreads = 256;
-constexpr int kConvertThreads = 192;
-constexpr int kScaleWarp = 14;
-constexpr int kIssuer = 15;
-constexpr int kThreads = 512;
-// Registers of a thread: the launch gives 128 to each, the softmax, which holds a
-// row of 128 logits, takes what the other two warpgroups leave.  (184 / 72: the
-// converters spill what they prefetch and bound the kernel, 1.09 ms at 8,100 tokens;
-// 176 / 80 0.87; 168 / 88 0.81; 160 / 96 0.80.)
-constexpr int kSoftmaxRegs = 160;
-constexpr int kOtherRegs = 96;
-static_assert(2 * kSoftmaxRegs + 2 * kOtherRegs == 4 * 128, "the shares add up to the launch's registers");
-// Blocks whose scales are kept.  Those of block j are written once the products of
-// q and K of block j - kKSlots (at most 4) are done, when a softmax may still be at
-// that block.
-constexpr int kScaleSlots = 8;
+constexpr int kTileThreads = 256;       // softmax threads of an M tile
+constexpr int kSoftmaxThreads = 2 * kTileThreads;
+constexpr int kConvertThreads = 160;
+constexpr int kScaleWarp = 21;
+constexpr int kIssuer = 22;
+constexpr int kThreads = 768;
+// Registers of a thread: the launch gives 80 to each, the softmax takes what the
+// other two of the six warpgroups leave.
+constexpr int kSoftmaxRegs = 88;
+constexpr int kOtherRegs = 64;
+static_assert(4 * kSoftmaxRegs + 2 * kOtherRegs == 6 * 80, "the shares add up to the launch's registers");
 constexpr float kSlack = 8.f;
 constexpr int kShift = 7;               // weights enter 2^7 larger: at most 2^15 in F16
 constexpr int kFar = 60;                // V exponents this far below E take the slow form
-
-template <typename T, bool kE4m3>
-struct Shape {
-    static constexpr bool kSplit = sizeof(T) == 4;
-    static constexpr bool kCodeK = kE4m3 && std::is_same<T, __nv_bfloat16>::value;
-    static constexpr int kParts = kSplit || kCodeK ? 2 : 1;  // of q
-    static constexpr int kQPart = kCodeK ? kCodeTileBytes : kTileBytes;
-    static constexpr int kKTile = kCodeK ? kCodeTileBytes : kTileBytes;
-    static constexpr int kKSlots = kSplit ? 1 : kCodeK ? 4 : 2;
-    static constexpr int kVSlots = kSplit ? 2 : 3;
-    static constexpr int kQBytes = 2 * kParts * kQPart;
-    static constexpr int kSmem = kQBytes + kKSlots * kKTile + kVSlots * kTileBytes + 3072;
-    static_assert(kSmem <= 227 * 1024, "operands exceed shared memory");
-};
 
 // What the softmax needs of a block's pages.
 struct BlockScale {
@@ -107,14 +89,35 @@ struct BlockScale {
 
 struct Control {
     uint64_t q_full, s_full[2], p_full[2], o_full[2];
-    uint64_t k_full[4], k_empty[4], v_full[3], v_empty[3];
-    uint64_t drained;                           // after a wait that ran out: no product in flight
+    uint64_t k_full[3], k_empty[3], v_full[3], v_empty[3];
+    uint64_t turn[2];           // of the issuers: a phase a block
+    uint64_t drained[2];        // after a wait that ran out: no product in flight
     uint32_t tmem;
-    int odd_v;                                  // a V value that is not finite was met
-    BlockScale scale[kScaleSlots];
-    int q_exp[2][kTile];                        // of a row of q in E4M3 parts
+    int odd_v;                  // a V value that is not finite was met
+    union {
+        int q_exp[2][kTile];          // of a row of q in E4M3 parts
+        float half[2][2][kTile];      // of a row's logits the largest, by each of its threads; l at the end
+    };
 };
-static_assert(sizeof(Control) <= 3072, "the control block has 3 KiB");
+static_assert(sizeof(Control) % 16 == 0, "the scales follow it");
+
+template <typename T, bool kE4m3>
+struct Shape {
+    static constexpr bool kSplit = sizeof(T) == 4;
+    static constexpr bool kCodeK = kE4m3 && std::is_same<T, __nv_bfloat16>::value;
+    static constexpr int kParts = kSplit || kCodeK ? 2 : 1;  // of q
+    static constexpr int kQPart = kCodeK ? kCodeTileBytes : kTileBytes;
+    static constexpr int kKTile = kCodeK ? kCodeTileBytes : kTileBytes;
+    static constexpr int kKSlots = kSplit ? 1 : kCodeK ? 3 : 2;
+    static constexpr int kVSlots = kSplit ? 2 : 3;
+    // Blocks whose scales are kept.  Those of block j are written once the products of
+    // q and K of block j - kKSlots are done, when a softmax may still be at that block.
+    static constexpr int kScaleSlots = 2 * kKSlots;
+    static constexpr int kQBytes = 2 * kParts * kQPart;
+    static constexpr int kControl = kQBytes + kKSlots * kKTile + kVSlots * kTileBytes;  // its offset
+    static constexpr int kSmem = kControl + sizeof(Control) + kScaleSlots * sizeof(BlockScale);
+    static_assert(kSmem <= 227 * 1024, "operands exceed shared memory");
+};
 
 __device__ __forceinline__ void record(DeviceError *err, int code, int a, int b) {
     if (atomicCAS(&err->code, 0, code) == 0) {
@@ -218,6 +221,16 @@ __device__ __forceinline__ bool wait_for(uint64_t *bar, uint32_t parity, DeviceE
     return false;
 }
 
+// Barrier of the two warps that share rows (w and w + 4): ids 1 .. 8.
+__device__ __forceinline__ void pair_barrier(int warp) {
+    asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp >> 3) * 4 + (warp & 3)) : "memory");
+}
+
+// Barrier of an M tile's softmax threads.
+__device__ __forceinline__ void tile_barrier(int i) {
+    asm volatile("bar.sync %0, 256;" ::"r"(9 + i) : "memory");
+}
+
 // One value of the cache, as it stands in the pool.
 template <bool kE4m3>
 __device__ float cached_value(const PoolView &pool, int64_t page, int layer, int kv, int h, int r, int d) {
@@ -249,12 +262,12 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return *reinterpret_cast<const float2 *>(&d);
 }
 
-// The issuing thread: S_i = q_i K^T and O_i += P_i V, block by block, the two M tiles
-// in turn.  nb0, nb1: blocks of each tile.
+// The issuing thread of M tile i: S_i = q_i K^T and O_i += P_i V, block by block.  nb:
+// blocks of the CTA, blocks: of the tile.  Each tile has its own issuer, since a wait or
+// commit costs one about 130 cycles during which only the other's products are queued.
 template <class S>
 __device__ __forceinline__ void issue_products(Control *ctl, uint32_t q_addr, uint32_t k_ring, uint32_t v_ring,
-                                               uint32_t tmem, int nb0, int nb1, DeviceError *err) {
-    const int nb = max(nb0, nb1);
+                                               uint32_t tmem, int i, int nb, int blocks, DeviceError *err) {
     constexpr uint32_t qk_desc = mma_idesc(kTile, kKeys, false);
     constexpr uint32_t pv_desc = mma_idesc(kTile, kHeadDim, true);
     auto k_ready = [&](int j) {
@@ -263,7 +276,7 @@ __device__ __forceinline__ void issue_products(Control *ctl, uint32_t q_addr, ui
     auto v_ready = [&](int j) {
         return wait_for(&ctl->v_full[j % S::kVSlots], (j / S::kVSlots) & 1, err);
     };
-    auto logits = [&](int i, int j) {  // S_i of block j
+    auto logits = [&](int j) {  // S_i of block j
         const uint32_t kb = k_ring + (j % S::kKSlots) * S::kKTile;
 #pragma unroll
         for (int part = 0; part < S::kParts; ++part) {
@@ -285,7 +298,7 @@ __device__ __forceinline__ void issue_products(Control *ctl, uint32_t q_addr, ui
         }
         tc_commit(smem_u32(&ctl->s_full[i]));
     };
-    auto weigh = [&](int i, int j) {  // O_i += P_i V of block j
+    auto weigh = [&](int j) {  // O_i += P_i V of block j
         const uint32_t vb = v_ring + (j % S::kVSlots) * kTileBytes;
 #pragma unroll
         for (int part = 0; part < (S::kSplit ? 2 : 1); ++part) {
@@ -297,48 +310,62 @@ __device__ __forceinline__ void issue_products(Control *ctl, uint32_t q_addr, ui
             }
         }
     };
-    const int n_blocks[2] = {nb0, nb1};
-    bool ok = nb > 0 && wait_for(&ctl->q_full, 0, err) && k_ready(0);
-    if (ok) {
-        for (int i = 0; i < 2; ++i) {
-            if (n_blocks[i] > 0) {
-                logits(i, 0);
-            }
-        }
+    // The issuers take turns, so that a tile's products stand in line as a whole: mixed,
+    // both tiles would get theirs late, and at the same time, and their softmaxes would
+    // then compete for the exponentials.
+    auto turn = [&](int round) { return wait_for(&ctl->turn[i], round & 1, err); };
+    auto pass = [&]() { mbar_arrive(smem_u32(&ctl->turn[i ^ 1])); };
+    bool ok = (blocks == 0 || (wait_for(&ctl->q_full, 0, err) && k_ready(0))) && turn(0);
+    if (ok && blocks > 0) {
+        logits(0);
         tc_commit(smem_u32(&ctl->k_empty[0]));
     }
+    pass();
     for (int j = 0; ok && j < nb; ++j) {
-        ok = v_ready(j);
-        for (int i = 0; ok && i < 2; ++i) {
-            if (j >= n_blocks[i]) {
-                continue;
+        if (j >= blocks) {
+            // a block that only the other tile takes: its buffers are let go at once (the
+            // other issuer may wait for them in its turn)
+            ok = k_ready(j);
+            if (ok) {
+                mbar_arrive(smem_u32(&ctl->k_empty[j % S::kKSlots]));
+                ok = v_ready(j);
             }
-            ok = wait_for(&ctl->p_full[i], j & 1, err);
+            if (ok) {
+                mbar_arrive(smem_u32(&ctl->v_empty[j % S::kVSlots]));
+                ok = turn(j + 1);
+            }
+            if (ok) {
+                pass();
+            }
+            continue;
+        }
+        const bool more = j + 1 < blocks;
+        ok = v_ready(j) && (S::kKSlots == 1 || !more || k_ready(j + 1)) && wait_for(&ctl->p_full[i], j & 1, err) &&
+             turn(j + 1);
+        if (!ok) {
+            break;
+        }
+        tc_fence_after();
+        weigh(j);
+        if (more) {
+            ok = S::kKSlots > 1 || k_ready(j + 1);
             if (!ok) {
                 break;
             }
-            tc_fence_after();
-            weigh(i, j);
-            if (j + 1 < n_blocks[i]) {
-                ok = k_ready(j + 1);
-                if (ok) {
-                    logits(i, j + 1);
-                }
-            } else {
-                tc_commit(smem_u32(&ctl->o_full[i]));
-            }
+            logits(j + 1);
+        } else {
+            tc_commit(smem_u32(&ctl->o_full[i]));
         }
-        if (ok) {
-            tc_commit(smem_u32(&ctl->v_empty[j % S::kVSlots]));
-            if (j + 1 < nb) {
-                tc_commit(smem_u32(&ctl->k_empty[(j + 1) % S::kKSlots]));
-            }
+        pass();
+        if (more) {
+            tc_commit(smem_u32(&ctl->k_empty[(j + 1) % S::kKSlots]));
         }
+        tc_commit(smem_u32(&ctl->v_empty[j % S::kVSlots]));
     }
-    if (!ok && nb > 0) {
+    if (!ok) {
         // products in flight end before the memory they use is given up
-        tc_commit(smem_u32(&ctl->drained));
-        mbar_wait_bounded(smem_u32(&ctl->drained), 0);
+        tc_commit(smem_u32(&ctl->drained[i]));
+        mbar_wait_bounded(smem_u32(&ctl->drained[i]), 0);
     }
 }
 
@@ -352,7 +379,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t q_smem = smem_u32(smem);
     const uint32_t k_ring = q_smem + S::kQBytes;
     const uint32_t v_ring = k_ring + S::kKSlots * S::kKTile;
-    Control *ctl = reinterpret_cast<Control *>(smem + S::kQBytes + S::kKSlots * S::kKTile + S::kVSlots * kTileBytes);
+    Control *ctl = reinterpret_cast<Control *>(smem + S::kControl);
+    BlockScale *scales = reinterpret_cast<BlockScale *>(ctl + 1);
     const WindowTile t = tiles[blockIdx.x];
     const int h = blockIdx.y;
     const int G = pool.n_head_kv;
@@ -372,18 +400,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(smem_u32(&ctl->q_full), kSoftmaxThreads);
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&ctl->s_full[i]), 1);
-            mbar_init(smem_u32(&ctl->p_full[i]), kTile);
+            mbar_init(smem_u32(&ctl->p_full[i]), kTileThreads);
             mbar_init(smem_u32(&ctl->o_full[i]), 1);
+            mbar_init(smem_u32(&ctl->drained[i]), 1);
         }
         for (int i = 0; i < S::kKSlots; ++i) {
             mbar_init(smem_u32(&ctl->k_full[i]), S::kCodeK ? 1 : kConvertThreads + 1);
-            mbar_init(smem_u32(&ctl->k_empty[i]), 1);
+            mbar_init(smem_u32(&ctl->k_empty[i]), 2);
         }
         for (int i = 0; i < S::kVSlots; ++i) {
             mbar_init(smem_u32(&ctl->v_full[i]), kConvertThreads);
-            mbar_init(smem_u32(&ctl->v_empty[i]), 1);
+            mbar_init(smem_u32(&ctl->v_empty[i]), 2);
         }
-        mbar_init(smem_u32(&ctl->drained), 1);
+        mbar_init(smem_u32(&ctl->turn[0]), 1);
+        mbar_init(smem_u32(&ctl->turn[1]), 1);
+        mbar_arrive(smem_u32(&ctl->turn[0]));
         ctl->odd_v = 0;
         fence_barrier_init();
     }
@@ -410,18 +441,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         return page;
     };
 
-    if (warp < 8) {
+    if (warp < kSoftmaxThreads / 32) {
         // ------------------------------------------------------------ softmax
         take_registers<kSoftmaxRegs>();
-        const int i = warp >> 2;                      // M tile
+        const int i = warp >> 3;                      // M tile
+        const int half = (warp >> 2) & 1;             // of a block's keys, and of o's dims
         const int row = (warp & 3) * 32 + lane;       // = 4 token + head
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t s_col = tmem + lanes + i * kKeys;
-        const uint32_t o_col = tmem + lanes + 256 + i * kHeadDim;
+        const uint32_t s_col = tmem + lanes + i * kKeys + half * 64;
+        const uint32_t o_col = tmem + lanes + 256 + i * kHeadDim + half * 64;
         // q: sixteen lanes hold a row, 8 dims each; rows past the last token are zeros
-#pragma unroll 4
-        for (int it = 0; it < 16; ++it) {
-            const int idx = it * kTile + row;
+#pragma unroll 2
+        for (int it = 0; it < 8; ++it) {
+            const int idx = it * kTileThreads + half * kTile + row;
             const int r = idx >> 4;
             const int c = idx & 15;
             const int tok = i * kTileTokens + (r >> 2);
@@ -477,12 +509,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive(smem_u32(&ctl->q_full));
         float q_scale = 1.f;
         if (S::kCodeK) {
-            if (i == 0) {  // q_exp of the tile's rows
-                asm volatile("bar.sync 1, 128;" ::: "memory");
-            } else {
-                asm volatile("bar.sync 2, 128;" ::: "memory");
-            }
+            tile_barrier(i);  // q_exp of the tile's rows
             q_scale = pow2(ctl->q_exp[i][row]);
+            tile_barrier(i);  // before `half` takes its place
         }
 
         const int my_tok = i * kTileTokens + (row >> 2);
@@ -498,29 +527,36 @@ __global__ void __launch_bounds__(kThreads, 1)
                 break;
             }
             tc_fence_after();
-            float s[kKeys];
-            tmem_load64(s_col, s);
-            tmem_load64(s_col + 64, s + 64);
-            const BlockScale &b = ctl->scale[j % kScaleSlots];
-            if (j * kKeys + kKeys - 1 > first_last) {
-                const int lim = my_last - j * kKeys;  // columns 0 .. lim are seen
-#pragma unroll
-                for (int k = 0; k < kKeys; ++k) {
-                    s[k] = k <= lim ? s[k] : -INFINITY;
-                }
-            }
+            const BlockScale &b = scales[j % S::kScaleSlots];
+            const bool masked = j * kKeys + 64 * half + 63 > first_last;
+            const int lim = my_last - j * kKeys - 64 * half;  // columns 0 .. lim of this half are seen
             float mx = -INFINITY;
 #pragma unroll
-            for (int p = 0; p < kBlockPages; ++p) {
-                float a = s[16 * p], c = s[16 * p + 1];
+            for (int c = 0; c < 2; ++c) {
+                float s[32];
+                tmem_load32(s_col + 32 * c, s);
+                if (masked) {
 #pragma unroll
-                for (int k = 2; k < 16; k += 2) {
-                    a = fmaxf(a, s[16 * p + k]);
-                    c = fmaxf(c, s[16 * p + k + 1]);
+                    for (int k = 0; k < 32; ++k) {
+                        s[k] = 32 * c + k <= lim ? s[k] : -INFINITY;
+                    }
                 }
-                mx = fmaxf(mx, fmaxf(a, c) * b.k_scale[p]);
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    float a = s[16 * p], d = s[16 * p + 1];
+#pragma unroll
+                    for (int k = 2; k < 16; k += 2) {
+                        a = fmaxf(a, s[16 * p + k]);
+                        d = fmaxf(d, s[16 * p + k + 1]);
+                    }
+                    mx = fmaxf(mx, fmaxf(a, d) * b.k_scale[4 * half + 2 * c + p]);
+                }
             }
             mx *= q_scale;
+            // the row's maximum over both halves
+            ctl->half[i][half][row] = mx;
+            pair_barrier(warp);
+            mx = fmaxf(mx, ctl->half[i][half ^ 1][row]);
             // the bound and E move (o has to follow) only when they must
             if (__any_sync(0xffffffffu, mx > m + kSlack || b.grow < 1.f)) {
                 const float m_new = fmaxf(m, mx);
@@ -530,7 +566,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 l *= corr;
                 if (j > 0) {
 #pragma unroll 1
-                    for (int c = 0; c < kHeadDim; c += 16) {
+                    for (int c = 0; c < 64; c += 16) {
                         float o[16];
                         tmem_load16(o_col + c, o);
 #pragma unroll
@@ -545,19 +581,27 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool far = kE4m3 && b.far != 0;
             const float bound = m == -INFINITY ? 0.f : m;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
+            for (int c = 0; c < 2; ++c) {
+                float s[32];
+                tmem_load32(s_col + 32 * c, s);
+                if (masked) {
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) {
+                        s[k] = 32 * c + k <= lim ? s[k] : -INFINITY;
+                    }
+                }
                 uint32_t hi[16], lo[16];
 #pragma unroll
                 for (int p = 0; p < 2; ++p) {
                     // 2^(eV - E) belongs to the weight and not to l: in the exponent, and
                     // taken out of the page's sum again; where that could underflow
                     // (V pages 2^60 apart), by a product instead
-                    const int page = 2 * c + p;
+                    const int page = 4 * half + 2 * c + p;
                     const float sc = b.k_scale[page] * q_scale;
                     const float sh = b.shift[page] - bound;
                     const float back = b.back[page];
                     const float2 scale = make_float2(sc, sc), off = make_float2(sh, sh);
-                    float2 *x = reinterpret_cast<float2 *>(s + 16 * page);
+                    float2 *x = reinterpret_cast<float2 *>(s + 16 * p);
                     float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
@@ -597,41 +641,42 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (ok && blocks > 0) {
             ok = __all_sync(0xffffffffu, wait_for(&ctl->o_full[i], 0, err));
         }
+        // the row's sum over both halves (bounds are the same)
+        if (blocks > 0) {
+            ctl->half[i][half][row] = l;
+            pair_barrier(warp);
+            l += ctl->half[i][half ^ 1][row];
+        }
         if (ok) {
             tc_fence_after();
             const bool live = my_tok < t.tokens;
             const bool odd = *reinterpret_cast<volatile int *>(&ctl->odd_v) != 0;
             // a part's o is not normalised; o carries 2^kShift as l does
             const float f = pow2(max(e_v, -126)) * (t.part < 0 ? 1.f / l : 1.f);
-            T *dst = out + (static_cast<int64_t>(t.row0) + my_tok) * out_stride + (kGqa * h + (row & 3)) * kHeadDim;
+            T *dst = out + (static_cast<int64_t>(t.row0) + my_tok) * out_stride + (kGqa * h + (row & 3)) * kHeadDim +
+                     64 * half;
             float *part = work + (static_cast<int64_t>(t.part) * G + h) * kWindowPartFloats;
+#pragma unroll 1
             for (int c = 0; c < 4; ++c) {
-                float o[32];
+                float o[16];
                 if (blocks > 0) {
-                    tmem_load32(o_col + 32 * c, o);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) {
-                        o[k] = 0.f;
-                    }
+                    tmem_load16(o_col + 16 * c, o);
                 }
 #pragma unroll
-                for (int k = 0; k < 32; ++k) {
+                for (int k = 0; k < 16; ++k) {
                     o[k] = blocks > 0 ? o[k] * f : 0.f;
                 }
                 if (odd && live) {
                     const int keys = min(my_last + 1, t.blocks * kKeys);
                     for (int key = 0; key < keys; ++key) {
-                        const int64_t page = pages[t.page_off + (t.key0 + key) / kPageTokens];
-                        if (page < 0 || page >= pool.n_pages) {
-                            continue;
-                        }
+                        const int page = page_at(key / kPageTokens);
 #pragma unroll 1
-                        for (int k = 0; k < 32; ++k) {
-                            const float x = cached_value<kE4m3>(pool, page, layer, 1, h, key & 15, 32 * c + k);
+                        for (int k = 0; k < 16; ++k) {
+                            const float x =
+                                cached_value<kE4m3>(pool, page, layer, 1, h, key & 15, 64 * half + 16 * c + k);
                             if (!(fabsf(x) <= 3.402823466e38f)) {
 #pragma unroll
-                                for (int z = 0; z < 32; ++z) {
+                                for (int z = 0; z < 16; ++z) {
                                     o[z] += z == k ? x : 0.f;
                                 }
                             }
@@ -639,16 +684,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
                 if (t.part >= 0) {
-                    for (int k = 0; k < 32; k += 4) {
-                        store4(part + (i * kTile + row) * kHeadDim + 32 * c + k, o + k);
+                    for (int k = 0; k < 16; k += 4) {
+                        store4(part + (i * kTile + row) * kHeadDim + 64 * half + 16 * c + k, o + k);
                     }
                 } else if (live) {
-                    for (int k = 0; k < 32; k += 4) {
-                        store4(dst + 32 * c + k, o + k);
+                    for (int k = 0; k < 16; k += 4) {
+                        store4(dst + 16 * c + k, o + k);
                     }
                 }
             }
-            if (t.part >= 0) {
+            if (t.part >= 0 && half == 0) {
                 float2 *ml = reinterpret_cast<float2 *>(part + kWindowTokens * kGqa * kHeadDim);
                 ml[i * kTile + row] = make_float2(m, l);
             }
@@ -661,18 +706,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int tid = threadIdx.x - kSoftmaxThreads;
             // A half tile is 1024 (F16: a quarter, 512 x 2) 16-byte pieces: 8 bits, 16 dims of a
             // row; F16, 8 dims.  Steps of 1024 pieces, K (where it is converted) then V of
-            // each block; the pieces of kAhead steps are in registers: a step's loads go
-            // out when the step kAhead before it is stored.
+            // each block; the pieces of the next step are in registers: its loads go out
+            // when the step before it is stored.
             // Eight consecutive threads store to eight different bank groups: 8 bits, dims
             // 0-63 or 64-127 of two neighbouring rows (an even and an odd row's swizzles
             // interleave); F16, half a row.
             constexpr int kTileSteps = kE4m3 ? 1 : 2;
             constexpr int kSteps = (S::kCodeK ? 1 : 2) * kTileSteps;
-            constexpr int kAhead = 2;
+            constexpr int kAhead = 1;
             constexpr int kPieces = 1024;
             constexpr int kEach = (kPieces + kConvertThreads - 1) / kConvertThreads;
             static_assert(kConvertThreads % 16 == 0, "a thread keeps its place in the row");
-            static_assert(kSteps <= kAhead || kSteps % kAhead == 0, "steps keep their registers");
             const int c = kE4m3 ? ((tid >> 3) & 1) * 4 + (tid & 3) : tid & 15;  // piece of the row
             const int row0 = kE4m3 ? 2 * (tid >> 4) + ((tid >> 2) & 1) : tid >> 4;
             constexpr int kRowStep = (kE4m3 ? 2 : 1) * kConvertThreads / 16;
@@ -813,7 +857,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         break;
                     }
                 }
-                BlockScale &b = ctl->scale[j % kScaleSlots];
+                BlockScale &b = scales[j % S::kScaleSlots];
                 if (lane < kBlockPages) {
                     b.k_scale[lane] = scale_log2 * pow2(exps.x);
                     b.shift[lane] = static_cast<float>(kShift + (far ? 0 : d));
@@ -848,7 +892,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         } else if (lane == 0) {
             // ---------------------------------------------------------- products
-            issue_products<S>(ctl, q_smem, k_ring, v_ring, tmem, nb0, nb1, err);
+            const int i = warp - kIssuer;
+            issue_products<S>(ctl, q_smem, k_ring, v_ring, tmem, i, nb, i == 0 ? nb0 : nb1, err);
         }
     }
     if (bad >= 0) {
