@@ -831,11 +831,37 @@ int upload_rows(hkv_engine *eng, Staging &stage, RowCache &rc, int32_t n, const 
     return HKV_OK;
 }
 
-// The most key blocks one CTA of a window attention takes: enough CTAs for the GPU
-// where the tiles alone are too few, and no part shorter than two blocks (a CTA
-// costs about two blocks to start and join).
-int64_t window_split(int64_t total_blocks, int64_t n_head_kv, int64_t sms) {
-    return std::max<int64_t>(2, (total_blocks * n_head_kv + sms - 1) / sms);
+// The most key blocks one CTA of a window attention takes, of tiles with `blocks`
+// each.  Where the tiles alone do not fill the GPU's SMs, the least for which their
+// parts still run at once (700 tokens into an empty slot: 27 us at 3 blocks, 40 at 2,
+// where a few parts start a second wave; 37 tokens behind 770: 19 us at 1, 21 at 2, 25 at
+// 3).  Otherwise an SM's share of all blocks, so that no long tile ends the launch alone.
+int64_t window_split(const std::vector<int64_t> &blocks, int64_t n_head_kv, int64_t sms) {
+    auto ctas = [&](int64_t most) {
+        int64_t n = 0;
+        for (const int64_t b : blocks) {
+            n += (b + most - 1) / most;
+        }
+        return n * n_head_kv;
+    };
+    int64_t total = 0, longest = 1;
+    for (const int64_t b : blocks) {
+        total += b;
+        longest = std::max(longest, b);
+    }
+    if (ctas(longest) > sms) {
+        return (total * n_head_kv + sms - 1) / sms;
+    }
+    int64_t lo = 1, hi = longest;  // hi fits
+    while (lo < hi) {
+        const int64_t mid = (lo + hi) / 2;
+        if (ctas(mid) <= sms) {
+            hi = mid;
+        } else {
+            lo = mid + 1;
+        }
+    }
+    return hi;
 }
 
 // Uploads the tiles and page lists of a window attention call.
@@ -851,13 +877,13 @@ int upload_window(hkv_engine *eng, int32_t n, const int32_t *slots, const int64_
         const int64_t last = begin[e] + std::min<int64_t>(i + kWindowTokens, count[e]);
         return (last + kWindowKeys - 1) / kWindowKeys;
     };
-    int64_t total = 0;
+    std::vector<int64_t> all;
     for (int32_t e = 0; e < n; ++e) {
         for (int64_t i = 0; i < count[e]; i += kWindowTokens) {
-            total += blocks_of(e, i);
+            all.push_back(blocks_of(e, i));
         }
     }
-    const int64_t most = window_split(total, G, eng->num_sms);
+    const int64_t most = window_split(all, G, eng->num_sms);
     int64_t row0 = 0;
     int32_t parts = 0;
     for (int32_t e = 0; e < n; ++e) {
@@ -1850,6 +1876,7 @@ int hkv_window_attn(hkv_engine *eng, const hkv_window_attn_args *args, hkv_strea
     w.merges = wc.merges;
     w.n_merges = wc.n_merges;
     w.work = eng->window_work;
+    w.one_wave = static_cast<int64_t>(wc.n_tiles) * eng->cfg.n_head_kv <= eng->num_sms;
     {
         ProfileScope ps(eng, HKV_KERNEL_ATTN, stream);
         launch_window(pool_view(eng), w, eng->d_err, stream);

@@ -281,6 +281,7 @@ struct WindowArgs {
     void *out;
     int64_t q_stride, out_stride;  // elements per row
     float scale_log2;
+    bool one_wave;  // every CTA has an SM at once
 };
 void launch_window(const PoolView &pool, const WindowArgs &args, DeviceError *err, cudaStream_t stream);
 

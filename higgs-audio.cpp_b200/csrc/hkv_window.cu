@@ -381,18 +381,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t v_ring = k_ring + S::kKSlots * S::kKTile;
     Control *ctl = reinterpret_cast<Control *>(smem + S::kControl);
     BlockScale *scales = reinterpret_cast<BlockScale *>(ctl + 1);
-    const WindowTile t = tiles[blockIdx.x];
     const int h = blockIdx.y;
     const int G = pool.n_head_kv;
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
-    const int n_tiles = t.tokens > kTileTokens ? 2 : 1;
-    // blocks of each M tile: up to the last key that its last token sees
-    const int key_end0 = t.pos0 + min(t.tokens, kTileTokens) - t.key0;
-    const int nb0 = min(t.blocks, max(0, (key_end0 + kKeys - 1) / kKeys));
-    const int nb1 = n_tiles == 2 ? t.blocks : 0;
-    const int nb = max(nb0, nb1);
-
     if (warp == kIssuer) {
         tmem_alloc(smem_u32(&ctl->tmem), 512);
     }
@@ -405,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(smem_u32(&ctl->drained[i]), 1);
         }
         for (int i = 0; i < S::kKSlots; ++i) {
-            mbar_init(smem_u32(&ctl->k_full[i]), S::kCodeK ? 1 : kConvertThreads + 1);
+            mbar_init(smem_u32(&ctl->k_full[i]), S::kCodeK ? 2 : kConvertThreads + 1);
             mbar_init(smem_u32(&ctl->k_empty[i]), 2);
         }
         for (int i = 0; i < S::kVSlots; ++i) {
@@ -422,6 +414,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = ctl->tmem;
+    // set up while the kernel before this one ended; its writes from here on
+    pdl_wait();
+    pdl_trigger();
+    const WindowTile t = tiles[blockIdx.x];
+    const int n_tiles = t.tokens > kTileTokens ? 2 : 1;
+    // blocks of each M tile: up to the last key that its last token sees
+    const int key_end0 = t.pos0 + min(t.tokens, kTileTokens) - t.key0;
+    const int nb0 = min(t.blocks, max(0, (key_end0 + kKeys - 1) / kKeys));
+    const int nb1 = n_tiles == 2 ? t.blocks : 0;
+    const int nb = max(nb0, nb1);
+
 
     // The slot's pages from the CTA's first key on.  Past its last one that one is
     // read again: K there is masked, V zeroed.
@@ -553,15 +556,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             mx *= q_scale;
+            const float grow = b.grow;
+            e_v = b.e;
+            const bool far = kE4m3 && b.far != 0;
             // the row's maximum over both halves
             ctl->half[i][half][row] = mx;
             pair_barrier(warp);
             mx = fmaxf(mx, ctl->half[i][half ^ 1][row]);
             // the bound and E move (o has to follow) only when they must
-            if (__any_sync(0xffffffffu, mx > m + kSlack || b.grow < 1.f)) {
+            if (__any_sync(0xffffffffu, mx > m + kSlack || grow < 1.f)) {
                 const float m_new = fmaxf(m, mx);
                 const float corr = (m_new == -INFINITY ? 1.f : exp2_fast(m - m_new));
-                const float o_corr = corr * b.grow;
+                const float o_corr = corr * grow;
                 m = m_new;
                 l *= corr;
                 if (j > 0) {
@@ -577,8 +583,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             }
-            e_v = b.e;
-            const bool far = kE4m3 && b.far != 0;
             const float bound = m == -INFINITY ? 0.f : m;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -835,14 +839,32 @@ __global__ void __launch_bounds__(kThreads, 1)
             bool ok = true;
             for (int j = 0; ok && j < nb; ++j) {
                 const int slot = j % S::kKSlots;
+                const uint32_t bar = smem_u32(&ctl->k_full[slot]);
                 const int index = j * kBlockPages + (lane & 7);
+                const bool there = index <= last_page;
                 const int64_t page = page_at(index);
                 const uint8_t *unit = head_base + page * page_stride;
                 int2 exps = make_int2(0, 0);
                 if (kE4m3) {
                     exps = *reinterpret_cast<const int2 *>(unit + 2 * kCodeBlockBytes);
                 }
-                const bool there = index <= last_page;
+                if (j >= S::kKSlots) {
+                    ok = __all_sync(0xffffffffu, wait_for(&ctl->k_empty[slot], (j / S::kKSlots - 1) & 1, err));
+                    if (!ok) {
+                        break;
+                    }
+                }
+                if (S::kCodeK) {
+                    // the copies go out before the exponents are looked at
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(bar, kCodeTileBytes);
+                    }
+                    __syncwarp();
+                    if (lane < kBlockPages) {
+                        bulk_load(k_ring + slot * S::kKTile + lane * kCodeBlockBytes, unit, kCodeBlockBytes, bar,
+                                  keep_policy());
+                    }
+                }
                 int top = there ? exps.y : INT32_MIN;
 #pragma unroll
                 for (int off = 4; off > 0; off >>= 1) {
@@ -851,12 +873,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int e_new = max(e, top);
                 const int d = there ? exps.y - e_new : 0;
                 const bool far = __any_sync(0xffffffffu, d < -kFar);
-                if (j >= S::kKSlots) {
-                    ok = __all_sync(0xffffffffu, wait_for(&ctl->k_empty[slot], (j / S::kKSlots - 1) & 1, err));
-                    if (!ok) {
-                        break;
-                    }
-                }
                 BlockScale &b = scales[j % S::kScaleSlots];
                 if (lane < kBlockPages) {
                     b.k_scale[lane] = scale_log2 * pow2(exps.x);
@@ -870,17 +886,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 e = e_new;
                 __syncwarp();
-                const uint32_t bar = smem_u32(&ctl->k_full[slot]);
-                if (S::kCodeK) {
-                    if (lane == 0) {
-                        mbar_arrive_expect_tx(bar, kCodeTileBytes);
-                    }
-                    __syncwarp();
-                    if (lane < kBlockPages) {
-                        bulk_load(k_ring + slot * S::kKTile + lane * kCodeBlockBytes, unit, kCodeBlockBytes, bar,
-                                  keep_policy());
-                    }
-                } else if (lane == 0) {
+                if (lane == 0) {
                     mbar_arrive(bar);
                 }
             }
@@ -913,6 +919,8 @@ template <typename T>
 __global__ void __launch_bounds__(256)
     window_combine_kernel(const WindowMerge *__restrict__ merges, int G, const float *__restrict__ work,
                           T *__restrict__ out, int64_t out_stride) {
+    pdl_wait();
+    pdl_trigger();
     const WindowMerge g = merges[blockIdx.x];
     const int h = blockIdx.y;
     const int row = blockIdx.z * 8 + (threadIdx.x >> 5);
@@ -960,13 +968,28 @@ void launch_window_t(const PoolView &pool, const WindowArgs &a, DeviceError *err
     }
     const unsigned G = static_cast<unsigned>(pool.n_head_kv);
     T *out = static_cast<T *>(a.out);
-    window_kernel<T, kE4m3><<<dim3(static_cast<unsigned>(a.n_tiles), G), kThreads, Shape<T, kE4m3>::kSmem, stream>>>(
-        pool, a.tiles, a.pages, a.layer, static_cast<const T *>(a.q), a.q_stride, out, a.out_stride, a.work,
-        a.scale_log2, err);
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(a.n_tiles), G);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Shape<T, kE4m3>::kSmem;
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    // A launch of one wave is set up while the kernel before it runs (37 tokens behind
+    // 770: 25 -> 19 us with the parts of one block that this makes worth it); one of
+    // several waves ends 4% later so, its first CTAs then waiting in the places of the last.
+    cfg.numAttrs = a.one_wave ? 1 : 0;
+    cudaLaunchKernelEx(&cfg, window_kernel<T, kE4m3>, pool, a.tiles, a.pages, a.layer, static_cast<const T *>(a.q),
+                       a.q_stride, out, a.out_stride, a.work, a.scale_log2, err);
     if (a.n_merges > 0) {
-        window_combine_kernel<T>
-            <<<dim3(static_cast<unsigned>(a.n_merges), G, kWindowTokens * kGqa / 8), 256, 0, stream>>>(
-                a.merges, static_cast<int>(G), a.work, out, a.out_stride);
+        cfg.gridDim = dim3(static_cast<unsigned>(a.n_merges), G, kWindowTokens * kGqa / 8);
+        cfg.blockDim = dim3(256);
+        cfg.dynamicSmemBytes = 0;
+        cfg.numAttrs = 1;
+        cudaLaunchKernelEx(&cfg, window_combine_kernel<T>, a.merges, static_cast<int>(G),
+                           static_cast<const float *>(a.work), out, a.out_stride);
     }
 }
 
