@@ -159,6 +159,25 @@ __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
                  : "memory");
     return v;
 }
+// Loads that stay in order with the waits and barriers around them (volatile) and
+// products that the compiler may place among them as it likes (not volatile).
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ int2 lds8(uint32_t addr) {
+    int2 v;
+    asm volatile("ld.shared.v2.s32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ void mma_16816_pure(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+        "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint4 v) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
                  : "memory");
@@ -1370,44 +1389,64 @@ __global__ void __launch_bounds__(Ring<kE4m3, kCtaMerge>::kWarps * 32, 1)
                 fence_proxy_async_smem();
                 __syncwarp();
             }
+            // A page that is not there is the first one again, its logits masked: no
+            // branch parts the two pages' instructions, which the compiler then mixes.
+            if (cnt == 1) {
+                st[1] = st[0];
+            }
             const int g = lane >> 2;
             const int t = lane & 3;
             float sv[2][4];  // logits of rows g (heads a, b) and g + 8 of each page
-            int ev[2] = {kExpMin, kExpMin};
+            int ev[2];
+            {
+                uint4 kx[2][2], ky[2][2];  // rows g and g + 8: the same swizzle
+                float s_scale[2];
 #pragma unroll
-            for (int hh = 0; hh < 2; ++hh) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    sv[hh][j] = kNegInf;
-                }
-                if (hh < cnt) {
-                    float sc[4] = {0.f, 0.f, 0.f, 0.f};
-                    float sd[4] = {0.f, 0.f, 0.f, 0.f};
-                    const float s_scale = scale_log2 * pow2(ld_shared_s32(st[hh] + 2 * kCodeBlockBytes));
-                    ev[hh] = ld_shared_s32(st[hh] + 2 * kCodeBlockBytes + 4);
+                for (int hh = 0; hh < 2; ++hh) {
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        // rows g and g + 8: the same swizzle
                         const uint32_t at = st[hh] + g * kHeadDim + (((2 * t + i) ^ g) << 4);
-                        const uint4 x = ld_shared_v4(at);
-                        const uint4 y = ld_shared_v4(at + 8 * kHeadDim);
-                        const uint32_t w0[4] = {x.x, x.y, x.z, x.w};
-                        const uint32_t w1[4] = {y.x, y.y, y.z, y.w};
+                        kx[hh][i] = lds16(at);
+                        ky[hh][i] = lds16(at + 8 * kHeadDim);
+                    }
+                    const int2 e = lds8(st[hh] + 2 * kCodeBlockBytes);
+                    s_scale[hh] = scale_log2 * pow2(e.x);
+                    ev[hh] = e.y;
+                }
+                float sc[2][2][4] = {};
 #pragma unroll
-                        for (int ks = 0; ks < 4; ++ks) {
-                            mma_16816(ks & 1 ? sd : sc, codes_to_half2(w0[ks]), codes_to_half2(w1[ks]),
-                                      codes_to_half2_hi(w0[ks]), codes_to_half2_hi(w1[ks]), qb[4 * i + ks][0],
-                                      qb[4 * i + ks][1]);
+                for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks) {
+#pragma unroll
+                        for (int hh = 0; hh < 2; ++hh) {
+                            const uint32_t x = ks == 0 ? kx[hh][i].x : ks == 1 ? kx[hh][i].y : ks == 2 ? kx[hh][i].z : kx[hh][i].w;
+                            const uint32_t y = ks == 0 ? ky[hh][i].x : ks == 1 ? ky[hh][i].y : ks == 2 ? ky[hh][i].z : ky[hh][i].w;
+                            mma_16816_pure(sc[hh][ks & 1], codes_to_half2(x), codes_to_half2(y), codes_to_half2_hi(x),
+                                           codes_to_half2_hi(y), qb[4 * i + ks][0], qb[4 * i + ks][1]);
                         }
                     }
+                }
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {
                     const int tok = row0 + hh * kPageTokens + g;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        sc[j] += sd[j];
-                        sc[j] += __shfl_xor_sync(0xffffffffu, sc[j], 2);
-                        sv[hh][j] = tok + (j >> 1) * 8 < ntok ? sc[j] * s_scale : kNegInf;
+                        float x = sc[hh][0][j] + sc[hh][1][j];
+                        x += __shfl_xor_sync(0xffffffffu, x, 2);
+                        sv[hh][j] = hh < cnt && tok + (j >> 1) * 8 < ntok ? x * s_scale[hh] : kNegInf;
                     }
                 }
+            }
+            uint4 va[2], vb[2], vc[2], vd[2];  // rows 2t, 2t + 1, 2t + 8, 2t + 9 of each page's V
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+                const uint32_t vt = st[hh] + kCodeBlockBytes;
+                const int r = 2 * t;
+                va[hh] = lds16(vt + r * kHeadDim + ((g ^ r) << 4));
+                vb[hh] = lds16(vt + (r + 1) * kHeadDim + ((g ^ (r + 1)) << 4));
+                vc[hh] = lds16(vt + (r + 8) * kHeadDim + ((g ^ r) << 4));
+                vd[hh] = lds16(vt + (r + 9) * kHeadDim + ((g ^ (r + 1)) << 4));
             }
             float mx_a = fmaxf(fmaxf(sv[0][0], sv[0][2]), fmaxf(sv[1][0], sv[1][2]));
             float mx_b = fmaxf(fmaxf(sv[0][1], sv[0][3]), fmaxf(sv[1][1], sv[1][3]));
@@ -1458,27 +1497,19 @@ __global__ void __launch_bounds__(Ring<kE4m3, kCtaMerge>::kWarps * 32, 1)
             }
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh) {
-                if (hh < cnt) {
-                    const uint32_t vt = st[hh] + kCodeBlockBytes;
-                    const int r = 2 * t;
-                    const uint4 a = ld_shared_v4(vt + r * kHeadDim + ((g ^ r) << 4));
-                    const uint4 b = ld_shared_v4(vt + (r + 1) * kHeadDim + ((g ^ (r + 1)) << 4));
-                    const uint4 c = ld_shared_v4(vt + (r + 8) * kHeadDim + ((g ^ r) << 4));
-                    const uint4 d = ld_shared_v4(vt + (r + 9) * kHeadDim + ((g ^ (r + 1)) << 4));
-                    const uint32_t va[4] = {a.x, a.y, a.z, a.w};
-                    const uint32_t vb[4] = {b.x, b.y, b.z, b.w};
-                    const uint32_t vc[4] = {c.x, c.y, c.z, c.w};
-                    const uint32_t vd[4] = {d.x, d.y, d.z, d.w};
+                const uint32_t wa[4] = {va[hh].x, va[hh].y, va[hh].z, va[hh].w};
+                const uint32_t wb[4] = {vb[hh].x, vb[hh].y, vb[hh].z, vb[hh].w};
+                const uint32_t wc[4] = {vc[hh].x, vc[hh].y, vc[hh].z, vc[hh].w};
+                const uint32_t wd[4] = {vd[hh].x, vd[hh].y, vd[hh].z, vd[hh].w};
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) {
+                for (int w = 0; w < 4; ++w) {
 #pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            // dims 4w + 2 half and + 1 of the lane's 16, two rows a pair
-                            const uint32_t ab = __byte_perm(va[w], vb[w], half ? 0x7362 : 0x5140);
-                            const uint32_t cd = __byte_perm(vc[w], vd[w], half ? 0x7362 : 0x5140);
-                            mma_16816(o[2 * w + half], codes_to_half2(ab), codes_to_half2_hi(ab),
-                                      codes_to_half2(cd), codes_to_half2_hi(cd), pb[hh][0], pb[hh][1]);
-                        }
+                    for (int half = 0; half < 2; ++half) {
+                        // dims 4w + 2 half and + 1 of the lane's 16, two rows a pair
+                        const uint32_t ab = __byte_perm(wa[w], wb[w], half ? 0x7362 : 0x5140);
+                        const uint32_t cd = __byte_perm(wc[w], wd[w], half ? 0x7362 : 0x5140);
+                        mma_16816_pure(o[2 * w + half], codes_to_half2(ab), codes_to_half2_hi(ab), codes_to_half2(cd),
+                                       codes_to_half2_hi(cd), pb[hh][0], pb[hh][1]);
                     }
                 }
             }
