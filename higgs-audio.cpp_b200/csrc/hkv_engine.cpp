@@ -1782,7 +1782,7 @@ int hkv_qkv_write(hkv_engine *eng, const hkv_qkv_write_args *args, hkv_stream st
     if ((a.q_norm != nullptr || a.k_norm != nullptr) && !(a.eps >= 0.f && std::isfinite(a.eps))) {
         return fail(eng, HKV_ERR_INVALID, "eps must be finite and not negative");
     }
-    WriteArgs w = kv_write_args(nullptr, 0, a.layer, a.dtype, a.k, a.v, a.k_stride, a.v_stride, true);
+    WriteArgs w = kv_write_args(nullptr, 0, a.layer, a.dtype, a.k, a.v, a.k_stride, a.v_stride, a.rotated == 0);
     w.q = a.q;
     w.q_out = a.q_out;
     w.q_stride = a.q_stride;

@@ -102,7 +102,8 @@ class QkvWriteArgs(ctypes.Structure):
     _fields_ = [("layer", ctypes.c_int32), ("n", ctypes.c_int32),
                 ("slots", ctypes.POINTER(ctypes.c_int32)),
                 ("n_tokens", ctypes.POINTER(ctypes.c_int64)), ("dtype", ctypes.c_int32),
-                ("eps", ctypes.c_float), ("q", ctypes.c_void_p), ("k", ctypes.c_void_p),
+                ("rotated", ctypes.c_int32), ("eps", ctypes.c_float), ("q", ctypes.c_void_p),
+                ("k", ctypes.c_void_p),
                 ("v", ctypes.c_void_p), ("q_stride", ctypes.c_int64), ("k_stride", ctypes.c_int64),
                 ("v_stride", ctypes.c_int64), ("q_out_stride", ctypes.c_int64),
                 ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p),
@@ -457,12 +458,13 @@ class Engine:
     def qkv_write(self, layer: int, slots: Sequence[int], n_tokens: Sequence[int], q, k, v,
                   q_norm=None, k_norm=None, eps: float = 1e-6, q_out=None, dtype: int = F32,
                   q_stride: int = 0, k_stride: int = 0, v_stride: int = 0, q_out_stride: int = 0,
-                  stream=None) -> None:
-        """hkv_qkv_write: norm (optional) and rotation of q and k heads, K/V rows of several
-        slots into the cache, q to q_out.  Strides in elements, 0 for packed rows."""
+                  rotated: bool = False, stream=None) -> None:
+        """hkv_qkv_write: norm (optional) and rotation of q and k heads (unless they are
+        `rotated` already), K/V rows of several slots into the cache, q to q_out.  Strides in
+        elements, 0 for packed rows."""
         n, arr = _slots_arg(slots)
-        a = QkvWriteArgs(layer, n, arr, _counts_arg(n_tokens, n), dtype, eps, _ptr(q), _ptr(k),
-                         _ptr(v), q_stride, k_stride, v_stride, q_out_stride, _ptr(q_norm),
+        a = QkvWriteArgs(layer, n, arr, _counts_arg(n_tokens, n), dtype, 1 if rotated else 0, eps,
+                         _ptr(q), _ptr(k), _ptr(v), q_stride, k_stride, v_stride, q_out_stride, _ptr(q_norm),
                          _ptr(k_norm), _ptr(q_out))
         self._check(self.lib.hkv_qkv_write(self.handle, ctypes.byref(a), _stream(stream)))
 

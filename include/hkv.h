@@ -33,7 +33,7 @@
  *     q and the attention output are head-major [n_head][head_dim]; query
  *     head h reads KV head h / (n_head / n_head_kv) (:441-456).
  *   * Slot operations are thread-safe (one mutex per engine).  Compute calls
- *     on one engine share its split-partial buffer: issue them on one stream
+ *     on one engine share its split-partial buffers: issue them on one stream
  *     (or order the streams) in the order the GPU should run them.
  */
 #ifndef HKV_H
@@ -106,12 +106,13 @@ typedef struct hkv_pool_stats {
 
 /* Kernel ids for the CUDA-event profiler. */
 typedef enum hkv_kernel_id {
-    HKV_KERNEL_APPEND = 0,  /* hkv_append, hkv_rope_append, hkv_rope_append_range */
-    HKV_KERNEL_ATTN = 1,    /* hkv_decode_attn                                    */
+    HKV_KERNEL_APPEND = 0,  /* hkv_append, hkv_rope_append, hkv_rope_append_range,
+                               hkv_qkv_write                                      */
+    HKV_KERNEL_ATTN = 1,    /* hkv_decode_attn, hkv_window_attn                   */
     HKV_KERNEL_COMBINE = 2, /* reserved: nothing is recorded under this id; the
                                combine launch that follows some attention launches
                                is timed with them (ATTN or STEP)              */
-    HKV_KERNEL_GATHER = 3,  /* hkv_gather                                         */
+    HKV_KERNEL_GATHER = 3,  /* hkv_gather, hkv_cache_read                         */
     HKV_KERNEL_STEP = 4,    /* hkv_decode_step (append + attention, one launch)   */
     HKV_KERNEL_GEMV = 5,    /* Q4_K projections (hkv_q4k_*, hkv_backbone_decode)  */
     HKV_KERNEL_EMBED = 6,   /* embedding rows (hkv_backbone_embed_*)              */
@@ -253,7 +254,8 @@ int hkv_gather(hkv_engine *eng, int32_t slot, int32_t layer, int64_t pos0, int64
  * n_tokens[e]) (0: none), the rows of all slots back to back in q, k, v and q_out.
  * Each head of q and k is first normed where its weight is given,
  *     y = x / sqrt(mean(x^2) + eps) * w        (:5727-5733),
- * then rotated (NEOX, at its position); k and v go into the cache, q to q_out.
+ * then rotated (NEOX, at its position; not where `rotated` says that the caller has,
+ * whose rows then go in as they are); k and v go into the cache, q to q_out.
  * Sums are F32; q_out is rounded once, to dtype.  For prompts, windows and batches of
  * decode tokens whose projections are not hkv_q4k_qkv's; hkv_window_attn and
  * a later hkv_slot_advance follow it as after hkv_rope_append_range.  Strides are in
@@ -265,6 +267,7 @@ typedef struct hkv_qkv_write_args {
     const int32_t *slots;     /* host [n]                                       */
     const int64_t *n_tokens;  /* host [n]                                       */
     int32_t dtype;            /* hkv_dtype of q, k, v and q_out                 */
+    int32_t rotated;          /* nonzero: q and k are rotated already           */
     float eps;
     const void *q;            /* NULL or [rows][n_head][128]                    */
     const void *k, *v;        /* [rows][n_head_kv][128]                         */
@@ -283,8 +286,9 @@ int hkv_qkv_write(hkv_engine *eng, const hkv_qkv_write_args *args, hkv_stream st
  * (hkv_qkv_write's q_out); out: [rows][n_head * 128]; both of dtype, the rows of all
  * slots back to back, strides in elements (0: packed), each a multiple of 16 bytes.
  * Softmax statistics and sums are F32.  With F32 tensors q and the weights enter the
- * products in two F16 parts (22 bits, as in hkv_decode_attn; |q| up to 65504); with
- * F16 or BF16 ones q as it is and the weights rounded to F16. */
+ * products in two F16 parts (22 bits, as in hkv_decode_attn), with F16 or BF16 ones q
+ * as it is and the weights rounded to F16; |q| up to 65504, and to 2^-25 below 2^-14.
+ * A value that is not finite reaches the rows that see it and no other. */
 typedef struct hkv_window_attn_args {
     int32_t layer;
     int32_t n;                /* slots, each at most once */

@@ -470,6 +470,24 @@ def test_qkv_write_equals_the_appends(cache8):
             assert np.array_equal(p, q)
 
 
+def test_qkv_write_of_rotated_rows(cache8):
+    """`rotated`: the rows go in as they are, and q comes out as it went in."""
+    rng = np.random.default_rng(75)
+    import hkv
+    c = cache8(G=2)
+    s = c.slot()
+    k, v = rows(rng, 37, 2), rows(rng, 37, 2)
+    q = rng.standard_normal((37, 8 * D)).astype(np.float32)
+    out = torch.empty((37, 8 * D), device=DEV)
+    c.eng.qkv_write(0, [s], [37], dev(q), dev(k), dev(v), q_out=out, rotated=True)
+    c.model_write(s, k, v, roped=True)
+    c.eng.advance([s], 37)
+    c.check(s)
+    assert np.array_equal(out.cpu().numpy(), q)
+    with pytest.raises(hkv.HkvError, match="F16 caches"):  # what an 8-bit engine does not do
+        c.eng.split_export(2, 0)
+
+
 def test_calls_on_other_streams_and_engines(cache8):
     """Two engines on two streams in turn; the descriptor of one call outlives the next."""
     rng = np.random.default_rng(81)

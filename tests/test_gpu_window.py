@@ -170,6 +170,41 @@ def test_window_ignores_what_it_must_not_see(hkv_lib, cache):
 
 
 @pytest.mark.parametrize("cache", ["e4m3", "f16"])
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+def test_window_rows_before_a_value_that_is_not_finite(hkv_lib, cache, name):
+    """A NaN in one dim of V at position 40 (and inf, -inf in an F16 cache): rows before it do not
+    know of it, rows from it on have it in that dim and KV head alone."""
+    import hkv
+    rng = np.random.default_rng(27)
+    G = 2
+    eng = engine(hkv, G, cache)
+    s = eng.acquire()
+    fill(eng, rng, s, 10, G)
+    k, v = rows(rng, 90, G), rows(rng, 90, G)
+    v[30, 1, 77] = np.nan
+    if cache == "f16":
+        v[60, 0, 3], v[61, 0, 100] = np.inf, -np.inf
+    eng.rope_append_range(0, s, 90, dev(k), dev(v))
+    q = torch.from_numpy(rng.standard_normal((90, 8, D)).astype(np.float32)).to(DEV)
+    out = window(eng, hkv, [s], [90], q, name).float().cpu().numpy().reshape(90, 8, D)
+    want = np.zeros((90, 8, D), bool)
+    want[30:, 4:, 77] = True
+    assert np.array_equal(np.isnan(out), want)
+    if cache == "f16":
+        want[:] = False
+        want[60:, :4, 3] = want[61:, :4, 100] = True
+        assert np.array_equal(np.isinf(out), want)
+        assert (out[60:, :4, 3] > 0).all() and (out[61:, :4, 100] < 0).all()
+    k[50, 0, 5] = np.nan  # in K: the rows that see it, of that KV head
+    eng.rope_append_range(0, s, 90, dev(k), dev(np.nan_to_num(v, nan=1.0, posinf=1.0, neginf=1.0)))
+    out = window(eng, hkv, [s], [90], q, name).float().cpu().numpy().reshape(90, 8, D)
+    want[:] = False
+    want[50:, :4] = True
+    assert np.array_equal(np.isnan(out), want)
+    eng.close()
+
+
+@pytest.mark.parametrize("cache", ["e4m3", "f16"])
 def test_one_token_window_is_the_decode(hkv_lib, oracle, rope_tables, cache):
     """n_tokens = 1 against hkv_decode_attn on the same cache (both F32 paths)."""
     import hkv
