@@ -74,6 +74,13 @@ constexpr int kOtherRegs = 64;
 static_assert(4 * kSoftmaxRegs + 2 * kOtherRegs == 6 * 80, "the shares add up to the launch's registers");
 constexpr float kSlack = 8.f;
 constexpr int kShift = 7;               // weights enter 2^7 larger: at most 2^15 in F16
+// F32 tensors: blocks after which o moves from TMEM to the row's place in `out` (or in
+// the part) and is added there in F32.  The tensor cores cut their sums instead of
+// rounding them: each of a block's 16 products takes about 2^-24 of o away, always
+// towards zero, 1e-5 of it over 4000 keys.  Eight ragged windows (1024 keys on average
+// behind 2034): error 6.6e-6 and 431 us without, 2.5e-6 and 459 us every 8 blocks,
+// 1.5e-6 and 481 us every 4.
+constexpr int kDrainBlocks = 4;
 constexpr int kFar = 60;                // V exponents this far below E take the slow form
 
 // What the softmax needs of a block's pages.
@@ -191,6 +198,54 @@ __device__ __forceinline__ void store4(__nv_bfloat16 *p, const float *x) {
         make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
 }
 
+// 16 dims of a row, held by each of four neighbouring lanes, to 4 dims of the four rows:
+// o[4 r ..] is then row r's dims 4 j .. 4 j + 3 in lane j of the four.  Rows r are the
+// four heads of a token, so an access is 64 bytes of each instead of 16 of 32 rows.
+__device__ __forceinline__ void four_rows(float (&o)[16], int lane) {
+#pragma unroll
+    for (int step = 1; step < 4; step *= 2) {
+        const bool up = (lane & step) != 0;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            if ((r & step) == 0) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    float &a = o[4 * r + k], &b = o[4 * (r + step) + k];
+                    const float got = __shfl_xor_sync(0xffffffffu, up ? a : b, step);
+                    a = up ? got : a;
+                    b = up ? b : got;
+                }
+            }
+        }
+    }
+}
+// What the four lanes of a token hold of x, by row.
+__device__ __forceinline__ float4 of_rows(float x, int lane) {
+    const int from = lane & ~3;
+    return make_float4(__shfl_sync(0xffffffffu, x, from), __shfl_sync(0xffffffffu, x, from + 1),
+                       __shfl_sync(0xffffffffu, x, from + 2), __shfl_sync(0xffffffffu, x, from + 3));
+}
+__device__ __forceinline__ float row_of(const float4 &x, int r) {
+    return r == 0 ? x.x : r == 1 ? x.y : r == 2 ? x.z : x.w;
+}
+// o += scale * s, where the scale is not 0.
+__device__ __forceinline__ void plus4(float *o, const float4 &s, float scale) {
+    o[0] = scale != 0.f ? fmaf(s.x, scale, o[0]) : o[0];
+    o[1] = scale != 0.f ? fmaf(s.y, scale, o[1]) : o[1];
+    o[2] = scale != 0.f ? fmaf(s.z, scale, o[2]) : o[2];
+    o[3] = scale != 0.f ? fmaf(s.w, scale, o[3]) : o[3];
+}
+
+// *p += x in L2, and a load from there.
+__device__ __forceinline__ void add_at(float *p, const float *x) {
+    asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1,%2,%3,%4};" ::"l"(p), "f"(x[0]), "f"(x[1]), "f"(x[2]),
+                 "f"(x[3])
+                 : "memory");
+}
+__device__ __forceinline__ float4 load_at(const float *p) {
+    return __ldcg(reinterpret_cast<const float4 *>(p));
+}
+
 // A wait of one role.  One that runs out is recorded and ends its role; the waits
 // that depend on it run out in turn, and the CTA leaves.
 // The threads sleep in try_wait (20 us at a time), so that they leave the issue
@@ -278,21 +333,23 @@ __device__ __forceinline__ void issue_products(Control *ctl, uint32_t q_addr, ui
     };
     auto logits = [&](int j) {  // S_i of block j
         const uint32_t kb = k_ring + (j % S::kKSlots) * S::kKTile;
+        // the low part first: the tensor cores' F32 sums are cut, not rounded, and its own
+        // are 2^-11 as large
 #pragma unroll
-        for (int part = 0; part < S::kParts; ++part) {
+        for (int part = S::kParts - 1; part >= 0; --part) {
             const uint32_t qa = q_addr + (i * S::kParts + part) * S::kQPart;
             if (S::kCodeK) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     mma_ss_e4m3(tmem + i * kKeys, smem_desc(qa + k * 32, 16, 1024), smem_desc(kb + k * 32, 16, 1024),
-                                qk_desc, part > 0 || k > 0);
+                                qk_desc, part < S::kParts - 1 || k > 0);
                 }
             } else {
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     const uint32_t step = (k >> 2) * (kTileBytes / 2) + (k & 3) * 32;
                     mma_ss(tmem + i * kKeys, smem_desc(qa + step, 16, 1024), smem_desc(kb + step, 16, 1024), qk_desc,
-                           part > 0 || k > 0);
+                           part < S::kParts - 1 || k > 0);
                 }
             }
         }
@@ -306,7 +363,7 @@ __device__ __forceinline__ void issue_products(Control *ctl, uint32_t q_addr, ui
             for (int k = 0; k < 8; ++k) {
                 const uint32_t p = tmem + i * kKeys + (k >> 1) * 32 + part * 16 + (k & 1) * 8;
                 mma_ts(tmem + 256 + i * kHeadDim, p, smem_desc(vb + k * 2048, kTileBytes / 2, 1024), pv_desc,
-                       j > 0 || part > 0 || k > 0);
+                       (S::kSplit ? j % kDrainBlocks : j) > 0 || part > 0 || k > 0);
             }
         }
     };
@@ -524,6 +581,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         float m = -INFINITY, l = 0.f;
         int e_v = 0;
         bool ok = true;
+        const bool live = my_tok < t.tokens;
+        // the token's four rows, from this lane's dims on
+        const int my_dim = 64 * half + 4 * (lane & 3);
+        T *dst = out + (static_cast<int64_t>(t.row0) + my_tok) * out_stride + kGqa * h * kHeadDim + my_dim;
+        float *part = work + (static_cast<int64_t>(t.part) * G + h) * kWindowPartFloats;
+        float *part_rows = part + (i * kTile + (row & ~3)) * kHeadDim + my_dim;
+        // F32 tensors: where o is added up, and what that sum has to be multiplied by
+        float *sums = t.part >= 0 ? part_rows : reinterpret_cast<float *>(dst);
+        const bool keeps = t.part >= 0 || live;
+        float kept = 0.f;
         for (int j = 0; j < blocks; ++j) {
             if (!__all_sync(0xffffffffu, wait_for(&ctl->s_full[i], j & 1, err))) {
                 ok = false;
@@ -563,6 +630,35 @@ __global__ void __launch_bounds__(kThreads, 1)
             ctl->half[i][half][row] = mx;
             pair_barrier(warp);
             mx = fmaxf(mx, ctl->half[i][half ^ 1][row]);
+            const bool drain = S::kSplit && j > 0 && j % kDrainBlocks == 0;
+            if (drain) {
+                // where the bound has stood since the last time (as a rule), an addition
+                // in L2 that nothing waits for
+                const bool first = j == kDrainBlocks;
+                const bool in_place = !first && __all_sync(0xffffffffu, kept == 1.f);
+                const float4 scale = of_rows(kept, lane);
+#pragma unroll 1
+                for (int c = 0; c < 64; c += 16) {
+                    float o[16];
+                    tmem_load16(o_col + c, o);
+                    four_rows(o, lane);
+                    if (keeps && in_place) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            add_at(sums + r * kHeadDim + c, o + 4 * r);
+                        }
+                    } else if (keeps) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            if (!first) {
+                                plus4(o + 4 * r, load_at(sums + r * kHeadDim + c), row_of(scale, r));
+                            }
+                            store4(sums + r * kHeadDim + c, o + 4 * r);
+                        }
+                    }
+                }
+                kept = 1.f;
+            }
             // the bound and E move (o has to follow) only when they must
             if (__any_sync(0xffffffffu, mx > m + kSlack || grow < 1.f)) {
                 const float m_new = fmaxf(m, mx);
@@ -570,7 +666,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const float o_corr = corr * grow;
                 m = m_new;
                 l *= corr;
-                if (j > 0) {
+                kept *= o_corr;
+                if (j > 0 && !drain) {
 #pragma unroll 1
                     for (int c = 0; c < 64; c += 16) {
                         float o[16];
@@ -653,47 +750,49 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (ok) {
             tc_fence_after();
-            const bool live = my_tok < t.tokens;
             const bool odd = *reinterpret_cast<volatile int *>(&ctl->odd_v) != 0;
             // a part's o is not normalised; o carries 2^kShift as l does
-            const float f = pow2(max(e_v, -126)) * (t.part < 0 ? 1.f / l : 1.f);
-            T *dst = out + (static_cast<int64_t>(t.row0) + my_tok) * out_stride + (kGqa * h + (row & 3)) * kHeadDim +
-                     64 * half;
-            float *part = work + (static_cast<int64_t>(t.part) * G + h) * kWindowPartFloats;
+            const float4 f = of_rows(pow2(max(e_v, -126)) * (t.part < 0 ? 1.f / l : 1.f), lane);
+            const float4 scale = of_rows(kept, lane);
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
+            for (int c = 0; c < 64; c += 16) {
                 float o[16];
                 if (blocks > 0) {
-                    tmem_load16(o_col + 16 * c, o);
+                    tmem_load16(o_col + c, o);
                 }
+                four_rows(o, lane);
 #pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    o[k] = blocks > 0 ? o[k] * f : 0.f;
+                for (int r = 0; r < 4; ++r) {
+                    if (S::kSplit && blocks > kDrainBlocks && keeps) {
+                        plus4(o + 4 * r, load_at(sums + r * kHeadDim + c), row_of(scale, r));
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        o[4 * r + k] = blocks > 0 ? o[4 * r + k] * row_of(f, r) : 0.f;
+                    }
                 }
                 if (odd && live) {
                     const int keys = min(my_last + 1, t.blocks * kKeys);
                     for (int key = 0; key < keys; ++key) {
                         const int page = page_at(key / kPageTokens);
 #pragma unroll 1
-                        for (int k = 0; k < 16; ++k) {
-                            const float x =
-                                cached_value<kE4m3>(pool, page, layer, 1, h, key & 15, 64 * half + 16 * c + k);
+                        for (int k = 0; k < 4; ++k) {
+                            const float x = cached_value<kE4m3>(pool, page, layer, 1, h, key & 15, my_dim + c + k);
                             if (!(fabsf(x) <= 3.402823466e38f)) {
 #pragma unroll
                                 for (int z = 0; z < 16; ++z) {
-                                    o[z] += z == k ? x : 0.f;
+                                    o[z] += (z & 3) == k ? x : 0.f;
                                 }
                             }
                         }
                     }
                 }
-                if (t.part >= 0) {
-                    for (int k = 0; k < 16; k += 4) {
-                        store4(part + (i * kTile + row) * kHeadDim + 64 * half + 16 * c + k, o + k);
-                    }
-                } else if (live) {
-                    for (int k = 0; k < 16; k += 4) {
-                        store4(dst + 16 * c + k, o + k);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if (t.part >= 0) {
+                        store4(part_rows + r * kHeadDim + c, o + 4 * r);
+                    } else if (live) {
+                        store4(dst + r * kHeadDim + c, o + 4 * r);
                     }
                 }
             }

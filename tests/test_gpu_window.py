@@ -170,6 +170,30 @@ def test_window_ignores_what_it_must_not_see(hkv_lib, cache):
 
 
 @pytest.mark.parametrize("cache", ["e4m3", "f16"])
+def test_long_f32_sums_keep_their_bits(hkv_lib, cache):
+    """V = 1 everywhere: each output is the sum of the weights over itself.  The tensor cores cut each
+    of the 16 products of 128 keys by up to an ulp of the sum (at most 2^-23 of it, half of that on
+    average); over 30,000 keys added up there this would come to 1.4e-5.  With the sums moved out after
+    8 blocks at most 8 * 16 cuts act on any part of it: 128 * 2^-24 on average, and one rounding to F32
+    (2^-24) for each of the 30 moves and, of l, a few per block at random."""
+    import hkv
+    rng = np.random.default_rng(28)
+    n, t = 28000, 2100
+    eng = hkv.Engine(n_layers=1, n_head=4, n_head_kv=1, n_pages=2000, max_slots=1, context_length=n + t, device=0,
+                     shuffle_seed=9, cache=cache)
+    s = eng.acquire()
+    k = torch.from_numpy((rng.standard_normal((n + t, 1, D)) * 0.3).astype(np.float32)).to(DEV)
+    v = torch.ones_like(k)
+    eng.rope_append_range(0, s, n, k[:n].contiguous(), v[:n].contiguous())
+    eng.advance([s], n)
+    eng.rope_append_range(0, s, t, k[n:].contiguous(), v[n:].contiguous())
+    q = torch.from_numpy(rng.standard_normal((t, 4, D)).astype(np.float32)).to(DEV)
+    out = window(eng, hkv, [s], [t], q, "f32").double()
+    assert abs((out - 1).mean().item()) < 128 * 2.0 ** -24 + 31 * 2.0 ** -24
+    eng.close()
+
+
+@pytest.mark.parametrize("cache", ["e4m3", "f16"])
 @pytest.mark.parametrize("name", ["f32", "bf16"])
 def test_window_rows_before_a_value_that_is_not_finite(hkv_lib, cache, name):
     """A NaN in one dim of V at position 40 (and inf, -inf in an F16 cache): rows before it do not
