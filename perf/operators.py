@@ -157,6 +157,7 @@ def prepare(case, seed):
         pages = sum((p + t + PAGE - 1) // PAGE for p, t in zip(old, new))
         eng = hkv.Engine(n_layers=1, n_head=GROUP * heads, n_head_kv=heads, n_pages=pages, max_slots=n,
                          context_length=most, device=0, shuffle_seed=11, cache="e4m3")
+        turn = rotation(most)
         s["eng"], s["slots"] = eng, [eng.acquire(p + t) for p, t in zip(old, new)]
         s["dtype"] = {"f32": hkv.F32, "f16": hkv.F16, "bf16": hkv.BF16}[case.get("dtype", "f32")]
     else:
@@ -175,11 +176,13 @@ def prepare(case, seed):
     for e, (p, t) in enumerate(zip(old, new)):
         k, v = rows(gen, p, heads, gain), rows(gen, p, heads, 1.0)
         if own:
+            # rotated by this file's own table, so that both sides hold the same rows
             if p:
-                eng.rope_append_range(0, s["slots"][e], p, k, v)
+                eng.qkv_write(0, [s["slots"][e]], [p], None, rotate(k, turn[0][:p, None], turn[1][:p, None]), v, rotated=True)
                 eng.advance([s["slots"][e]], p)
             if behind:
-                eng.rope_append_range(0, s["slots"][e], t, s["k"][at:at + t], s["v"][at:at + t])
+                x = rotate(s["k"][at:at + t], turn[0][p:p + t, None], turn[1][p:p + t, None])
+                eng.qkv_write(0, [s["slots"][e]], [t], None, x, s["v"][at:at + t], rotated=True)
         else:
             for x, c, x_e in ((rotate(k, s["cos"][:p, None], s["sin"][:p, None]), s["kc"], s["ke"]), (v, s["vc"], s["ve"])):
                 full = (p + PAGE - 1) // PAGE * PAGE
