@@ -78,8 +78,8 @@ constexpr int kShift = 7;               // weights enter 2^7 larger: at most 2^1
 // the part) and is added there in F32.  The tensor cores cut their sums instead of
 // rounding them: each of a block's 16 products takes about 2^-24 of o away, always
 // towards zero, 1e-5 of it over 4000 keys.  Eight ragged windows (1024 keys on average
-// behind 2034): error 6.6e-6 and 431 us without, 2.5e-6 and 459 us every 8 blocks,
-// 1.5e-6 and 481 us every 4.
+// behind 2034): error 6.6e-6 and 434 us without, 2.5e-6 and 472 us every 8 blocks,
+// 1.5e-6 and 493 us every 4 (531 with sums read back and rescaled each time).
 constexpr int kDrainBlocks = 4;
 constexpr int kFar = 60;                // V exponents this far below E take the slow form
 
@@ -632,11 +632,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             mx = fmaxf(mx, ctl->half[i][half ^ 1][row]);
             const bool drain = S::kSplit && j > 0 && j % kDrainBlocks == 0;
             if (drain) {
-                // where the bound has stood since the last time (as a rule), an addition
-                // in L2 that nothing waits for
+                // brought to the sums' units, where those are not too far (2^60 leaves a
+                // sum of 2^15 weights of 2^15 and V below 2^126), for an addition in L2
+                // that nothing waits for
                 const bool first = j == kDrainBlocks;
-                const bool in_place = !first && __all_sync(0xffffffffu, kept == 1.f);
-                const float4 scale = of_rows(kept, lane);
+                const bool in_place = !first && __all_sync(0xffffffffu, kept >= 0x1p-60f);
+                const float4 scale = of_rows(in_place ? 1.f / kept : kept, lane);
 #pragma unroll 1
                 for (int c = 0; c < 64; c += 16) {
                     float o[16];
@@ -645,6 +646,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (keeps && in_place) {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                o[4 * r + k] *= row_of(scale, r);
+                            }
                             add_at(sums + r * kHeadDim + c, o + 4 * r);
                         }
                     } else if (keeps) {
@@ -657,7 +662,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                 }
-                kept = 1.f;
+                kept = in_place ? kept : 1.f;
             }
             // the bound and E move (o has to follow) only when they must
             if (__any_sync(0xffffffffu, mx > m + kSlack || grow < 1.f)) {

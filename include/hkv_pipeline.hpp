@@ -36,8 +36,8 @@ inline void check(const hkv_engine *eng, int status, const char *what) {
 // kv_cache_slots / kv_cache_slot_busy arena.
 class PagedKvRuntime {
   public:
-    explicit PagedKvRuntime(const hkv_config &cfg) {
-        check(nullptr, hkv_engine_create(&cfg, &eng_), "hkv_engine_create");
+    explicit PagedKvRuntime(const hkv_config &cfg, hkv_cache_type cache = HKV_CACHE_F16) {
+        check(nullptr, hkv_engine_create_cache(&cfg, cache, &eng_), "hkv_engine_create_cache");
     }
     ~PagedKvRuntime() {
         if (eng_ != nullptr) {
@@ -152,6 +152,37 @@ inline void decode_layer(PagedKvRuntime &rt, int layer, const std::vector<int32_
           hkv_decode_step(rt.engine(), layer, static_cast<int32_t>(slots.size()), slots.data(),
                           q, k, v, out, stream),
           "hkv_decode_step");
+}
+
+// One layer of a prompt or a refreshed window for several slots (:6278-6279, :6603-6604 and
+// the attention behind them): the rows' K and V into the caches, q and k rotated on the way,
+// then attention of each row over those up to its own.  n_tokens[e] rows of slots[e], back to
+// back in q, k, v and out; q is rotated in place.  hkv_slot_advance follows the last layer.
+inline void window_layer(PagedKvRuntime &rt, int layer, const std::vector<int32_t> &slots,
+                         const std::vector<int64_t> &n_tokens, float *q, const float *k,
+                         const float *v, float *out, hkv_stream stream) {
+    if (slots.size() != n_tokens.size()) {
+        throw std::out_of_range("window_layer: as many counts as slots");
+    }
+    hkv_qkv_write_args w{};
+    w.layer = layer;
+    w.n = static_cast<int32_t>(slots.size());
+    w.slots = slots.data();
+    w.n_tokens = n_tokens.data();
+    w.dtype = HKV_F32;
+    w.q = w.q_out = q;
+    w.k = k;
+    w.v = v;
+    check(rt.engine(), hkv_qkv_write(rt.engine(), &w, stream), "hkv_qkv_write");
+    hkv_window_attn_args a{};
+    a.layer = layer;
+    a.n = w.n;
+    a.slots = w.slots;
+    a.n_tokens = w.n_tokens;
+    a.dtype = HKV_F32;
+    a.q = q;
+    a.out = out;
+    check(rt.engine(), hkv_window_attn(rt.engine(), &a, stream), "hkv_window_attn");
 }
 
 }  // namespace hkv_pipeline
