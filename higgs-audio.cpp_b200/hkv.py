@@ -17,6 +17,7 @@ from __future__ import annotations
 import ctypes
 import os
 import re
+import struct
 from array import array
 from pathlib import Path
 from typing import Optional, Sequence
@@ -103,8 +104,7 @@ class QkvWriteArgs(ctypes.Structure):
                 ("slots", ctypes.POINTER(ctypes.c_int32)),
                 ("n_tokens", ctypes.POINTER(ctypes.c_int64)), ("dtype", ctypes.c_int32),
                 ("rotated", ctypes.c_int32), ("eps", ctypes.c_float), ("q", ctypes.c_void_p),
-                ("k", ctypes.c_void_p),
-                ("v", ctypes.c_void_p), ("q_stride", ctypes.c_int64), ("k_stride", ctypes.c_int64),
+                ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("q_stride", ctypes.c_int64), ("k_stride", ctypes.c_int64),
                 ("v_stride", ctypes.c_int64), ("q_out_stride", ctypes.c_int64),
                 ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p),
                 ("q_out", ctypes.c_void_p)]
@@ -117,6 +117,12 @@ class WindowAttnArgs(ctypes.Structure):
                 ("n_tokens", ctypes.POINTER(ctypes.c_int64)), ("dtype", ctypes.c_int32),
                 ("q", ctypes.c_void_p), ("out", ctypes.c_void_p), ("q_stride", ctypes.c_int64),
                 ("out_stride", ctypes.c_int64)]
+
+
+# The two structs' layouts: a packed copy costs a call a seventh of building the Structure.
+_QKV_WRITE = struct.Struct("@iiPPiifPPPqqqqPPP")
+_WINDOW_ATTN = struct.Struct("@iiPPiPPqq")
+assert _QKV_WRITE.size == ctypes.sizeof(QkvWriteArgs) and _WINDOW_ATTN.size == ctypes.sizeof(WindowAttnArgs)
 
 
 class PagedView(ctypes.Structure):
@@ -192,15 +198,15 @@ SIGNATURES = {
     "hkv_prefix_drop": ([_P, ctypes.POINTER(PrefixKey)], ctypes.c_int),
     "hkv_slot_pages": ([_P, _I32, _I32P, _I64, _I64P], ctypes.c_int),
     "hkv_pool_stats_get": ([_P, ctypes.POINTER(PoolStats)], ctypes.c_int),
-    "hkv_append": ([_P, _I32, _I32, _I32P, _P, _P, _P], ctypes.c_int),
-    "hkv_rope_append": ([_P, _I32, _I32, _I32P, _P, _P, _P], ctypes.c_int),
+    "hkv_append": ([_P, _I32, _I32, _P, _P, _P, _P], ctypes.c_int),
+    "hkv_rope_append": ([_P, _I32, _I32, _P, _P, _P, _P], ctypes.c_int),
     "hkv_rope_append_range": ([_P, _I32, _I32, _I64, _P, _P, _P], ctypes.c_int),
-    "hkv_decode_attn": ([_P, _I32, _I32, _I32P, _P, _P, _P], ctypes.c_int),
-    "hkv_decode_step": ([_P, _I32, _I32, _I32P, _P, _P, _P, _P, _P], ctypes.c_int),
+    "hkv_decode_attn": ([_P, _I32, _I32, _P, _P, _P, _P], ctypes.c_int),
+    "hkv_decode_step": ([_P, _I32, _I32, _P, _P, _P, _P, _P, _P], ctypes.c_int),
     "hkv_gather": ([_P, _I32, _I32, _I64, _I64, _P, _P, _P], ctypes.c_int),
-    "hkv_qkv_write": ([_P, ctypes.POINTER(QkvWriteArgs), _P], ctypes.c_int),
-    "hkv_window_attn": ([_P, ctypes.POINTER(WindowAttnArgs), _P], ctypes.c_int),
-    "hkv_cache_read": ([_P, _I32, _I32, _I32P, _I64P, _I64P, _I32, _P, _P, _P], ctypes.c_int),
+    "hkv_qkv_write": ([_P, _P, _P], ctypes.c_int),    # a QkvWriteArgs or its bytes
+    "hkv_window_attn": ([_P, _P, _P], ctypes.c_int),  # a WindowAttnArgs or its bytes
+    "hkv_cache_read": ([_P, _I32, _I32, _P, _P, _P, _I32, _P, _P, _P], ctypes.c_int),
     "hkv_sync_check": ([_P, _P], ctypes.c_int),
     "hkv_rope_tables": ([_P, _P, _P], ctypes.c_int),
     "hkv_decode_attn_noalloc": ([ctypes.POINTER(PagedView), _I32, _I32, _I32P, _I32P, _I32P,
@@ -264,8 +270,10 @@ def _ptr(x) -> Optional[int]:
         return None
     if isinstance(x, int):
         return x
-    if hasattr(x, "data_ptr"):
-        return int(x.data_ptr())
+    try:
+        return x.data_ptr()
+    except AttributeError:
+        pass
     if isinstance(x, np.ndarray):
         return int(x.ctypes.data)
     raise TypeError(f"cannot take a device pointer from {type(x)!r}")
@@ -286,10 +294,20 @@ def _slots_arg(slots: Sequence[int]):
     return len(a), (ctypes.c_int32 * len(a)).from_buffer(a)
 
 
-def _counts_arg(counts: Sequence[int], n: int):
-    if len(counts) != n:
-        raise ValueError(f"{len(counts)} lengths for {n} slots")
-    return (ctypes.c_int64 * n).from_buffer(array("q", counts))
+def _slots_in(slots: Sequence[int]):
+    """A slot list as an array (which the caller holds on to), its length and address."""
+    a = array("i", slots)
+    address, n = a.buffer_info()
+    return a, n, address
+
+
+def _counts_in(counts: Sequence[int], n: int):
+    """n lengths as an array (which the caller holds on to) and its address."""
+    a = array("q", counts)
+    address, have = a.buffer_info()
+    if have != n:
+        raise ValueError(f"{have} lengths for {n} slots")
+    return a, address
 
 
 class ScopedBackendKvCacheSlot:
@@ -421,12 +439,12 @@ class Engine:
 
     # ------------------------------------------------------------- compute
     def append(self, layer: int, slots: Sequence[int], k, v, stream=None) -> None:
-        n, arr = _slots_arg(slots)
+        held, n, arr = _slots_in(slots)
         self._check(self.lib.hkv_append(self.handle, layer, n, arr, _ptr(k), _ptr(v),
                                         _stream(stream)))
 
     def rope_append(self, layer: int, slots: Sequence[int], k, v, stream=None) -> None:
-        n, arr = _slots_arg(slots)
+        held, n, arr = _slots_in(slots)
         self._check(self.lib.hkv_rope_append(self.handle, layer, n, arr, _ptr(k), _ptr(v),
                                              _stream(stream)))
 
@@ -435,12 +453,12 @@ class Engine:
                                                    _ptr(v), _stream(stream)))
 
     def decode_attn(self, layer: int, slots: Sequence[int], q, out, stream=None) -> None:
-        n, arr = _slots_arg(slots)
+        held, n, arr = _slots_in(slots)
         self._check(self.lib.hkv_decode_attn(self.handle, layer, n, arr, _ptr(q), _ptr(out),
                                              _stream(stream)))
 
     def decode_step(self, layer: int, slots: Sequence[int], q, k, v, out, stream=None) -> None:
-        n, arr = _slots_arg(slots)
+        held, n, arr = _slots_in(slots)
         self._check(self.lib.hkv_decode_step(self.handle, layer, n, arr, _ptr(q), _ptr(k),
                                              _ptr(v), _ptr(out), _stream(stream)))
 
@@ -462,27 +480,30 @@ class Engine:
         """hkv_qkv_write: norm (optional) and rotation of q and k heads (unless they are
         `rotated` already), K/V rows of several slots into the cache, q to q_out.  Strides in
         elements, 0 for packed rows."""
-        n, arr = _slots_arg(slots)
-        a = QkvWriteArgs(layer, n, arr, _counts_arg(n_tokens, n), dtype, 1 if rotated else 0, eps,
-                         _ptr(q), _ptr(k), _ptr(v), q_stride, k_stride, v_stride, q_out_stride, _ptr(q_norm),
-                         _ptr(k_norm), _ptr(q_out))
-        self._check(self.lib.hkv_qkv_write(self.handle, ctypes.byref(a), _stream(stream)))
+        held, n, arr = _slots_in(slots)
+        lengths, counts = _counts_in(n_tokens, n)
+        a = _QKV_WRITE.pack(layer, n, arr, counts, dtype, 1 if rotated else 0, eps, _ptr(q) or 0,
+                            _ptr(k) or 0, _ptr(v) or 0, q_stride, k_stride, v_stride, q_out_stride,
+                            _ptr(q_norm) or 0, _ptr(k_norm) or 0, _ptr(q_out) or 0)
+        self._check(self.lib.hkv_qkv_write(self.handle, a, _stream(stream)))
 
     def window_attn(self, layer: int, slots: Sequence[int], n_tokens: Sequence[int], q, out,
                     dtype: int = F32, q_stride: int = 0, out_stride: int = 0, stream=None) -> None:
         """hkv_window_attn: token i of each slot over its rows [0, used + i]; q rotated."""
-        n, arr = _slots_arg(slots)
-        a = WindowAttnArgs(layer, n, arr, _counts_arg(n_tokens, n), dtype, _ptr(q), _ptr(out),
-                           q_stride, out_stride)
-        self._check(self.lib.hkv_window_attn(self.handle, ctypes.byref(a), _stream(stream)))
+        held, n, arr = _slots_in(slots)
+        lengths, counts = _counts_in(n_tokens, n)
+        a = _WINDOW_ATTN.pack(layer, n, arr, counts, dtype, _ptr(q) or 0, _ptr(out) or 0, q_stride,
+                              out_stride)
+        self._check(self.lib.hkv_window_attn(self.handle, a, _stream(stream)))
 
     def cache_read(self, layer: int, slots: Sequence[int], pos0: Sequence[int],
                    n_rows: Sequence[int], k_out, v_out, dtype: int = F16, stream=None) -> None:
         """hkv_cache_read: rows of several slots as F16 or F32 values, packed."""
-        n, arr = _slots_arg(slots)
-        self._check(self.lib.hkv_cache_read(self.handle, layer, n, arr, _counts_arg(pos0, n),
-                                            _counts_arg(n_rows, n), dtype, _ptr(k_out),
-                                            _ptr(v_out), _stream(stream)))
+        held, n, arr = _slots_in(slots)
+        firsts, first = _counts_in(pos0, n)
+        lengths, counts = _counts_in(n_rows, n)
+        self._check(self.lib.hkv_cache_read(self.handle, layer, n, arr, first, counts, dtype,
+                                            _ptr(k_out), _ptr(v_out), _stream(stream)))
 
     def sync_check(self, stream=None) -> None:
         self._check(self.lib.hkv_sync_check(self.handle, _stream(stream)))
