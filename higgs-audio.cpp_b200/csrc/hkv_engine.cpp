@@ -294,6 +294,8 @@ struct hkv_engine {
     int64_t kernel_launches = 0;  // every kernel this engine enqueued
     std::vector<hkv::Slot> slots;
     std::vector<int32_t> free_slots;  // stack
+    std::vector<uint32_t> slot_marks;  // of each slot: the last call that listed it (check_row_slots)
+    uint32_t slot_mark = 0;
     std::map<std::pair<uint64_t, int64_t>, hkv::Prefix> prefixes;
     uint64_t epoch = 1;
     int64_t page_bytes = 0;
@@ -973,15 +975,19 @@ int check_row_slots(hkv_engine *eng, int32_t n, const int32_t *slots, const int6
         return fail(eng, HKV_ERR_INVALID, "empty slot list");
     }
     *total = 0;
+    eng->slot_marks.resize(eng->slots.size());
+    if (++eng->slot_mark == 0) {  // wrapped: old marks are not to be taken for new ones
+        std::fill(eng->slot_marks.begin(), eng->slot_marks.end(), 0u);
+        eng->slot_mark = 1;
+    }
     for (int32_t e = 0; e < n; ++e) {
         if (!slot_ok(eng, slots[e])) {
             return fail(eng, HKV_ERR_BAD_SLOT, "slot %d is not live (batch entry %d)", slots[e], e);
         }
-        for (int32_t f = 0; f < e; ++f) {
-            if (slots[f] == slots[e]) {
-                return fail(eng, HKV_ERR_INVALID, "slot %d appears twice in one batch", slots[e]);
-            }
+        if (eng->slot_marks[slots[e]] == eng->slot_mark) {
+            return fail(eng, HKV_ERR_INVALID, "slot %d appears twice in one batch", slots[e]);
         }
+        eng->slot_marks[slots[e]] = eng->slot_mark;
         if (count[e] < 0 || count[e] > eng->cfg.context_length) {
             return fail(eng, HKV_ERR_RANGE, "%lld rows for batch entry %d", static_cast<long long>(count[e]), e);
         }
@@ -1634,6 +1640,8 @@ int hkv_rope_append_range(hkv_engine *eng, int32_t layer, int32_t slot, int64_t 
     const int64_t begin = s.used;
     const int64_t end = s.used + n_tokens;
     if (eng->cache_type == HKV_CACHE_E4M3) {
+        st = refuse_capture(eng, stream);
+        if (st != HKV_OK) return st;
         const int64_t row = static_cast<int64_t>(eng->cfg.n_head_kv) * kHeadDim;
         return write_rows(eng, kv_write_args(nullptr, 0, layer, HKV_F32, k_prerope, v, row, row, true), 1, &slot,
                           &begin, &n_tokens, stream);

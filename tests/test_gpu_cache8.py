@@ -537,6 +537,24 @@ def test_capture_is_refused(cache8):
     c.check(s)
 
 
+def test_range_append_in_a_capture_is_refused(cache8):
+    import hkv
+    c = cache8(G=1)
+    s = c.slot()
+    z = torch.zeros((4, 1, D), device=DEV)
+    c.prefill(s, np.ones((4, 1, D), np.float32), np.ones((4, 1, D), np.float32))
+    side = torch.cuda.Stream()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        g.capture_begin()
+        try:
+            with pytest.raises(hkv.HkvError, match="captured"):
+                c.eng.rope_append_range(0, s, 4, z, z, stream=side.cuda_stream)
+        finally:
+            g.capture_end()
+    c.check(s)
+
+
 def test_backbone_runs_on_an_8_bit_cache(hkv_lib):
     """hkv_backbone_decode on an E4M3 engine: the fused step equals the calls it is made of."""
     import hkv

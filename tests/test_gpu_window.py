@@ -193,6 +193,37 @@ def test_long_f32_sums_keep_their_bits(hkv_lib, cache):
     eng.close()
 
 
+@pytest.mark.parametrize("cache,rise,v_step", [
+    ("e4m3", 10.0, 0), ("e4m3", -10.0, 0), ("e4m3", 0.0, 3), ("e4m3", 0.0, -3), ("e4m3", 4.0, 3), ("f16", 10.0, 0),
+    ("f16", 4.0, 1)])
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+def test_long_tiles_whose_bounds_move(hkv_lib, cache, rise, v_step, name):
+    """Sixteen slots of 8 KV heads, so that no tile is split: 17 blocks of keys whose logits rise or fall
+    by up to 163 bits over the slot, and V pages whose sizes do, by 2^51: what is summed first has to be
+    held in other units many times, and to vanish in the end."""
+    import hkv
+    rng = np.random.default_rng(29)
+    G, n = 8, 2100
+    eng = engine(hkv, G, cache, n_pages=16 * 134)
+    dirs = rng.choice([-1.0, 1.0], (1, G, D)).astype(np.float32)
+    new = [20] * 15 + [64]
+    slots = [eng.acquire() for _ in new]
+    for s, t in zip(slots, new):
+        at = np.arange(n + t, dtype=np.float32) / n
+        k = dirs * (rise * (at - 0.5))[:, None, None] + 0.05 * rows(rng, n + t, G)
+        v = rows(rng, n + t, G) * np.exp2(v_step * (np.arange(n + t) // 128 - 8)).astype(np.float32)[:, None, None]
+        for r0, r1 in ((0, n), (n, n + t)):
+            eng.qkv_write(0, [s], [r1 - r0], None, dev(k[r0:r1]), dev(v[r0:r1]), rotated=True)
+            if r0 == 0:
+                eng.advance([s], n)
+    q = np.repeat(dirs, sum(new), 0).repeat(4, 1) + 0.3 * rng.standard_normal((sum(new), 4 * G, D)).astype(np.float32)
+    q = torch.from_numpy(q.astype(np.float32)).to(DEV)
+    out = window(eng, hkv, slots, new, q, name)
+    check(eng, hkv, slots, new, q, out, name)
+    assert torch.equal(out, window(eng, hkv, slots, new, q, name))
+    eng.close()
+
+
 @pytest.mark.parametrize("cache", ["e4m3", "f16"])
 @pytest.mark.parametrize("name", ["f32", "bf16"])
 def test_window_rows_before_a_value_that_is_not_finite(hkv_lib, cache, name):
