@@ -102,7 +102,8 @@ struct BlockScale {
 };
 
 struct Control {
-    uint64_t q_full, s_full[2], p_full[2], o_full[2];
+    uint64_t q_full, s_full[2], o_full[2];
+    uint64_t p_full[2][2];      // of a tile: weights of keys 0-31 and 64-95 of the block, and of the others
     uint64_t k_full[3], k_empty[3], v_full[3], v_empty[3];
     uint64_t turn[2];           // of the issuers: a phase a block
     uint64_t drained[2];        // after a wait that ran out: no product in flight
@@ -120,6 +121,10 @@ struct Shape {
     static constexpr bool kSplit = sizeof(T) == 4;
     static constexpr bool kCodeK = kE4m3 && std::is_same<T, __nv_bfloat16>::value;
     static constexpr int kParts = kSplit || kCodeK ? 2 : 1;  // of q
+    // F32: the products of half a block's weights start while the other half's are
+    // formed (8100 tokens 1230 -> 1197 us); a BF16 block's softmax is too short for that
+    // to pay for its second store and barrier (611 -> 616 us).
+    static constexpr bool kEarly = kSplit;
     static constexpr int kQPart = kCodeK ? kCodeTileBytes : kTileBytes;
     static constexpr int kKTile = kCodeK ? kCodeTileBytes : kTileBytes;
     static constexpr int kKSlots = kSplit ? 1 : kCodeK ? 3 : 2;
@@ -144,6 +149,11 @@ __device__ __forceinline__ void record(DeviceError *err, int code, int a, int b)
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
 }
 __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
@@ -362,15 +372,16 @@ __device__ __forceinline__ void issue_products(Control *ctl, uint32_t q_addr, ui
         }
         tc_commit(smem_u32(&ctl->s_full[i]));
     };
-    auto weigh = [&](int j) {  // O_i += P_i V of block j
+    auto weigh = [&](int j, int c) {  // O_i += P_i V of block j, the keys that p_full[i][c] stands for
         const uint32_t vb = v_ring + (j % S::kVSlots) * kTileBytes;
 #pragma unroll
         for (int part = 0; part < (S::kSplit ? 2 : 1); ++part) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
+            for (int n = 0; n < 4; ++n) {
+                const int k = 4 * (n >> 1) + 2 * c + (n & 1);
                 const uint32_t p = tmem + i * kKeys + (k >> 1) * 32 + part * 16 + (k & 1) * 8;
                 mma_ts(tmem + 256 + i * kHeadDim, p, smem_desc(vb + k * 2048, kTileBytes / 2, 1024), pv_desc,
-                       (S::kSplit ? j % kDrainBlocks : j) > 0 || part > 0 || k > 0);
+                       (S::kSplit ? j % kDrainBlocks : j) > 0 || part > 0 || c > 0 || n > 0);
             }
         }
     };
@@ -404,13 +415,24 @@ __device__ __forceinline__ void issue_products(Control *ctl, uint32_t q_addr, ui
             continue;
         }
         const bool more = j + 1 < blocks;
-        ok = v_ready(j) && (S::kKSlots == 1 || !more || k_ready(j + 1)) && wait_for(&ctl->p_full[i], j & 1, err) &&
-             turn(j + 1);
+        ok = v_ready(j);
+        if (S::kEarly) {
+            ok = ok && wait_for(&ctl->p_full[i][0], j & 1, err);
+            if (!ok) {
+                break;
+            }
+            tc_fence_after();
+            weigh(j, 0);
+        }
+        ok = ok && (S::kKSlots == 1 || !more || k_ready(j + 1)) && wait_for(&ctl->p_full[i][1], j & 1, err) && turn(j + 1);
         if (!ok) {
             break;
         }
         tc_fence_after();
-        weigh(j);
+        if (!S::kEarly) {
+            weigh(j, 0);
+        }
+        weigh(j, 1);
         if (more) {
             ok = S::kKSlots > 1 || k_ready(j + 1);
             if (!ok) {
@@ -456,7 +478,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(smem_u32(&ctl->q_full), kSoftmaxThreads);
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&ctl->s_full[i]), 1);
-            mbar_init(smem_u32(&ctl->p_full[i]), kTileThreads);
+            mbar_init(smem_u32(&ctl->p_full[i][0]), kTileThreads);
+            mbar_init(smem_u32(&ctl->p_full[i][1]), kTileThreads);
             mbar_init(smem_u32(&ctl->o_full[i]), 1);
             mbar_init(smem_u32(&ctl->drained[i]), 1);
         }
@@ -622,10 +645,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int p = 0; p < 2; ++p) {
                     float a = s[16 * p], d = s[16 * p + 1];
 #pragma unroll
-                    for (int k = 2; k < 16; k += 2) {
-                        a = fmaxf(a, s[16 * p + k]);
-                        d = fmaxf(d, s[16 * p + k + 1]);
+                    for (int k = 2; k < 14; k += 4) {
+                        a = max3(a, s[16 * p + k], s[16 * p + k + 1]);
+                        d = max3(d, s[16 * p + k + 2], s[16 * p + k + 3]);
                     }
+                    a = max3(a, s[16 * p + 14], s[16 * p + 15]);
                     mx = fmaxf(mx, fmaxf(a, d) * b.k_scale[4 * half + 2 * c + p]);
                 }
             }
@@ -734,10 +758,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
-                        hi[8 * p + k] = half2_bits(x[k].x, x[k].y);
-                        if (S::kSplit) {
-                            const float2 f = half2_floats(hi[8 * p + k]);
-                            lo[8 * p + k] = half2_bits(x[k].x - f.x, x[k].y - f.y);
+                        if (S::kSplit && kE4m3) {
+                            // cut, not rounded, so that the low part does not wait for
+                            // the high one's conversion: 22 bits all the same (two more
+                            // registers, which the form for F16 pages does not have)
+                            const float2 f = make_float2(__uint_as_float(__float_as_uint(x[k].x) & 0xffffe000u),
+                                                         __uint_as_float(__float_as_uint(x[k].y) & 0xffffe000u));
+                            const float2 r = fma2(f, make_float2(-1.f, -1.f), x[k]);
+                            hi[8 * p + k] = half2_bits(f.x, f.y);
+                            lo[8 * p + k] = half2_bits(r.x, r.y);
+                        } else {
+                            hi[8 * p + k] = half2_bits(x[k].x, x[k].y);
+                            if (S::kSplit) {
+                                const float2 f = half2_floats(hi[8 * p + k]);
+                                lo[8 * p + k] = half2_bits(x[k].x - f.x, x[k].y - f.y);
+                            }
                         }
                     }
                 }
@@ -746,10 +781,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (S::kSplit) {
                     tmem_store16(s_col + 32 * c + 16, lo);
                 }
+                if (S::kEarly || c == 1) {
+                    tmem_store_wait();
+                    tc_fence_before();
+                    mbar_arrive(smem_u32(&ctl->p_full[i][c]));
+                }
             }
-            tmem_store_wait();
-            tc_fence_before();
-            mbar_arrive(smem_u32(&ctl->p_full[i]));
         }
         if (ok && blocks > 0) {
             ok = __all_sync(0xffffffffu, wait_for(&ctl->o_full[i], 0, err));
