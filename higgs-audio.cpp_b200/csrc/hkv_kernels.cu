@@ -840,7 +840,7 @@ __global__ void __launch_bounds__(Ring<kE4m3, kCtaMerge>::kWarps * 32, 1)
     constexpr int kStages = Ring<kE4m3, kCtaMerge>::kStages;
     constexpr int kStage = Ring<kE4m3, kCtaMerge>::kStage;
     constexpr int kWarpSmem = Ring<kE4m3, kCtaMerge>::kWarpSmem;
-    constexpr int kMergeBatch = Ring<kE4m3, kCtaMerge>::kWarps > 8 ? 4 : 8;  // by the registers a thread has
+    constexpr int kMergeBatch = Ring<kE4m3, kCtaMerge>::kWarps > 8 ? 5 : 8;  // by the registers a thread has
     float *cta_slots = reinterpret_cast<float *>(smem + kAttnWarps * kWarpSmem);
     int *run_ticket = reinterpret_cast<int *>(smem + kAttnWarps * kWarpSmem + kAttnWarps * 2 * kCtaPartBytes);
     float *cl_slots = reinterpret_cast<float *>(smem + kAttnWarps * kWarpSmem + kCtaSmem);

@@ -94,6 +94,15 @@ constexpr int32_t kCombineMaxParts = 32;
 inline bool plan_combine(bool cta_merge, int32_t max_parts) {
     return cta_merge && max_parts > 1 && max_parts <= kCombineMaxParts;
 }
+// For the wide variant of the 8-bit kernel the combine launch pays where a segment
+// would take two levels, which a batch of unequal lengths then waits for: 16 slots of
+// 256-4096 positions 25.3 -> 22.3 us, 32 of 32-2048 20.2 -> 18.8, 20 of 1-8000 38.4 ->
+// 37.7 (layers one behind the other without a pause: 22.1 -> 21.1, 17.7 -> 17.8, 35.1 ->
+// 36.0).  With equal lengths, one level each, it loses: 24 of 2000 27.8 -> 28.6, 64 of
+// 500 23.6 -> 25.2.
+inline bool plan_wide_combine(int32_t max_parts) {
+    return max_parts > kMergeSingleMax && max_parts <= kCombineMaxParts;
+}
 
 // Share costs in sixteenths of a unit, from per-warp timestamps of the
 // attention kernel on B200 (16 slots of 256-4096 positions): a unit takes
@@ -350,7 +359,7 @@ inline PlanSummary build_plan(int32_t *w, int32_t n, int32_t G, const int32_t *p
         starts[k] = static_cast<int32_t>(U);
     }
     fill_records(a, n, G, W, starts.data(), s.cta_merge ? kAttnWarps : 1, s);
-    s.combine = plan_combine(s.cta_merge, s.max_parts);
+    s.combine = rules.cta_merge ? plan_combine(s.cta_merge, s.max_parts) : plan_wide_combine(s.max_parts);
     return s;
 }
 

@@ -222,6 +222,39 @@ def test_decode_over_ragged_lengths(cache8, G, fused):
         slots = slots[::-1]
 
 
+@pytest.mark.parametrize("seed,n,hi", [(7, 16, 4096), (1, 32, 2048), (2, 15, 2000), (3, 20, 8000)])
+def test_decode_over_batches_of_unequal_lengths(cache8, seed, n, hi):
+    """Segments of more than 16 partials among shorter ones (the combine launch), and of more than 32
+    (two levels in the launch): the fused step and the separate calls agree bit for bit, and every third
+    slot is within the bound of float64."""
+    rng = np.random.default_rng(seed)
+    lens = [hi] + [int(x) for x in rng.integers(1, hi, n - 1)]
+    c = cache8(G=8, n_pages=sum(x // PAGE + 2 for x in lens), max_slots=n, context=hi + 32)
+    slots = [c.slot() for _ in lens]
+    for s, t in zip(slots, lens):
+        c.eng.rope_append_range(0, s, t, dev(rows(rng, t, 8)), dev(rows(rng, t, 8)))
+        c.eng.advance([s], t)
+    q, k, v = (rng.standard_normal((n, h, D)).astype(np.float32) for h in (32, 8, 8))
+    out, again = torch.zeros((2, n, 32 * D), device=DEV).unbind(0)
+    c.eng.rope_append(0, slots, dev(k), dev(v))
+    c.eng.decode_attn(0, slots, dev(q), out)
+    c.eng.decode_step(0, slots, dev(q), dev(k), dev(v), again)
+    c.eng.sync_check()
+    assert torch.equal(out, again)
+    q_rot = torch.empty((n, 32, D), device=DEV)
+    kk, vv = torch.empty((2, max(lens) + 1, 8, D), device=DEV).unbind(0)
+    import hkv
+    c.eng.qkv_write(0, slots, [1] * n, dev(q), dev(k), dev(v), q_out=q_rot)
+    for e in range(0, n, 3):
+        t = lens[e] + 1
+        c.eng.cache_read(0, [slots[e]], [0], [t], kk, vv, dtype=hkv.F32)
+        torch.cuda.synchronize()
+        k64, v64 = kk[:t].cpu().numpy(), vv[:t].cpu().numpy()
+        want, big = attention(q_rot[e:e + 1].double().cpu().numpy(), k64, v64, t - 1)
+        got = out[e].double().cpu().numpy().reshape(1, 32, D)
+        assert float(np.abs(got - want).max()) <= attention_tolerance(big, t, np.abs(v64).max()), e
+
+
 @pytest.mark.parametrize("G,length", [(8, 1100), (8, 1500), (8, 32767), (1, 32767), (2, 5000), (1, 17)])
 def test_decode_of_one_request(cache8, G, length):
     """One request alone: its segments go through clusters, the combine launch or groups."""
