@@ -259,6 +259,38 @@ def test_window_rows_before_a_value_that_is_not_finite(hkv_lib, cache, name):
     eng.close()
 
 
+@pytest.mark.parametrize("cache,n_pages", [("e4m3", 140000), ("f16", 72000)])
+def test_pools_beyond_32_bit_offsets(hkv_lib, cache, n_pages):
+    """Layers of 4.6 GB, pages scattered over them: writes, reads, windows and a decode step in the
+    second layer (bytes 4.6e9 to 9.2e9 of the pool)."""
+    import hkv
+    rng = np.random.default_rng(30)
+    G = 8
+    eng = hkv.Engine(n_layers=2, n_head=4 * G, n_head_kv=G, n_pages=n_pages, max_slots=4, context_length=4096, device=0,
+                     shuffle_seed=31, cache=cache)
+    old, new = [300, 17, 0], [70, 64, 33]
+    slots = [eng.acquire() for _ in old]
+    for s, p, n in zip(slots, old, new):
+        fill(eng, rng, s, p, G, layer=1)
+        fill(eng, rng, s, n, G, layer=1, advance=False)
+    assert max(max(eng.pages(s)) for s in slots) > n_pages // 2
+    q = torch.from_numpy(rng.standard_normal((sum(new), 4 * G, D)).astype(np.float32)).to(DEV)
+    for name in ("f32", "bf16"):
+        check(eng, hkv, slots, new, q, window(eng, hkv, slots, new, q, name, layer=1), name, layer=1)
+    for s, n in zip(slots, new):
+        eng.advance([s], n)
+    # one token more: the decode step's output is the window's over the row it wrote
+    x, k, v = (torch.from_numpy(rng.standard_normal((3, h, D)).astype(np.float32)).to(DEV) for h in (4 * G, G, G))
+    step = torch.empty((3, 4 * G * D), device=DEV)
+    eng.decode_step(1, slots, x, k, v, step)
+    turned = torch.empty_like(x)
+    eng.qkv_write(1, slots, [1] * 3, x, k, v, q_out=turned)
+    one = window(eng, hkv, slots, [1] * 3, turned, layer=1)
+    check(eng, hkv, slots, [1] * 3, turned, one, "f32", layer=1)
+    check(eng, hkv, slots, [1] * 3, turned, step, "f32", layer=1)
+    eng.close()
+
+
 @pytest.mark.parametrize("cache", ["e4m3", "f16"])
 def test_one_token_window_is_the_decode(hkv_lib, oracle, rope_tables, cache):
     """n_tokens = 1 against hkv_decode_attn on the same cache (both F32 paths)."""
