@@ -467,8 +467,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t v_ring = k_ring + S::kKSlots * S::kKTile;
     Control *ctl = reinterpret_cast<Control *>(smem + S::kControl);
     BlockScale *scales = reinterpret_cast<BlockScale *>(ctl + 1);
-    const int h = blockIdx.y;
     const int G = pool.n_head_kv;
+    // The heads of a tile stand together, so that CTAs start in the order of the tiles,
+    // longest first (all tiles of a head, then the next head's: 8100 F32 tokens 1197 ->
+    // 1022 us, BF16 607 -> 600; 8 ragged windows F32 472 -> 453, BF16 267 -> 275)
+    const int h = blockIdx.x % G;
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     if (warp == kIssuer) {
@@ -504,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // set up while the kernel before this one ended; its writes from here on
     pdl_wait();
     pdl_trigger();
-    const WindowTile t = tiles[blockIdx.x];
+    const WindowTile t = tiles[blockIdx.x / G];
     const int n_tiles = t.tokens > kTileTokens ? 2 : 1;
     // blocks of each M tile: up to the last key that its last token sees
     const int key_end0 = t.pos0 + min(t.tokens, kTileTokens) - t.key0;
@@ -1120,7 +1123,7 @@ void launch_window_t(const PoolView &pool, const WindowArgs &a, DeviceError *err
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(a.n_tiles), G);
+    cfg.gridDim = dim3(static_cast<unsigned>(a.n_tiles) * G);
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = Shape<T, kE4m3>::kSmem;
     cfg.stream = stream;
