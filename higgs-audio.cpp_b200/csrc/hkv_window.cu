@@ -29,9 +29,9 @@
 //
 // What bounds it: the chain S, softmax, P, O of a block, which the two tiles of a CTA
 // take in turns; tensor pipe, exponentials and issue slots are each under half.  8 KV
-// heads, 8-bit cache: a BF16 prompt of 8100 608-640 us (0.54-0.52 of the measured bf16
-// rate); 8 F32 windows of 4-1024 behind 584-4000 473 us (0.50 of the rate for the
-// doubled products; the softmax's longer chain and the moves of o weigh most); 37 behind
+// heads, 8-bit cache: a BF16 prompt of 8100 595-640 us by its data (0.56-0.52 of the
+// measured bf16 rate); 8 F32 windows of 4-1024 behind 584-4000 461 us (0.51 of the rate
+// for the doubled products; the softmax's longer chain and the moves of o weigh most); 37 behind
 // 770 16.5 us (launch, one block's chain, the join).
 //
 // The rescaling of o when the bound m moves is put off until a row passes it by
@@ -85,8 +85,8 @@ constexpr int kShift = 7;               // weights enter 2^7 larger: at most 2^1
 // the part) and is added there in F32.  The tensor cores cut their sums instead of
 // rounding them: each of a block's 16 products takes about 2^-24 of o away, always
 // towards zero, 1e-5 of it over 4000 keys.  Eight ragged windows (1024 keys on average
-// behind 2034): error 5.7e-6 and 410 us without, 2.5e-6 and 445 us every 8 blocks,
-// 1.5e-6 and 473 us every 4 (some 40 us more with sums read back and rescaled each time).
+// behind 2034): error 5.7e-6 and 390 us without, 2.5e-6 and 430 us every 8 blocks,
+// 1.5e-6 and 461 us every 4 (some 40 us more with sums read back and rescaled each time).
 constexpr int kDrainBlocks = 4;
 constexpr int kFar = 60;                // V exponents this far below E take the slow form
 
