@@ -109,12 +109,15 @@ struct Control {
     uint64_t drained[2];        // after a wait that ran out: no product in flight
     uint32_t tmem;
     int odd_v;                  // a V value that is not finite was met
-    union {
-        int q_exp[2][kTile];          // of a row of q in E4M3 parts
-        float half[2][2][kTile];      // of a row's logits the largest, by each of its threads; l at the end
-    };
+    // One region per M tile: the tiles go through their blocks without a barrier between
+    // them, so what a tile writes must not lie over what the other may still read.
+    union TileRows {
+        int q_exp[kTile];             // of a row of q in E4M3 parts
+        float half[2][kTile];         // of a row's logits the largest, by each of its threads; l at the end
+    } rows[2];
 };
 static_assert(sizeof(Control) % 16 == 0, "the scales follow it");
+static_assert(sizeof(Control::TileRows) == 2 * kTile * sizeof(float), "a tile's exponents lie over its own halves");
 
 template <typename T, bool kE4m3>
 struct Shape {
@@ -567,7 +570,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 const int e = block_exponent(amax);
                 if (c == 0) {
-                    ctl->q_exp[i][r] = e;
+                    ctl->rows[i].q_exp[r] = e;
                 }
                 const float inv = pow2(-e);
                 uint32_t hi[2], lo[2];
@@ -603,7 +606,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         float q_scale = 1.f;
         if (S::kCodeK) {
             tile_barrier(i);  // q_exp of the tile's rows
-            q_scale = pow2(ctl->q_exp[i][row]);
+            q_scale = pow2(ctl->rows[i].q_exp[row]);
             tile_barrier(i);  // before `half` takes its place
         }
 
@@ -661,9 +664,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             e_v = b.e;
             const bool far = kE4m3 && b.far != 0;
             // the row's maximum over both halves
-            ctl->half[i][half][row] = mx;
+            ctl->rows[i].half[half][row] = mx;
             pair_barrier(warp);
-            mx = fmaxf(mx, ctl->half[i][half ^ 1][row]);
+            mx = fmaxf(mx, ctl->rows[i].half[half ^ 1][row]);
             const bool drain = S::kSplit && j > 0 && j % kDrainBlocks == 0;
             if (drain) {
                 // brought to the sums' units, where those are not too far (2^60 leaves a
@@ -796,9 +799,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         // the row's sum over both halves (bounds are the same)
         if (blocks > 0) {
-            ctl->half[i][half][row] = l;
+            ctl->rows[i].half[half][row] = l;
             pair_barrier(warp);
-            l += ctl->half[i][half ^ 1][row];
+            l += ctl->rows[i].half[half ^ 1][row];
         }
         if (ok) {
             tc_fence_after();
