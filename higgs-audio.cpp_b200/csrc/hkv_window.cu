@@ -266,8 +266,8 @@ __device__ __forceinline__ float4 load_at(const float *p) {
     return __ldcg(reinterpret_cast<const float4 *>(p));
 }
 
-// A wait of one role.  One that runs out is recorded and ends its role; the waits
-// that depend on it run out in turn, and the CTA leaves.
+// A wait of one role.  One that runs out is recorded and ends its role (a softmax warp
+// still goes to its barriers); the waits that depend on it run out in turn, and the CTA leaves.
 // The threads sleep in try_wait (20 us at a time), so that they leave the issue
 // slots to the warps that work.
 __device__ __forceinline__ bool try_wait_long(uint32_t bar, uint32_t parity) {
@@ -628,9 +628,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool keeps = t.part >= 0 || live;
         float kept = 0.f;
         for (int j = 0; j < blocks; ++j) {
-            if (!__all_sync(0xffffffffu, wait_for(&ctl->s_full[i], j & 1, err))) {
-                ok = false;
-                break;
+            // The two warps of a row pair find out on their own that a wait ran out, at
+            // different blocks perhaps.  One that did goes through the barriers that are
+            // left, so that its partner meets it at each: one per block and one at the end.
+            ok = ok && __all_sync(0xffffffffu, wait_for(&ctl->s_full[i], j & 1, err));
+            if (!ok) {
+                pair_barrier(warp);
+                continue;
             }
             tc_fence_after();
             const BlockScale &b = scales[j % S::kScaleSlots];
