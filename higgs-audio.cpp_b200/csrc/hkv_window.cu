@@ -616,7 +616,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int blocks = i == 0 ? nb0 : nb1;
         float m = -INFINITY, l = 0.f;
         int e_v = 0;
-        bool ok = true;
         const bool live = my_tok < t.tokens;
         // the token's four rows, from this lane's dims on
         const int my_dim = 64 * half + 4 * (lane & 3);
@@ -627,14 +626,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         float *sums = t.part >= 0 ? part_rows : reinterpret_cast<float *>(dst);
         const bool keeps = t.part >= 0 || live;
         float kept = 0.f;
-        for (int j = 0; j < blocks; ++j) {
-            // The two warps of a row pair find out on their own that a wait ran out, at
-            // different blocks perhaps.  One that did goes through the barriers that are
-            // left, so that its partner meets it at each: one per block and one at the end.
-            ok = ok && __all_sync(0xffffffffu, wait_for(&ctl->s_full[i], j & 1, err));
-            if (!ok) {
-                pair_barrier(warp);
-                continue;
+        int j = 0;
+        for (; j < blocks; ++j) {
+            if (!__all_sync(0xffffffffu, wait_for(&ctl->s_full[i], j & 1, err))) {
+                break;
             }
             tc_fence_after();
             const BlockScale &b = scales[j % S::kScaleSlots];
@@ -797,6 +792,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                     mbar_arrive(smem_u32(&ctl->p_full[i][c]));
                 }
             }
+        }
+        // The two warps of a row pair find out on their own that a wait ran out, at different
+        // blocks perhaps.  One that did goes to the barriers that are left, so that its
+        // partner meets it at each: one per block and one at the end.
+        bool ok = j == blocks;
+        for (; j < blocks; ++j) {
+            pair_barrier(warp);
         }
         if (ok && blocks > 0) {
             ok = __all_sync(0xffffffffu, wait_for(&ctl->o_full[i], 0, err));
