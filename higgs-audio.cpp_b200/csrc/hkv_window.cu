@@ -88,6 +88,10 @@ constexpr int kShift = 7;               // weights enter 2^7 larger: at most 2^1
 // behind 2034): error 5.7e-6 and 390 us without, 2.5e-6 and 430 us every 8 blocks,
 // 1.5e-6 and 461 us every 4 (some 40 us more with sums read back and rescaled each time).
 constexpr int kDrainBlocks = 4;
+// The least exponent of a row of q in E4M3 parts: with K's least, -100, the factor of a
+// logit stays a normal float, as masked logits (-inf) need it.  Smaller rows round to
+// multiples of 2^-30, F16 ones to 2^-25.
+constexpr int kQExpMin = -20;
 constexpr int kFar = 60;                // V exponents this far below E take the slow form
 
 // What the softmax needs of a block's pages.
@@ -568,7 +572,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int off = 8; off > 0; off >>= 1) {
                     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
                 }
-                const int e = block_exponent(amax);
+                const int e = max(block_exponent(amax), kQExpMin);
                 if (c == 0) {
                     ctl->rows[i].q_exp[r] = e;
                 }

@@ -289,7 +289,7 @@ int hkv_qkv_write(hkv_engine *eng, const hkv_qkv_write_args *args, hkv_stream st
  * products in two F16 parts (22 bits, as in hkv_decode_attn), with F16 or BF16 ones q
  * as it is and the weights rounded to F16; |q| up to 65504, and to 2^-25 below 2^-14
  * (BF16 on an 8-bit cache instead: values below 2^-9 of their row's largest are off by
- * up to 2^-17 of that).
+ * up to 2^-17 of that, and all values by up to 2^-30).
  * A value that is not finite reaches the rows that see it and no other. */
 typedef struct hkv_window_attn_args {
     int32_t layer;
