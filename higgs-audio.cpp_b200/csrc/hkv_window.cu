@@ -1,11 +1,13 @@
 // hkv_window.cu -- attention of several new tokens per slot over the paged cache
 // (prompts, refreshed windows): row i of a slot sees rows [0, used + i].
 //
-//   s_t = (q . c_t) 2^eK scale log2(e),  w_t = 2^(s_t - m),
-//   o   = sum_t w_t 2^(eV - E) c_t,      out = o 2^E / sum_t w_t
+//   s_t = (q . c_t) 2^eK scale log2(e),  w_t = 2^(s_t + eV - m),
+//   o   = sum_t w_t c_t,                 out = o / sum_t w_t 2^-eV
 //
-// with codes c (F16 values in an F16 cache: eK = eV = 0), m a running bound of
-// the logits and E the largest eV so far; one pass over the keys.
+// with codes c (F16 values in an F16 cache: eK = eV = 0) and m the row's running bound
+// of s_t + eV over the keys that it sees; one pass over them.  V's exponent belongs to
+// the weight: a row's weights are then at most 1 whatever the exponents are, and keep
+// their bits by what a key adds to the row's output, its V as well as its logit.
 //
 // One CTA takes up to 64 tokens x the 4 query heads of a KV head, as two M = 128
 // tiles (row = 4 token + head), so that a key is read and converted once for 256
@@ -88,21 +90,25 @@ constexpr int kShift = 7;               // weights enter 2^7 larger: at most 2^1
 // behind 2034): error 5.7e-6 and 390 us without, 2.5e-6 and 430 us every 8 blocks,
 // 1.5e-6 and 461 us every 4 (some 40 us more with sums read back and rescaled each time).
 constexpr int kDrainBlocks = 4;
+// V exponents this far below the largest so far: a weight of such a page may underflow in
+// F32 though its key weighs, so the sum of the weights is formed apart.  At less, terms
+// down to 2^-50 of a row's largest enter it.
+constexpr int kFar = 80;
 // The least exponent of a row of q in E4M3 parts: with K's least, -100, the factor of a
 // logit stays a normal float, as masked logits (-inf) need it.  Smaller rows round to
 // multiples of 2^-30, F16 ones to 2^-25.
 constexpr int kQExpMin = -20;
-constexpr int kFar = 60;                // V exponents this far below E take the slow form
 
-// What the softmax needs of a block's pages.
+// What the softmax needs of a page.
+struct alignas(16) PageScale {
+    float k;      // scale * log2(e) * 2^eK
+    float v_exp;  // eV
+    float shift;  // of the weights' exponent: kShift + eV
+    float back;   // 2^-(kShift + eV): from weights to terms of the sum; 0 in a far block
+};
 struct BlockScale {
-    float k_scale[kBlockPages];  // scale * log2(e) * 2^eK
-    float shift[kBlockPages];    // of the exponent: kShift + eV - E
-    float back[kBlockPages];     // 2^(E - eV): takes eV - E out of the sum of the weights again
-    float grow;                  // 2^(E before - E)
-    int e;                       // E: the largest eV of the CTA's blocks so far
-    int far;                     // some eV - E < -kFar: shift is kShift, the weights times 1 / back
-    int unused;
+    PageScale page[kBlockPages];
+    int far;      // some eV is more than kFar below the largest so far
 };
 
 struct Control {
@@ -619,7 +625,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int first_last = t.pos0 + i * kTileTokens - t.key0;         // and the tile's first row
         const int blocks = i == 0 ? nb0 : nb1;
         float m = -INFINITY, l = 0.f;
-        int e_v = 0;
+        // what a page's products are multiplied by (finite: 0 * inf would be no logit)
+        auto logit_scale = [&](const PageScale &page) {
+            return S::kCodeK ? fminf(page.k * q_scale, 3.402823466e38f) : page.k;
+        };
         const bool live = my_tok < t.tokens;
         // the token's four rows, from this lane's dims on
         const int my_dim = 64 * half + 4 * (lane & 3);
@@ -659,22 +668,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                         d = max3(d, s[16 * p + k + 2], s[16 * p + k + 3]);
                     }
                     a = max3(a, s[16 * p + 14], s[16 * p + 15]);
-                    mx = fmaxf(mx, fmaxf(a, d) * b.k_scale[4 * half + 2 * c + p]);
+                    const PageScale page = b.page[4 * half + 2 * c + p];
+                    mx = fmaxf(mx, fmaf(fmaxf(a, d), logit_scale(page), kE4m3 ? page.v_exp : 0.f));
                 }
             }
-            mx *= q_scale;
-            const float grow = b.grow;
-            e_v = b.e;
-            const bool far = kE4m3 && b.far != 0;
-            // the row's maximum over both halves
+            // the row's bound over both halves
             ctl->rows[i].half[half][row] = mx;
             pair_barrier(warp);
             mx = fmaxf(mx, ctl->rows[i].half[half ^ 1][row]);
             const bool drain = S::kSplit && j > 0 && j % kDrainBlocks == 0;
             if (drain) {
                 // brought to the sums' units, where those are not too far (2^60 leaves a
-                // sum of 2^15 weights of 2^15 and V below 2^126), for an addition in L2
-                // that nothing waits for
+                // sum of 2^9 weights of 2^15 and V of 2^16 below 2^100), for an addition in
+                // L2 that nothing waits for
                 const bool first = j == kDrainBlocks;
                 const bool in_place = !first && __all_sync(0xffffffffu, kept >= 0x1p-60f);
                 const float4 scale = of_rows(in_place ? 1.f / kept : kept, lane);
@@ -704,14 +710,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 kept = in_place ? kept : 1.f;
             }
-            // the bound and E move (o has to follow) only when they must
-            if (__any_sync(0xffffffffu, mx > m + kSlack || grow < 1.f)) {
+            // the bound moves (o has to follow) only when it must
+            if (__any_sync(0xffffffffu, mx > m + kSlack)) {
                 const float m_new = fmaxf(m, mx);
                 const float corr = (m_new == -INFINITY ? 1.f : exp2_fast(m - m_new));
-                const float o_corr = corr * grow;
                 m = m_new;
                 l *= corr;
-                kept *= o_corr;
+                kept *= corr;
                 if (j > 0 && !drain) {
 #pragma unroll 1
                     for (int c = 0; c < 64; c += 16) {
@@ -719,13 +724,42 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tmem_load16(o_col + c, o);
 #pragma unroll
                         for (int k = 0; k < 16; ++k) {
-                            o[k] *= o_corr;
+                            o[k] *= corr;
                         }
                         tmem_store16(o_col + c, reinterpret_cast<const uint32_t (&)[16]>(o));
                     }
                 }
             }
             const float bound = m == -INFINITY ? 0.f : m;
+            const bool far = kE4m3 && b.far != 0;
+            if (far) {
+#pragma unroll 1
+                for (int p = 0; p < 4; ++p) {
+                    const PageScale page = b.page[4 * half + p];
+                    const float sc = logit_scale(page);
+                    float s[16];
+                    tmem_load16(s_col + 16 * p, s);
+                    float r = -INFINITY;
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        s[k] = 16 * p + k <= lim ? s[k] : -INFINITY;
+                        r = fmaxf(r, s[k] * sc);
+                    }
+                    if (far) {
+                        // V exponents far apart (`back` is 0): the page's terms of the sum by
+                        // its own largest logit, and from there to the sum's units in two
+                        // steps that do not underflow
+                        const float top = r == -INFINITY ? 0.f : r;
+                        float terms = 0.f;
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            terms += exp2_fast(__fmul_rn(s[k], sc) - top);
+                        }
+                        const float h = exp2_fast(0.5f * (r - bound));
+                        l = fmaf(terms * h, h, l);
+                    }
+                }
+            }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 float s[32];
@@ -739,15 +773,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 uint32_t hi[16], lo[16];
 #pragma unroll
                 for (int p = 0; p < 2; ++p) {
-                    // 2^(eV - E) belongs to the weight and not to l: in the exponent, and
-                    // taken out of the page's sum again; where that could underflow
-                    // (V pages 2^60 apart), by a product instead
-                    const int page = 4 * half + 2 * c + p;
-                    const float sc = b.k_scale[page] * q_scale;
-                    const float sh = b.shift[page] - bound;
-                    const float back = b.back[page];
-                    const float2 scale = make_float2(sc, sc), off = make_float2(sh, sh);
+                    const PageScale page = b.page[4 * half + 2 * c + p];
+                    const float sc = logit_scale(page);
+                    const float sh = page.shift - bound;
                     float2 *x = reinterpret_cast<float2 *>(s + 16 * p);
+                    const float2 scale = make_float2(sc, sc), off = make_float2(sh, sh);
                     float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
@@ -755,15 +785,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                         x[k] = make_float2(exp2_fast(e.x), exp2_fast(e.y));
                         sum = add2(sum, x[k]);
                     }
-                    if (far) {
-                        const float w = 1.f / back;
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            x[k] = make_float2(x[k].x * w, x[k].y * w);
-                        }
-                        l += sum.x + sum.y;
+                    if (!kE4m3) {
+                        l += sum.x + sum.y;  // with the 2^kShift of o
                     } else {
-                        l = fmaf(sum.x + sum.y, back, l);
+                        l = fmaf(sum.x + sum.y, page.back, l);
                     }
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
@@ -816,8 +841,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (ok) {
             tc_fence_after();
             const bool odd = *reinterpret_cast<volatile int *>(&ctl->odd_v) != 0;
-            // a part's o is not normalised; o carries 2^kShift as l does
-            const float4 f = of_rows(pow2(max(e_v, -126)) * (t.part < 0 ? 1.f / l : 1.f), lane);
+            // F16 cache: o and l carry 2^kShift, a part's o is not normalised.  8-bit cache:
+            // o carries it, and a part's o and l are brought to l in [1, 2) by a power of
+            // two that m takes up, so that o is of the size of V and its weight in the
+            // join that of its logits.
+            float own = t.part < 0 ? 1.f / l : 1.f;
+            if (kE4m3 && t.part >= 0) {
+                const int e = min(max(static_cast<int>((__float_as_uint(l) >> 23) & 255u) - 127 + 12, -126), 126);
+                own = pow2(-e);
+                l *= own;
+                m += static_cast<float>(e);
+            }
+            constexpr float kUnit = kE4m3 ? 1.f / (1 << kShift) : 1.f;
+            const float4 f = of_rows(own, lane);
             const float4 scale = of_rows(kept, lane);
 #pragma unroll 1
             for (int c = 0; c < 64; c += 16) {
@@ -833,7 +869,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        o[4 * r + k] = blocks > 0 ? o[4 * r + k] * row_of(f, r) : 0.f;
+                        o[4 * r + k] = blocks > 0 ? o[4 * r + k] * kUnit * row_of(f, r) : 0.f;
                     }
                 }
                 if (odd && live) {
@@ -999,7 +1035,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         } else if (warp == kScaleWarp) {
             // ------------------------------------------- exponents, and K's codes
-            int e = INT32_MIN;  // E
+            int e = INT32_MIN;  // the largest V exponent so far
             bool ok = true;
             for (int j = 0; ok && j < nb; ++j) {
                 const int slot = j % S::kKSlots;
@@ -1034,21 +1070,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int off = 4; off > 0; off >>= 1) {
                     top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
                 }
-                const int e_new = max(e, top);
-                const int d = there ? exps.y - e_new : 0;
-                const bool far = __any_sync(0xffffffffu, d < -kFar);
+                e = max(e, top);
+                const int e_v = there ? exps.y : 0;
+                const bool far = __any_sync(0xffffffffu, there && e_v < e - kFar);
                 BlockScale &b = scales[j % S::kScaleSlots];
                 if (lane < kBlockPages) {
-                    b.k_scale[lane] = scale_log2 * pow2(exps.x);
-                    b.shift[lane] = static_cast<float>(kShift + (far ? 0 : d));
-                    b.back[lane] = pow2(min(-d, 126));
+                    b.page[lane] = {scale_log2 * pow2(exps.x), static_cast<float>(e_v), static_cast<float>(kShift + e_v),
+                                    far ? 0.f : ldexpf(1.f, -(kShift + e_v))};
                 }
                 if (lane == 0) {
-                    b.grow = j == 0 ? 1.f : pow2(max(e - e_new, -126));
-                    b.e = e_new;
                     b.far = far ? 1 : 0;
                 }
-                e = e_new;
                 __syncwarp();
                 if (lane == 0) {
                     mbar_arrive(bar);

@@ -290,6 +290,8 @@ int hkv_qkv_write(hkv_engine *eng, const hkv_qkv_write_args *args, hkv_stream st
  * as it is and the weights rounded to F16; |q| up to 65504, and to 2^-25 below 2^-14
  * (BF16 on an 8-bit cache instead: values below 2^-9 of their row's largest are off by
  * up to 2^-17 of that, and all values by up to 2^-30).
+ * On an 8-bit cache a weight p_t of a key whose V has the exponent e_t is held so to
+ * 2^-32 of the row's largest p_t 2^e_t, over the keys that the row sees, and no finer.
  * A value that is not finite reaches the rows that see it and no other. */
 typedef struct hkv_window_attn_args {
     int32_t layer;

@@ -40,6 +40,49 @@ def test_rows_of_different_scales(hkv_lib, cache, name):
     eng.close()
 
 
+def cached(eng, hkv, slot, n, G, layer=0):
+    """Rows [0, n) of a slot as float64."""
+    k, v = torch.empty((2, n, G, D), device=DEV).unbind(0)
+    eng.cache_read(layer, [slot], [0], [n], k, v, dtype=hkv.F32)
+    torch.cuda.synchronize()
+    return k.double().cpu().numpy(), v.double().cpu().numpy()
+
+
+def weighed(q, k, v, first, dtype, spare):
+    """Float64 attention of rows q [T][H][D] over the rows k, v [L][G][D] and, for each output, a bound that
+    goes by what the row weighs, not by the largest V of the slot.
+
+    A weight is off relative to itself as attention_tolerance() derives (big: the largest sum_d |q_d k_d| * scale
+    of the row), so an output by twice that times sum_t p_t |V_t| of its dim; F32 sums add 2^-23 of that for
+    each 16 rows.  F16 and BF16 tensors round weights to F16: 2^-11 more.  Weights are held in F16 in
+    units in which the largest p_t 2^eV of the row is at least 2^spare, to 2^-25 (half the least F16): each key
+    adds up to 2^-(25 + spare) max_t(p_t 448 2^eV), and 448 * 2^eV is under twice the largest |V| of its page."""
+    T, H, _ = q.shape
+    L, G, _ = k.shape
+    page = np.zeros((L, G))
+    for p in range(0, L, 16):
+        page[p:p + 16] = 2 * np.abs(v[p:p + 16]).max((0, 2))
+    out, bound = np.zeros((T, H, D)), np.zeros((T, H, D))
+    for h in range(H):
+        g = h // (H // G)
+        for i in range(T):
+            n = first + i + 1
+            s = k[:n, g] @ q[i, h] / np.sqrt(float(D))
+            big = float((np.abs(k[:n, g]) @ np.abs(q[i, h])).max()) / np.sqrt(float(D))
+            p = np.exp(s - s.max())
+            p /= p.sum()
+            out[i, h] = p @ v[:n, g]
+            rel = 2 * (big * (2.0 ** -22 + 2.0 ** -19) + 2 * big * 2.0 ** -23 + 2.0 ** -21 + 2.0 ** -22)
+            if dtype != "f32":
+                rel += 2 * 2.0 ** -11
+            if dtype == "bf16":  # q in two E4M3 parts: 2^-10 / 224 of the row's largest a dim
+                rel += 2 * np.abs(q[i, h]).max() * 2.0 ** -10 / 224 * np.abs(k[:n, g]).sum(-1).max() / np.sqrt(float(D))
+            size = p @ np.abs(v[:n, g])
+            bound[i, h] = size * (rel + (n / 16 + 64) * 2.0 ** -23) + n * 2.0 ** -(25 + spare) * (p * page[:n, g]).max()
+    half = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}[dtype]
+    return out, bound + half * (np.abs(out) + bound) + (2.0 ** -25 if dtype == "f16" else 0.0)
+
+
 @pytest.mark.parametrize("cache", ["e4m3", "f16"])
 @pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
 def test_zero_rows_give_the_mean(hkv_lib, cache, name):
@@ -86,4 +129,65 @@ def test_zero_rows_among_others(hkv_lib):
     q[::3] = 0
     q = torch.from_numpy(q).to(DEV)
     check(eng, hkv, [s], [n], q, window(eng, hkv, [s], [n], q, "bf16"), "bf16")
+    eng.close()
+
+
+STEPS = [(12, 1), (24, 1), (40, 1), (70, 1), (-24, 1), (-70, 1), (24, 0), (-40, 0), (105, 0)]
+
+
+def far_pages(rng, n, G, step, zero):
+    """V pages whose sizes alternate 2^step apart, with pages of zeros between them where `zero` is 0."""
+    v = rows(rng, n, G).astype(np.float64)
+    for p in range((n + 15) // 16):
+        v[16 * p:16 * p + 16] *= 2.0 ** (step if p % 2 else 0) if zero or p % 3 else 0.0
+    return v.astype(np.float32)
+
+
+@pytest.mark.parametrize("step,zero", STEPS)
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+def test_window_goes_by_the_v_it_sees(hkv_lib, name, step, zero):
+    """V pages far apart in one tile: a row before a page of large V does not know of it, and a page that
+    weighs nothing takes no bits from one that does.  Split (one slot) and whole tiles (16 slots of 8 heads)."""
+    import hkv
+    if name == "f16" and step > 12:
+        step = 12  # its outputs end at 65504
+    rng = np.random.default_rng(91)
+    for G, count in ((1, 1), (8, 16)):
+        eng = engine(hkv, G, "e4m3", max_slots=count)
+        n = 150
+        slots = [eng.acquire() for _ in range(count)]
+        for i, s in enumerate(slots):
+            k = rows(rng, n, G)
+            if i % 2 == 0 and step > 0:
+                k[16:32] -= 4  # every second page weighs less, one far less, than its V is large
+            eng.rope_append_range(0, s, n, dev(k), dev(far_pages(rng, n, G, step, zero)))
+        q = torch.from_numpy((rng.standard_normal((count * n, 4 * G, D)) + 0.5).astype(np.float32)).to(DEV)
+        out = window(eng, hkv, slots, [n] * count, q, name).double().cpu().numpy().reshape(count, n, 4 * G, D)
+        x = q.to(DT[name]).double().cpu().numpy().reshape(count, n, 4 * G, D)
+        for i in range(0, count, 5):
+            k, v = cached(eng, hkv, slots[i], n, G)
+            h = slice(0, 4) if i % 2 else slice(4 * G - 4, 4 * G)
+            g = slice(h.start // 4, h.start // 4 + 1)
+            want, bound = weighed(x[i][:, h], k[:, g], v[:, g], 0, name, 7)
+            over = np.abs(out[i][:, h] - want) - bound
+            assert over.max() <= 0, (G, i, np.unravel_index(over.argmax(), over.shape), over.max())
+        eng.close()
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+def test_window_of_values_near_the_largest_floats(hkv_lib, name):
+    """V of up to 3e38 over 1,000 rows, split and joined: a mean, not infinity."""
+    import hkv
+    rng = np.random.default_rng(93)
+    eng = engine(hkv, 1, "e4m3")
+    s = eng.acquire()
+    n = 1000
+    v = (rng.uniform(1.0, 3.0, (n, 1, D)) * 1e38).astype(np.float32)
+    eng.rope_append_range(0, s, n, dev(rows(rng, n, 1)), dev(v))
+    eng.advance([s], 990)
+    q = torch.from_numpy(rng.standard_normal((10, 4, D)).astype(np.float32)).to(DEV)
+    out = window(eng, hkv, [s], [10], q, name).double().cpu().numpy().reshape(10, 4, D)
+    k, v = cached(eng, hkv, s, n, 1)
+    want, bound = weighed(q.to(DT[name]).double().cpu().numpy(), k, v, 990, name, 7)
+    assert (np.abs(out - want) <= bound).all()
     eng.close()
