@@ -82,6 +82,10 @@ constexpr int kSoftmaxRegs = 88;
 constexpr int kOtherRegs = 64;
 static_assert(4 * kSoftmaxRegs + 2 * kOtherRegs == 6 * 80, "the shares add up to the launch's registers");
 constexpr float kSlack = 8.f;
+// A bound is the rounded largest logit: beyond this size it may lie so far from the exact
+// one that a weight leaves F16.  There the logits are rounded before the bound is
+// subtracted, as a plain F32 softmax rounds them.
+constexpr float kHuge = 1 << 23;
 constexpr int kShift = 7;               // weights enter 2^7 larger: at most 2^15 in F16
 // F32 tensors: blocks after which o moves from TMEM to the row's place in `out` (or in
 // the part) and is added there in F32.  The tensor cores cut their sums instead of
@@ -625,6 +629,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int first_last = t.pos0 + i * kTileTokens - t.key0;         // and the tile's first row
         const int blocks = i == 0 ? nb0 : nb1;
         float m = -INFINITY, l = 0.f;
+        bool huge = false;  // of a row of the warp
         // what a page's products are multiplied by (finite: 0 * inf would be no logit)
         auto logit_scale = [&](const PageScale &page) {
             return S::kCodeK ? fminf(page.k * q_scale, 3.402823466e38f) : page.k;
@@ -717,6 +722,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 m = m_new;
                 l *= corr;
                 kept *= corr;
+                huge = __any_sync(0xffffffffu, fabsf(m) > kHuge && m != -INFINITY);
                 if (j > 0 && !drain) {
 #pragma unroll 1
                     for (int c = 0; c < 64; c += 16) {
@@ -732,7 +738,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             const float bound = m == -INFINITY ? 0.f : m;
             const bool far = kE4m3 && b.far != 0;
-            if (far) {
+            if (far || huge) {
 #pragma unroll 1
                 for (int p = 0; p < 4; ++p) {
                     const PageScale page = b.page[4 * half + p];
@@ -758,7 +764,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const float h = exp2_fast(0.5f * (r - bound));
                         l = fmaf(terms * h, h, l);
                     }
+                    if (huge) {
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            s[k] = fmaf(s[k], sc, kE4m3 ? page.v_exp : 0.f) - bound;
+                        }
+                        tmem_store16(s_col + 16 * p, reinterpret_cast<const uint32_t (&)[16]>(s));
+                    }
                 }
+                tmem_store_wait();
             }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -774,8 +788,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int p = 0; p < 2; ++p) {
                     const PageScale page = b.page[4 * half + 2 * c + p];
-                    const float sc = logit_scale(page);
-                    const float sh = page.shift - bound;
+                    const float sc = huge ? 1.f : logit_scale(page);
+                    const float sh = huge ? static_cast<float>(kShift) : page.shift - bound;
                     float2 *x = reinterpret_cast<float2 *>(s + 16 * p);
                     const float2 scale = make_float2(sc, sc), off = make_float2(sh, sh);
                     float2 sum = make_float2(0.f, 0.f);

@@ -132,6 +132,33 @@ def test_zero_rows_among_others(hkv_lib):
     eng.close()
 
 
+def test_logits_near_the_largest_floats(hkv_lib):
+    """BF16 on an 8-bit cache: K of 1e37 against q of 0.01, logits of up to 1e35, each row one key's V; a
+    product of codes and one exponent alone would overflow."""
+    import hkv
+    rng = np.random.default_rng(89)
+    G, n = 1, 100
+    eng = engine(hkv, G, "e4m3")
+    s = eng.acquire()
+    eng.rope_append_range(0, s, n, dev(rows(rng, n, G) * 1e36), dev(rows(rng, n, G)))
+    q = torch.from_numpy((rng.standard_normal((n, 4 * G, D)) * 0.01).astype(np.float32)).to(DEV)
+    out = window(eng, hkv, [s], [n], q, "bf16").double().cpu().numpy().reshape(n, 4, D)
+    k, v = cached(eng, hkv, s, n, G)
+    x = q.bfloat16().double().cpu().numpy()
+    sure = 0
+    for i in range(n):
+        for h in range(4):
+            a = np.sort(k[:i + 1, 0] @ x[i, h])[::-1]
+            # q is held to 2^-17 of its largest value in each dim
+            slack = 2.0 ** -17 * np.abs(x[i, h]).max() * np.abs(k[:i + 1, 0]).sum(-1).max() * 2
+            if len(a) == 1 or a[0] - a[1] > 4 * slack:
+                want = v[np.argmax(k[:i + 1, 0] @ x[i, h]), 0]
+                assert (np.abs(out[i, h] - want) <= 2.0 ** -8 * np.abs(want)).all(), (i, h)
+                sure += 1
+    assert sure > 300
+    eng.close()
+
+
 STEPS = [(12, 1), (24, 1), (40, 1), (70, 1), (-24, 1), (-70, 1), (24, 0), (-40, 0), (105, 0)]
 
 
@@ -190,4 +217,43 @@ def test_window_of_values_near_the_largest_floats(hkv_lib, name):
     k, v = cached(eng, hkv, s, n, 1)
     want, bound = weighed(q.to(DT[name]).double().cpu().numpy(), k, v, 990, name, 7)
     assert (np.abs(out - want) <= bound).all()
+    eng.close()
+
+
+@pytest.mark.parametrize("cache", ["e4m3", "f16"])
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16"])
+def test_large_logits(hkv_lib, cache, name):
+    """q and K of some 10^4: logits of up to 10^10, apart by far more than one, so that each row is the V of
+    one key, whatever its place; and all of them below -2^24 for the keys of one slot."""
+    import hkv
+    rng = np.random.default_rng(95)
+    G, n = 2, 200
+    eng = engine(hkv, G, cache)
+    q = rng.standard_normal((n, 4 * G, D)).astype(np.float32) * 8000
+    for sign in (0, -1):
+        s = eng.acquire()
+        k = rows(rng, n, G, 0.0) * np.float32(8000)
+        if sign:
+            k = -np.abs(k)
+            q = np.abs(q)
+        eng.rope_append_range(0, s, n, dev(k), dev(rows(rng, n, G))) if not sign else \
+            eng.qkv_write(0, [s], [n], None, dev(k), dev(rows(rng, n, G)), rotated=True)
+        x = torch.from_numpy(q).to(DEV)
+        out = window(eng, hkv, [s], [n], x, name).double().cpu().numpy().reshape(n, 4 * G, D)
+        kk, vv = cached(eng, hkv, s, n, G)
+        x = x.to(DT[name]).double().cpu().numpy()
+        sure = 0
+        for i in range(n):
+            for h in range(4 * G):
+                logits = kk[:i + 1, h // 4] @ x[i, h] / np.sqrt(float(D))
+                a = np.sort(logits)[::-1]
+                # F32 sums of 128 products, q to 2^-17 of its largest value: far less than 2^-14 of sum |q k|
+                slack = 2.0 ** -14 * (np.abs(kk[:i + 1, h // 4]) @ np.abs(x[i, h])).max() / np.sqrt(float(D))
+                if len(a) == 1 or a[0] - a[1] > 2 * slack + 40:
+                    want = vv[np.argmax(logits), h // 4]
+                    tol = {"f32": 2.0 ** -20, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}[name]
+                    assert (np.abs(out[i, h] - want) <= tol * np.abs(want) + 2.0 ** -25).all(), (sign, i, h)
+                    sure += 1
+        assert sure > n * 4 * G // 2
+        eng.release(s)
     eng.close()
