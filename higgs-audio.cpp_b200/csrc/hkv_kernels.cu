@@ -67,7 +67,10 @@ constexpr int kCtaSmem = kAttnWarps * 2 * kCtaPartBytes + 32;
 // in the cluster's first CTA, then the mbarrier that counts the filled slots.
 constexpr int kMaxCluster = 16;
 constexpr int kClusterSmem = kMaxCluster * kCtaPartBytes + 16;
-constexpr int kPShift = 14;  // o's weights are p 2^14 in the 8-bit format: at most 16384 in F16
+constexpr int kPShift = 14;  // o's weights are 2^14 larger in the 8-bit format: at most 16384 in F16
+// V exponents this far below the share's largest so far (8-bit format): a weight may
+// underflow though its key weighs, so l's terms are formed apart.
+constexpr int kFarExp = 100;
 constexpr int kWhereAppend = 0;
 constexpr int kWhereAttn = 1;
 constexpr int kWhereGather = 3;
@@ -809,12 +812,13 @@ __device__ __forceinline__ void signal_arrival(const Exchange &x, int layer, int
 //
 // kE4m3: the 8-bit cache.  Codes become F16 in registers (exact) on their way
 // into the same MMAs, and both exponents stay out of the products:
-//   s_t = (q . c_t) 2^eK scale          one factor per page, on the logits
-//   o   = sum_t p_t 2^(eV - E) c_t      E: the largest eV of the share so far,
-// so the weights of the second product are at most 1 whatever the exponents
-// are, and o is scaled by 2^E when it leaves the registers.  The weights enter
-// 2^kPShift larger: their F16 parts then keep their bits for pages whose V is
-// far smaller than another page's.  l sums the unscaled p_t.
+//   s_t = (q . c_t) 2^eK scale,   w_t = 2^(s_t + eV - m),   o = sum_t w_t c_t,
+//   l   = sum_t w_t 2^-eV,        out = o / l
+// with m the running maximum of s_t + eV: the weights of the second product are at most
+// 1 whatever the exponents are, and a page of large V that weighs nothing takes no bits
+// from the others.  They enter 2^kPShift larger, since their two F16 parts end at 2^-24.
+// eV is taken relative to e0, the segment's first one held to -6 .. 0, so that s_t + eV is
+// rounded about where s_t is and 2^-eV stays a normal float.
 // The dims of a head are permuted so that a lane's codes are whole 16-byte
 // chunks and no ldmatrix is needed: lane (g, t) = (lane / 4, lane % 4) reads
 // dims 32t .. 32t + 31 of K rows g and g + 8 (the MMA's k index may be any
@@ -959,7 +963,7 @@ __global__ void __launch_bounds__(Ring<kE4m3, kCtaMerge>::kWarps * 32, 1)
     float4 acc[kGqa];
 #endif
     float m_a = kNegInf, m_b = kNegInf, l_a = 0.f, l_b = 0.f;
-    int e_v = 0;  // E: o is held in units of 2^(E - kPShift)
+    int e0 = 0, e_top = 0;  // 8-bit cache: the reference of V's exponents, and the largest so far
     int seg_e = 0, seg_h = 0, seg_pos = 0, part = 0, p_first = 0, nparts = 1, ntok = 0;
     int run_w0 = wid, run_m = 1;  // this CTA's warps of the current segment: w0 .. w0 + m - 1
 
@@ -987,23 +991,38 @@ __global__ void __launch_bounds__(Ring<kE4m3, kCtaMerge>::kWarps * 32, 1)
         }
         __syncwarp();
 #endif
-        const float o_scale = kE4m3 ? pow2(max(e_v - kPShift, -126)) : 1.f;
+        l_a += __shfl_xor_sync(0xffffffffu, l_a, 4);
+        l_b += __shfl_xor_sync(0xffffffffu, l_b, 4);
+        l_a += __shfl_xor_sync(0xffffffffu, l_a, 8);
+        l_b += __shfl_xor_sync(0xffffffffu, l_b, 8);
+        l_a += __shfl_xor_sync(0xffffffffu, l_a, 16);
+        l_b += __shfl_xor_sync(0xffffffffu, l_b, 16);
+        float unit = 1.f, own_a = 1.f, own_b = 1.f;
+        if (kE4m3) {
+            // l brought to [2^-12, 2^-11) by a power of two that m takes up: a partial's
+            // weight is then that of its logits, and no merge of 2^11 of them overflows
+            auto exponent = [](float l) {
+                return min(max(static_cast<int>((__float_as_uint(l) >> 23) & 255u) - 127 + 12, -126), 126);
+            };
+            const int ea = exponent(l_a), eb = exponent(l_b);
+            unit = pow2(e0 - kPShift);
+            own_a = pow2(-ea);
+            own_b = pow2(-eb);
+            l_a *= own_a;
+            l_b *= own_b;
+            m_a += static_cast<float>(ea);
+            m_b += static_cast<float>(eb);
+        }
 #pragma unroll
         for (int mt = 0; mt < 8; ++mt) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 o[mt][j] += __shfl_xor_sync(0xffffffffu, o[mt][j], 2);
                 if (kE4m3) {
-                    o[mt][j] *= o_scale;
+                    o[mt][j] = o[mt][j] * unit * (j & 1 ? own_b : own_a);
                 }
             }
         }
-        l_a += __shfl_xor_sync(0xffffffffu, l_a, 4);
-        l_a += __shfl_xor_sync(0xffffffffu, l_a, 8);
-        l_a += __shfl_xor_sync(0xffffffffu, l_a, 16);
-        l_b += __shfl_xor_sync(0xffffffffu, l_b, 4);
-        l_b += __shfl_xor_sync(0xffffffffu, l_b, 8);
-        l_b += __shfl_xor_sync(0xffffffffu, l_b, 16);
         const int ha = (lane & 1) * 2;
         const int d0 = lane >> 2;
         // the two dims whose sums o[mt] holds
@@ -1340,7 +1359,7 @@ __global__ void __launch_bounds__(Ring<kE4m3, kCtaMerge>::kWarps * 32, 1)
             }
             m_a = m_b = kNegInf;
             l_a = l_b = 0.f;
-            e_v = kExpMin;
+            e_top = INT32_MIN;
         }
 
         if constexpr (kE4m3) {
@@ -1398,6 +1417,7 @@ __global__ void __launch_bounds__(Ring<kE4m3, kCtaMerge>::kWarps * 32, 1)
             const int t = lane & 3;
             float sv[2][4];  // logits of rows g (heads a, b) and g + 8 of each page
             int ev[2];
+            float ef[2];     // eV - e0
             {
                 uint4 kx[2][2], ky[2][2];  // rows g and g + 8: the same swizzle
                 float s_scale[2];
@@ -1412,6 +1432,13 @@ __global__ void __launch_bounds__(Ring<kE4m3, kCtaMerge>::kWarps * 32, 1)
                     const int2 e = lds8(st[hh] + 2 * kCodeBlockBytes);
                     s_scale[hh] = scale_log2 * pow2(e.x);
                     ev[hh] = e.y;
+                }
+                if (e_top == INT32_MIN) {
+                    e0 = min(max(ev[0], -6), 0);
+                }
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {
+                    ef[hh] = static_cast<float>(ev[hh] - e0);
                 }
                 float sc[2][2][4] = {};
 #pragma unroll
@@ -1434,7 +1461,7 @@ __global__ void __launch_bounds__(Ring<kE4m3, kCtaMerge>::kWarps * 32, 1)
                     for (int j = 0; j < 4; ++j) {
                         float x = sc[hh][0][j] + sc[hh][1][j];
                         x += __shfl_xor_sync(0xffffffffu, x, 2);
-                        sv[hh][j] = hh < cnt && tok + (j >> 1) * 8 < ntok ? x * s_scale[hh] : kNegInf;
+                        sv[hh][j] = hh < cnt && tok + (j >> 1) * 8 < ntok ? fmaf(x, s_scale[hh], ef[hh]) : kNegInf;
                     }
                 }
             }
@@ -1457,13 +1484,11 @@ __global__ void __launch_bounds__(Ring<kE4m3, kCtaMerge>::kWarps * 32, 1)
             }
             const float mn_a = fmaxf(m_a, mx_a);
             const float mn_b = fmaxf(m_b, mx_b);
-            const int e_new = max(e_v, max(ev[0], ev[1]));
+            e_top = max(e_top, max(ev[0], ev[1]));
             const float alpha_a = exp2f(m_a - mn_a);
             const float alpha_b = exp2f(m_b - mn_b);
-            const float grow = pow2(max(e_v - e_new, -126));
             m_a = mn_a;
             m_b = mn_b;
-            e_v = e_new;
             float sum_a = 0.f, sum_b = 0.f;
             uint32_t pb[2][2];  // the weights as the second product's B fragments
 #pragma unroll
@@ -1473,12 +1498,12 @@ __global__ void __launch_bounds__(Ring<kE4m3, kCtaMerge>::kWarps * 32, 1)
                 p[1] = exp2f(sv[hh][1] - mn_b);
                 p[2] = exp2f(sv[hh][2] - mn_a);
                 p[3] = exp2f(sv[hh][3] - mn_b);
-                sum_a += p[0] + p[2];
-                sum_b += p[1] + p[3];
-                const float w = pow2(max(ev[hh] - e_new + kPShift, -126));
+                const float back = pow2(e0 - ev[hh]);
+                sum_a = fmaf(p[0] + p[2], back, sum_a);
+                sum_b = fmaf(p[1] + p[3], back, sum_b);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    p[j] *= w;
+                    p[j] *= static_cast<float>(1 << kPShift);
                 }
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
@@ -1486,14 +1511,12 @@ __global__ void __launch_bounds__(Ring<kE4m3, kCtaMerge>::kWarps * 32, 1)
                                                       : pack_half2(p[2 * j], p[2 * j + 1]));
                 }
             }
-            l_a = l_a * alpha_a + sum_a;
-            l_b = l_b * alpha_b + sum_b;
 #pragma unroll
             for (int mt = 0; mt < 8; ++mt) {
-                o[mt][0] *= alpha_a * grow;
-                o[mt][1] *= alpha_b * grow;
-                o[mt][2] *= alpha_a * grow;
-                o[mt][3] *= alpha_b * grow;
+                o[mt][0] *= alpha_a;
+                o[mt][1] *= alpha_b;
+                o[mt][2] *= alpha_a;
+                o[mt][3] *= alpha_b;
             }
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh) {
@@ -1513,6 +1536,16 @@ __global__ void __launch_bounds__(Ring<kE4m3, kCtaMerge>::kWarps * 32, 1)
                     }
                 }
             }
+            if (min(ev[0], ev[1]) < e_top - kFarExp) {
+                sum_a = sum_b = 0.f;
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {
+                    sum_a += exp2f((sv[hh][0] - ef[hh]) - mn_a) + exp2f((sv[hh][2] - ef[hh]) - mn_a);
+                    sum_b += exp2f((sv[hh][1] - ef[hh]) - mn_b) + exp2f((sv[hh][3] - ef[hh]) - mn_b);
+                }
+            }
+            l_a = l_a * alpha_a + sum_a;
+            l_b = l_b * alpha_b + sum_b;
             __syncwarp();
             if (lane == 0) {
                 fence_proxy_async_smem();

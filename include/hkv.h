@@ -154,7 +154,9 @@ typedef enum hkv_cache_type { HKV_CACHE_F16 = 0, HKV_CACHE_E4M3 = 1 } hkv_cache_
  * slot, prefix and compute call of this header works on both; the KV-head split
  * (hkv_split_*) and hkv_decode_attn_noalloc take F16 only.  On an E4M3 engine the
  * appends quantise their rows, attention reads the codes, and hkv_gather returns
- * the values the codes stand for, rounded to F16. */
+ * the values the codes stand for, rounded to F16.  The one-token attention weighs V by
+ * two F16 parts a weight: 22 bits, or 2^-39 of the row's largest p_t 2^e_t (p_t the
+ * weight, e_t the exponent of the key's V) where that is more. */
 int hkv_engine_create_cache(const hkv_config *cfg, int32_t cache_type, hkv_engine **out);
 int hkv_engine_cache_type(const hkv_engine *eng, int32_t *out);
 
