@@ -128,15 +128,19 @@ class Staging {
         }
     }
 
+    // Both buffers, for uploads of up to `bytes`.
+    cudaError_t reserve(size_t bytes) {
+        cudaError_t e = cudaSuccess;
+        for (int i = 0; i < 2 && e == cudaSuccess; ++i) {
+            e = ensure(buf_[i], bytes);
+        }
+        return e;
+    }
+
     // Host memory for the next upload of `bytes`.
     cudaError_t begin(size_t bytes, void **host_out) {
         cur_ ^= 1;
         Buf &b = buf_[cur_];
-        if (b.copied == nullptr) {
-            cudaError_t e = cudaEventCreateWithFlags(&b.copied, cudaEventDisableTiming);
-            if (e == cudaSuccess) e = cudaEventCreateWithFlags(&b.used, cudaEventDisableTiming);
-            if (e != cudaSuccess) return e;
-        }
         if (b.copy_pending) {
             const auto t0 = std::chrono::steady_clock::now();
             cudaError_t e = cudaEventSynchronize(b.copied);
@@ -146,24 +150,8 @@ class Staging {
             if (e != cudaSuccess) return e;
             b.copy_pending = false;
         }
-        if (bytes > b.cap) {
-            if (b.host != nullptr) {
-                cudaEventSynchronize(b.used);
-                cudaFreeHost(b.host);
-                cudaFree(b.dev);
-                b.host = nullptr;
-                b.dev = nullptr;
-                b.cap = 0;
-            }
-            size_t cap = 4096;
-            while (cap < bytes) cap *= 2;
-            cudaError_t e = cudaHostAlloc(&b.host, cap, cudaHostAllocDefault);
-            if (e != cudaSuccess) return e;
-            e = cudaMalloc(&b.dev, cap);
-            if (e != cudaSuccess) return e;
-            b.cap = cap;
-            b.used_recorded = false;
-        }
+        const cudaError_t e = ensure(b, bytes);
+        if (e != cudaSuccess) return e;
         *host_out = b.host;
         return cudaSuccess;
     }
@@ -208,6 +196,35 @@ class Staging {
         bool copy_pending = false;
         bool used_recorded = false;
     };
+
+    // Events, and room for `bytes` (at least a page's worth, doubling).
+    static cudaError_t ensure(Buf &b, size_t bytes) {
+        if (b.copied == nullptr) {
+            cudaError_t e = cudaEventCreateWithFlags(&b.copied, cudaEventDisableTiming);
+            if (e == cudaSuccess) e = cudaEventCreateWithFlags(&b.used, cudaEventDisableTiming);
+            if (e != cudaSuccess) return e;
+        }
+        if (bytes > b.cap) {
+            if (b.host != nullptr) {
+                cudaEventSynchronize(b.used);
+                cudaFreeHost(b.host);
+                cudaFree(b.dev);
+                b.host = nullptr;
+                b.dev = nullptr;
+                b.cap = 0;
+            }
+            size_t cap = 4096;
+            while (cap < bytes) cap *= 2;
+            cudaError_t e = cudaHostAlloc(&b.host, cap, cudaHostAllocDefault);
+            if (e != cudaSuccess) return e;
+            e = cudaMalloc(&b.dev, cap);
+            if (e != cudaSuccess) return e;
+            b.cap = cap;
+            b.used_recorded = false;
+        }
+        return cudaSuccess;
+    }
+
     Buf buf_[2];
     int cur_ = 1;
     int64_t wait_ns_ = 0;
@@ -315,8 +332,7 @@ struct hkv_engine {
     hkv::Staging batch_stage, range_stage, gather_stage, cow_stage, write_stage, read_stage, window_stage;
     hkv::RowCache write_rows, read_rows;
     hkv::WindowCache window;
-    float *window_work = nullptr;   // parts of split window tiles, grown on demand
-    int64_t window_work_parts = 0;
+    float *window_work = nullptr;  // parts of split window tiles
     // Copy-on-write copies decided on the host and not yet enqueued:
     // {source page, destination page} pairs, flushed as one kernel launch.
     std::vector<int32_t> cow_pending;
@@ -833,39 +849,6 @@ int upload_rows(hkv_engine *eng, Staging &stage, RowCache &rc, int32_t n, const 
     return HKV_OK;
 }
 
-// The most key blocks one CTA of a window attention takes, of tiles with `blocks`
-// each.  Where the tiles alone do not fill the GPU's SMs, the least for which their
-// parts still run at once (700 tokens into an empty slot: 27 us at 3 blocks, 40 at 2,
-// where a few parts start a second wave; 37 tokens behind 770: 19 us at 1, 21 at 2, 25 at
-// 3).  Otherwise an SM's share of all blocks, so that no long tile ends the launch alone.
-int64_t window_split(const std::vector<int64_t> &blocks, int64_t n_head_kv, int64_t sms) {
-    auto ctas = [&](int64_t most) {
-        int64_t n = 0;
-        for (const int64_t b : blocks) {
-            n += (b + most - 1) / most;
-        }
-        return n * n_head_kv;
-    };
-    int64_t total = 0, longest = 1;
-    for (const int64_t b : blocks) {
-        total += b;
-        longest = std::max(longest, b);
-    }
-    if (ctas(longest) > sms) {
-        return (total * n_head_kv + sms - 1) / sms;
-    }
-    int64_t lo = 1, hi = longest;  // hi fits
-    while (lo < hi) {
-        const int64_t mid = (lo + hi) / 2;
-        if (ctas(mid) <= sms) {
-            hi = mid;
-        } else {
-            lo = mid + 1;
-        }
-    }
-    return hi;
-}
-
 // Uploads the tiles and page lists of a window attention call.
 int upload_window(hkv_engine *eng, int32_t n, const int32_t *slots, const int64_t *begin,
                   const int64_t *count, cudaStream_t stream) {
@@ -914,13 +897,9 @@ int upload_window(hkv_engine *eng, int32_t n, const int32_t *slots, const int64_
         }
         row0 += count[e];
     }
-    if (parts > eng->window_work_parts) {
-        cudaFree(eng->window_work);  // waits for the kernels that use it
-        eng->window_work = nullptr;
-        eng->window_work_parts = 0;
-        HKV_CUDA_TRY(eng, cudaMalloc(&eng->window_work,
-                                     static_cast<size_t>(parts) * G * kWindowPartFloats * sizeof(float)));
-        eng->window_work_parts = parts;
+    if (parts * G > window_part_units(eng->num_sms)) {
+        return fail(eng, HKV_ERR_OOM, "window needs %lld part units, %lld there", static_cast<long long>(parts * G),
+                    static_cast<long long>(window_part_units(eng->num_sms)));
     }
     // the longest runs first: they bound the launch's end
     std::stable_sort(tiles.begin(), tiles.end(),
@@ -1316,6 +1295,15 @@ int hkv_engine_create_cache(const hkv_config *cfg, int32_t cache_type, hkv_engin
         e = cudaMalloc(&eng->counters, counter_bytes);
         if (e == cudaSuccess) e = cudaMemset(eng->counters, 0, counter_bytes);
         if (e != cudaSuccess) return fail_create(e, "merge counters");
+        // What the calls over many rows need besides the pool is taken here: an allocation
+        // inside a call stalls the device, and is refused while another stream captures.
+        e = cudaMalloc(&eng->window_work, static_cast<size_t>(window_part_units(eng->num_sms)) *
+                                              kWindowPartFloats * sizeof(float));
+        const size_t descriptor = std::min<size_t>(static_cast<size_t>(cfg->n_pages) * sizeof(RowItem), 1 << 20);
+        for (Staging *stage : {&eng->write_stage, &eng->read_stage, &eng->window_stage}) {
+            if (e == cudaSuccess) e = stage->reserve(descriptor);
+        }
+        if (e != cudaSuccess) return fail_create(e, "window workspace");
         e = cudaDeviceSynchronize();
         if (e != cudaSuccess) return fail_create(e, "create sync");
     }

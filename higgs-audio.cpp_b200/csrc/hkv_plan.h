@@ -417,4 +417,43 @@ inline BatchView bind_plan(const int32_t *d, int32_t n, int32_t G, const PlanSum
     return b;
 }
 
+// The most key blocks one CTA of a window attention takes, of tiles with `blocks`
+// each.  Where the tiles alone do not fill the GPU's SMs, the least for which their
+// parts still run at once (700 tokens into an empty slot: 27 us at 3 blocks, 40 at 2,
+// where a few parts start a second wave; 37 tokens behind 770: 19 us at 1, 21 at 2, 25 at
+// 3).  Otherwise an SM's share of all blocks, so that no long tile ends the launch alone.
+inline int64_t window_split(const std::vector<int64_t> &blocks, int64_t n_head_kv, int64_t sms) {
+    auto ctas = [&](int64_t most) {
+        int64_t n = 0;
+        for (const int64_t b : blocks) {
+            n += (b + most - 1) / most;
+        }
+        return n * n_head_kv;
+    };
+    int64_t total = 0, longest = 1;
+    for (const int64_t b : blocks) {
+        total += b;
+        longest = std::max(longest, b);
+    }
+    if (ctas(longest) > sms) {
+        return (total * n_head_kv + sms - 1) / sms;
+    }
+    int64_t lo = 1, hi = longest;  // hi fits
+    while (lo < hi) {
+        const int64_t mid = (lo + hi) / 2;
+        if (ctas(mid) <= sms) {
+            hi = mid;
+        } else {
+            lo = mid + 1;
+        }
+    }
+    return hi;
+}
+
+// The most (part, KV head) units that a plan by window_split has.  Tiles that fit the SMs
+// together are cut into at most `sms` CTAs.  Otherwise a tile is cut where it is longer
+// than an SM's share of all blocks: there are fewer than sms / n_head_kv such tiles, and
+// their full shares are as many again.
+inline int64_t window_part_units(int64_t sms) { return 2 * sms; }
+
 }  // namespace hkv

@@ -12,7 +12,9 @@
  * layer's slab), K and V, all KV heads, in F16 (or in 8 bits, see
  * hkv_engine_create_cache).  Each live slot owns a page list; pages are reference
  * counted so slots can share a prefix (fork / published prefixes) and are
- * copied on the first write into a shared page (copy-on-write).
+ * copied on the first write into a shared page (copy-on-write).  Beside the pool an
+ * engine takes its partials and the window attention's parts (some 40 MB) when it is
+ * made; compute calls allocate only where a plan outgrows its upload buffer.
  *
  * Conventions:
  *   * Every function returns an hkv_status; on failure hkv_last_error() holds

@@ -257,3 +257,53 @@ def test_large_logits(hkv_lib, cache, name):
         assert sure > n * 4 * G // 2
         eng.release(s)
     eng.close()
+
+
+@pytest.mark.parametrize("cache", ["e4m3", "f16"])
+def test_no_memory_is_taken_inside_a_call(hkv_lib, cache):
+    """A new engine's first calls over many rows, the window split over keys, while another stream captures
+    (which CUDA refuses every allocation for): they run."""
+    import hkv
+    rng = np.random.default_rng(97)
+    G = 8
+    old, new = [3000, 500], [40, 700]
+
+    def calls(eng, slots, data, out, stream=None):
+        q, k, v = data
+        eng.qkv_write(0, slots, new, q, k, v, q_out=q, stream=stream)
+        eng.window_attn(0, slots, new, q, out, stream=stream)
+        kk, vv = torch.empty((2, sum(new), G, D), device=DEV).unbind(0) if stream is None else calls.back
+        eng.cache_read(0, slots, old, new, kk, vv, dtype=hkv.F32, stream=stream)
+        calls.back = (kk, vv)
+
+    results = []
+    data = [rng.standard_normal((sum(new), h, D)).astype(np.float32) for h in (4 * G, G, G)]
+    kept = [(rows(rng, n, G), rows(rng, n, G)) for n in old]
+    for captured in (False, True):
+        eng = engine(hkv, G, cache)
+        slots = [eng.acquire() for _ in old]
+        # one upload of a descriptor, so that the call in question has a buffer to itself: waiting for
+        # an upload's event is what CUDA forbids as well while a stream captures
+        k, v = (dev(np.concatenate(a)) for a in zip(*kept))
+        eng.qkv_write(0, slots, old, None, k, v)
+        for s, n in zip(slots, old):
+            eng.advance([s], n)
+        x = [dev(a) for a in data]
+        out = torch.empty((sum(new), 4 * G * D), device=DEV)
+        if not captured:
+            calls(eng, slots, x, out)
+        else:
+            work, side = torch.cuda.Stream(), torch.cuda.Stream()
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.stream(side):
+                graph.capture_begin()
+                try:
+                    calls(eng, slots, x, out, work.cuda_stream)
+                finally:
+                    graph.capture_end()
+            work.synchronize()
+        eng.sync_check()
+        results.append(out.clone())
+        eng.close()
+    assert torch.equal(*results)
