@@ -389,6 +389,7 @@ int fail(const hkv_engine *eng, int status, const char *fmt, ...) {
 }
 
 int cuda_fail(const hkv_engine *eng, cudaError_t e, const char *what) {
+    (void)cudaGetLastError();  // reported here: the next call's launches are judged by their own
     return fail(eng, HKV_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 

@@ -76,3 +76,32 @@ def test_decode_of_values_near_the_largest_floats(cache8, lens):
         kk, vv = cached(c.eng, c.hkv, slots[i], lens[i] + 1, 8)
         want, bound = weighed(c.rope(q[i:i + 1], [lens[i]]).astype(np.float64), kk, vv, lens[i], "f32", 14)
         assert (np.abs(out[i:i + 1] - want) <= bound).all(), i
+
+
+def test_a_failed_call_does_not_fail_the_next(cache8):
+    """A call that needs an allocation while a stream captures is refused by CUDA; the error is that call's
+    alone."""
+    rng = np.random.default_rng(107)
+    c = cache8(G=1)
+    s = c.slot()
+    c.prefill(s, rows(rng, 20, 1), rows(rng, 20, 1))
+    k, v = torch.zeros((2, 20, 1, D), dtype=torch.int16, device=DEV).unbind(0)
+    side, work = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    failed = False
+    with torch.cuda.stream(side):
+        graph.capture_begin()
+        try:
+            c.eng.gather(s, 0, 0, 20, k, v, stream=work.cuda_stream)
+        except c.hkv.HkvError as e:
+            failed = e.status == c.hkv.HKV_ERR_CUDA
+        try:
+            graph.capture_end()
+        except RuntimeError:
+            pass  # the refused allocation ended the capture
+    if failed:
+        c.eng.gather(s, 0, 0, 20, k, v, stream=work.cuda_stream)
+    work.synchronize()
+    want, _ = c.read(s, 0, 20, dtype=torch.float16)
+    assert np.array_equal(k.cpu().numpy().view(np.float16), want)
