@@ -271,7 +271,7 @@ def _ptr(x) -> Optional[int]:
     if isinstance(x, int):
         return x
     try:
-        return x.data_ptr()
+        return int(x.data_ptr())
     except AttributeError:
         pass
     if isinstance(x, np.ndarray):
@@ -289,14 +289,25 @@ def _stream(s) -> Optional[int]:
     raise TypeError(f"cannot take a CUDA stream handle from {type(s)!r}")
 
 
+def _slot_array(slots: Sequence[int]):
+    """Slot ids as int32: what int() makes of each, -1 (no slot) for one beyond 32 bits."""
+    if not isinstance(slots, (bytes, bytearray)):  # whose bytes array() would take for the ids' own
+        try:
+            return array("i", slots)
+        except (TypeError, OverflowError):
+            pass
+    ids = [int(s) for s in slots]
+    return array("i", [i if -2 ** 31 <= i < 2 ** 31 else -1 for i in ids])
+
+
 def _slots_arg(slots: Sequence[int]):
-    a = array("i", slots)
+    a = _slot_array(slots)
     return len(a), (ctypes.c_int32 * len(a)).from_buffer(a)
 
 
 def _slots_in(slots: Sequence[int]):
     """A slot list as an array (which the caller holds on to), its length and address."""
-    a = array("i", slots)
+    a = _slot_array(slots)
     address, n = a.buffer_info()
     return a, n, address
 
