@@ -286,6 +286,7 @@ __global__ void __launch_bounds__(kOneRow ? 96 : 256, kOneRow ? 1 : sizeof(T) ==
             }
         }
         put_codes(block, r0, lane, x, pow2(-e));
+        __syncwarp();  // every lane has its old exponent
         if (lane == 0) {
             exps[slice] = e;
         }
