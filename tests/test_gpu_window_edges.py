@@ -307,3 +307,63 @@ def test_no_memory_is_taken_inside_a_call(hkv_lib, cache):
         results.append(out.clone())
         eng.close()
     assert torch.equal(*results)
+
+
+@pytest.mark.parametrize("cache", ["e4m3", "f16"])
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+def test_values_that_are_not_finite_in_long_slots(hkv_lib, cache, name):
+    """V that is not finite in some of 1,250 pages, two of them 1,024 apart, in whole and in split tiles: the
+    rows that see one have it in its dim, those before it do not."""
+    import hkv
+    rng = np.random.default_rng(99)
+    G, n, t = 1, 19900, 100
+    eng = hkv.Engine(n_layers=1, n_head=4, n_head_kv=1, n_pages=1300, max_slots=1, context_length=n + t, device=0,
+                     shuffle_seed=9, cache=cache)
+    s = eng.acquire()
+    k, v = rows(rng, n + t, G), rows(rng, n + t, G)
+    bad = {160: 5, 160 + 1024 * 16: 6, 9999: 7, n + 50: 8, n + 99: 9}
+    for row, dim in bad.items():
+        v[row, 0, dim] = np.nan
+    eng.rope_append_range(0, s, n, dev(k[:n]), dev(v[:n]))
+    eng.advance([s], n)
+    eng.rope_append_range(0, s, t, dev(k[n:]), dev(v[n:]))
+    q = torch.from_numpy(rng.standard_normal((t, 4, D)).astype(np.float32)).to(DEV)
+    out = window(eng, hkv, [s], [t], q, name).float().cpu().numpy().reshape(t, 4, D)
+    want = np.zeros((t, 4, D), bool)
+    for row, dim in bad.items():
+        want[max(0, row - n):, :, dim] = True
+    assert np.array_equal(np.isnan(out), want)
+    eng.close()
+
+
+def test_one_bad_value_does_not_stop_a_prompt(hkv_lib):
+    """A prompt of 6,000 with one NaN in V at its start: not all of V is read again for it (the prompt
+    took 88 times as long when it was; the bound is ten times)."""
+    import hkv
+    rng = np.random.default_rng(109)
+    G, n = 8, 6000
+    eng = engine(hkv, G, "e4m3")
+    times = []
+    for bad in (False, True):
+        s = eng.acquire()
+        v = rows(rng, n, G)
+        if bad:
+            v[3, :, 17] = np.nan
+        eng.rope_append_range(0, s, n, dev(rows(rng, n, G)), dev(v))
+        q = torch.from_numpy(rng.standard_normal((n, 4 * G, D)).astype(np.float32)).to(DEV).bfloat16()
+        out = torch.empty((n, 4 * G * D), dtype=torch.bfloat16, device=DEV)
+        best = 1e9
+        for _ in range(4):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            eng.window_attn(0, [s], [n], q, out, dtype=hkv.BF16)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        times.append(best)
+        got = torch.isnan(out.view(n, 4 * G, D))
+        assert got[:, :, 17].sum() == (n - 3) * 4 * G * bad and got.sum() == got[:, :, 17].sum()
+        eng.release(s)
+    print("ms without and with:", times)
+    assert times[1] < 10 * times[0]
+    eng.close()
