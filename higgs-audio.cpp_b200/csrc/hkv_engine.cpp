@@ -1844,6 +1844,9 @@ int hkv_window_attn(hkv_engine *eng, const hkv_window_attn_args *args, hkv_strea
     st = check_stride(eng, "q", row, a.dtype, &w.q_stride);
     if (st == HKV_OK) st = check_stride(eng, "out", row, a.dtype, &w.out_stride);
     if (st != HKV_OK) return st;
+    if (a.q == a.out && w.q_stride != w.out_stride) {
+        return fail(eng, HKV_ERR_INVALID, "out in q's place needs equal strides");
+    }
     std::vector<int64_t> begin(static_cast<size_t>(a.n));
     for (int32_t e = 0; e < a.n; ++e) {
         const Slot &s = eng->slots[a.slots[e]];

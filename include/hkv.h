@@ -288,7 +288,8 @@ int hkv_qkv_write(hkv_engine *eng, const hkv_qkv_write_args *args, hkv_stream st
  * the last layer).  The many-token form of hkv_decode_attn: prompts and refreshed
  * windows (:6278-6279, :6603-6604).  q: [rows][n_head][128], rotated already
  * (hkv_qkv_write's q_out); out: [rows][n_head * 128]; both of dtype, the rows of all
- * slots back to back, strides in elements (0: packed), each a multiple of 16 bytes.
+ * slots back to back, strides in elements (0: packed), each a multiple of 16 bytes.  out
+ * may be q (with equal strides), and else shares no element with it.
  * Softmax statistics and sums are F32.  With F32 tensors q and the weights enter the
  * products in two F16 parts (22 bits, as in hkv_decode_attn), with F16 or BF16 ones q
  * as it is and the weights rounded to F16; |q| up to 65504, and to 2^-25 below 2^-14

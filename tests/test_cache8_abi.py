@@ -126,3 +126,10 @@ def test_the_model_rounds_as_e4m3_does():
     for amax, e in ((448.0, 0), (np.nextafter(448, 500), 1), (449.0, 1), (224.0, -1), (1.75, -8),
                     (1.76, -7), (0.0, -100), (1e-40, -100), (3.4e38, 120)):
         assert block_exponent([amax]) == e, amax
+
+
+def test_window_in_place_needs_equal_strides(eng):
+    import hkv
+    s = eng.acquire(0)
+    refused(eng, hkv.HKV_ERR_INVALID, eng.window_attn, 0, [s], [0], 16, 16, q_stride=8192)
+    refused(eng, hkv.HKV_ERR_NO_DEVICE, eng.window_attn, 0, [s], [0], 16, 16, q_stride=8192, out_stride=8192)

@@ -367,3 +367,24 @@ def test_one_bad_value_does_not_stop_a_prompt(hkv_lib):
     print("ms without and with:", times)
     assert times[1] < 10 * times[0]
     eng.close()
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("old,new", [([700], [300]), ([1500] * 16, [60] * 16)])
+def test_window_in_place(hkv_lib, name, old, new):
+    """out = q, with equal strides: the same bits as into another tensor, in split and in whole tiles."""
+    import hkv
+    rng = np.random.default_rng(115)
+    G = 8
+    eng = engine(hkv, G, "e4m3", n_pages=2000)
+    slots = [eng.acquire() for _ in old]
+    for s, p, n in zip(slots, old, new):
+        fill(eng, rng, s, p, G)
+        fill(eng, rng, s, n, G, advance=False)
+    q = torch.from_numpy(rng.standard_normal((sum(new), 4 * G, D)).astype(np.float32)).to(DEV)
+    out = window(eng, hkv, slots, new, q, name)
+    x = q.to(DT[name]).reshape(sum(new), -1)
+    eng.window_attn(0, slots, new, x, x, dtype=getattr(hkv, name.upper()))
+    eng.sync_check()
+    assert torch.equal(out, x)
+    eng.close()
