@@ -369,6 +369,65 @@ def test_one_bad_value_does_not_stop_a_prompt(hkv_lib):
     eng.close()
 
 
+@pytest.mark.parametrize("cache", ["e4m3", "f16"])
+def test_f32_windows_keep_22_bits_on_the_average(hkv_lib, cache):
+    """The root mean square error of F32 outputs, relative to theirs, against float64 over the cached rows.
+
+    A weight is off, relative to itself, by at most 2^-22 (two F16 parts), by 2^-22 |q| |k| / sqrt(128) through
+    q's two parts, and by the 16 cut steps of its logit's sum, each under 2^-23 of a partial sum that is a few
+    units at most: 16 * 2^-24 on the average for each unit.  Errors of different keys are independent, as their V
+    are: the output's is no more than a weight's, under 2^-17 for partial sums up to 8.  Twice that is the bound.  A
+    weight held in one F16 part would be off by 2^-12 / sqrt(3) on the average: nine times the bound."""
+    import hkv
+    rng = np.random.default_rng(111)
+    G = 2
+    eng = engine(hkv, G, cache)
+    err = size = 0.0
+    old, new = [0, 300, 1000], [150, 64, 20]
+    slots = [eng.acquire() for _ in old]
+    for s, p, n in zip(slots, old, new):
+        fill(eng, rng, s, p, G)
+        fill(eng, rng, s, n, G, advance=False)
+    q = torch.from_numpy(rng.standard_normal((sum(new), 4 * G, D)).astype(np.float32)).to(DEV)
+    out = window(eng, hkv, slots, new, q).double().cpu().numpy().reshape(-1, 4 * G, D)
+    x = q.double().cpu().numpy()
+    at = 0
+    for s, p, n in zip(slots, old, new):
+        k, v = cached(eng, hkv, s, p + n, G)
+        want, _ = weighed(x[at:at + n], k, v, p, "f32", 7)
+        err += ((out[at:at + n] - want) ** 2).sum()
+        size += (want ** 2).sum()
+        at += n
+    assert np.sqrt(err / size) < 2.0 ** -16
+    eng.close()
+
+
+@pytest.mark.parametrize("cache", ["e4m3", "f16"])
+def test_long_whole_tiles_keep_their_sums(hkv_lib, cache):
+    """V = 1 over 30,000 keys in tiles that are not split (19 slots of 8 KV heads): each output is the sum of the
+    weights over itself.  The tensor cores cut each of the 16 products of 128 keys by less than a unit in the last
+    place of the sum, half of that, 2^-24, on the average; sums leave them every 4 blocks, so no part of one is
+    cut more than 64 times: 64 * 2^-24.  The additions outside round to nearest, with no drift: 8 * 2^-24 are
+    left for them.  Without the moves the sum drifts by 1.4e-5."""
+    import hkv
+    rng = np.random.default_rng(113)
+    G, n, t, count = 8, 30000, 20, 19
+    eng = hkv.Engine(n_layers=1, n_head=32, n_head_kv=G, n_pages=count * 1877, max_slots=count, context_length=n + t,
+                     device=0, shuffle_seed=9, cache=cache)
+    gen = torch.Generator(device=DEV).manual_seed(113)
+    slots = [eng.acquire() for _ in range(count)]
+    for s in slots:
+        k = torch.randn((n + t, G, D), generator=gen, device=DEV) * 0.3
+        v = torch.ones_like(k)
+        eng.rope_append_range(0, s, n, k[:n].contiguous(), v[:n].contiguous())
+        eng.advance([s], n)
+        eng.rope_append_range(0, s, t, k[n:].contiguous(), v[n:].contiguous())
+    q = torch.randn((count * t, 32, D), generator=gen, device=DEV)
+    out = window(eng, hkv, slots, [t] * count, q).double()
+    assert abs((out - 1).mean().item()) < 72 * 2.0 ** -24
+    eng.close()
+
+
 @pytest.mark.parametrize("name", ["f32", "bf16"])
 @pytest.mark.parametrize("old,new", [([700], [300]), ([1500] * 16, [60] * 16)])
 def test_window_in_place(hkv_lib, name, old, new):
@@ -387,4 +446,63 @@ def test_window_in_place(hkv_lib, name, old, new):
     eng.window_attn(0, slots, new, x, x, dtype=getattr(hkv, name.upper()))
     eng.sync_check()
     assert torch.equal(out, x)
+    eng.close()
+
+
+def test_window_in_a_capture_is_refused(hkv_lib):
+    import hkv
+    eng = engine(hkv, 1, "e4m3")
+    rng = np.random.default_rng(117)
+    s = eng.acquire()
+    fill(eng, rng, s, 40, 1, advance=False)
+    q = torch.zeros((40, 4 * D), device=DEV)
+    out = torch.full_like(q, 5.0)
+    side = torch.cuda.Stream()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        g.capture_begin()
+        try:
+            with pytest.raises(hkv.HkvError, match="captured") as e:
+                eng.window_attn(0, [s], [40], q, out, stream=side.cuda_stream)
+            assert e.value.status == hkv.HKV_ERR_INVALID
+        finally:
+            g.capture_end()
+    eng.sync_check()
+    assert (out == 5.0).all()
+    eng.close()
+
+
+@pytest.mark.parametrize("cache", ["e4m3", "f16"])
+def test_windows_one_after_another(hkv_lib, cache):
+    """One engine: a plan found again on another stream (ordered behind the first), small and large split
+    windows in turn, two layers, and a slot given back and taken by another request in between."""
+    import hkv
+    rng = np.random.default_rng(119)
+    G = 8
+    eng = engine(hkv, G, cache, n_layers=2)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for old, new in (([30], [5]), ([2500, 100], [64, 300]), ([0], [3]), ([4000], [128]), ([17, 300, 900], [1, 90, 2])):
+        slots = [eng.acquire() for _ in old]
+        for layer in range(2):
+            for s, p in zip(slots, old):
+                fill(eng, rng, s, p, G, layer, advance=False)
+        for s, p in zip(slots, old):
+            eng.advance([s], p)
+        for layer in range(2):
+            for s, n in zip(slots, new):
+                fill(eng, rng, s, n, G, layer, advance=False)
+        torch.cuda.synchronize()
+        q = torch.from_numpy(rng.standard_normal((sum(new), 4 * G, D)).astype(np.float32)).to(DEV)
+        outs = torch.zeros((4, sum(new), 4 * G * D), device=DEV)
+        for i in range(4):
+            streams[i % 2].wait_stream(streams[1 - i % 2])
+            eng.window_attn(i // 2, slots, new, q, outs[i], stream=streams[i % 2].cuda_stream)
+        for s in streams:
+            s.synchronize()
+        eng.sync_check()
+        for layer in range(2):
+            assert torch.equal(outs[2 * layer], outs[2 * layer + 1])
+            check(eng, hkv, slots, new, q, outs[2 * layer], "f32", layer)
+        for s in slots:
+            eng.release(s)
     eng.close()
