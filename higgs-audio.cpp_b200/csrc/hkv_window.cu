@@ -630,10 +630,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int first_last = t.pos0 + i * kTileTokens - t.key0;         // and the tile's first row
         const int blocks = i == 0 ? nb0 : nb1;
         float m = -INFINITY, l = 0.f;
-        bool huge = false;  // of a row of the warp
-        // what a page's products are multiplied by (finite: 0 * inf would be no logit)
+        // What a page's products are multiplied by: with K's exponents up to 120 and those of q,
+        // |q| <= 65504, up to 8, a finite float.
         auto logit_scale = [&](const PageScale &page) {
-            return S::kCodeK ? fminf(page.k * q_scale, 3.402823466e38f) : page.k;
+            return S::kCodeK ? page.k * q_scale : page.k;
         };
         const bool live = my_tok < t.tokens;
         // the token's four rows, from this lane's dims on
@@ -723,7 +723,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 m = m_new;
                 l *= corr;
                 kept *= corr;
-                huge = __any_sync(0xffffffffu, fabsf(m) > kHuge && m != -INFINITY);
                 if (j > 0 && !drain) {
 #pragma unroll 1
                     for (int c = 0; c < 64; c += 16) {
@@ -739,6 +738,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             const float bound = m == -INFINITY ? 0.f : m;
             const bool far = kE4m3 && b.far != 0;
+            const bool huge = __any_sync(0xffffffffu, fabsf(bound) > kHuge);  // of a row of the warp
             if (far || huge) {
 #pragma unroll 1
                 for (int p = 0; p < 4; ++p) {
