@@ -172,8 +172,8 @@ constexpr int kAttnStages = HKV_ATTN_STAGES;  // TMA ring depth per warp (K+V bl
 // (half as large) each.  Without it (many segments): up to 12 warps x 4 stages.  A
 // page costs a warp as many instructions as an F16 page and half the time on the
 // bus, so the loop is bound by latency until a scheduler has three warps: 32 slots of
-// 2k-16k positions 122 us a layer with 8 warps, 111 with 10, 100 with 12 x 4 stages,
-// 108 with 12 x 2, 106 with 16 x 2 (which spills).
+// 2k-16k positions, layer behind layer, 118 us with 8 warps, 113 with 10, 101 with 12 x 4
+// stages, 111 with 12 x 2, 121 with 16 x 2 (which spills).
 #ifndef HKV_ATTN_STAGES_E4M3
 #define HKV_ATTN_STAGES_E4M3 4
 #endif

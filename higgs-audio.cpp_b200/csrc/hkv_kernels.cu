@@ -2102,7 +2102,7 @@ void launch_attention_t(const PoolView &pool, const RopeView &rope, const BatchV
     cudaLaunchAttribute attr[2];
     int n_attr = 0;
     // The 8-bit kernel is always launched as a dependent of the kernel before it, so
-    // that its CTAs are set up while that one ends (a batch-1 step: 10.5 -> 9.1 us), and
+    // that its CTAs are set up while that one ends (a batch-1 step of 1024 rows 8.8 us), and
     // waits at its start where it may not overlap.
     if (overlap_previous || kE4m3) {
         attr[n_attr].id = cudaLaunchAttributeProgrammaticStreamSerialization;

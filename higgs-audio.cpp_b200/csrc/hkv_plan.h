@@ -61,8 +61,8 @@ inline int32_t plan_warps(int64_t total_units, int64_t max_warps) {
 // CTA per SM, as few as the plan needs): three units a warp, since it takes pages
 // in pairs and every warp adds a partial to merge, but one warp an SM before any
 // has more than two units.  Measured with 1, 2, 3, 4 and 6 units a warp: 16 slots of
-// 16 rows 7.4 / 5.7 / 8.8 / 8.9 / 12.3 us (128, 128, 86 .. warps), 16 of 200 rows 13.3 /
-// 11.6 / 9.0 / 10.6 / 11.7, 32 of 300 rows 15.7 / 15.8 / 14.4 / 14.4 / 15.3.
+// 16 rows 7.5 / 5.6 / 8.8 / 8.8 / 12.0 us, 16 of 200 rows 13.2 / 11.4 / 9.1 / 10.5 /
+// 11.4, 32 of 300 rows 14.6 / 14.6 / 14.0 / 14.2 / 15.3.
 inline int32_t plan_wide_warps(int64_t total_units, int64_t sms) {
     const int64_t want = std::max((total_units + 2) / 3, std::min((total_units + 1) / 2, sms));
     return static_cast<int32_t>(std::min(want, sms * kAttnWarpsE4m3));
@@ -95,11 +95,11 @@ inline bool plan_combine(bool cta_merge, int32_t max_parts) {
     return cta_merge && max_parts > 1 && max_parts <= kCombineMaxParts;
 }
 // For the wide variant of the 8-bit kernel the combine launch pays where a segment
-// would take two levels, which a batch of unequal lengths then waits for: 16 slots of
-// 256-4096 positions 25.3 -> 22.3 us, 32 of 32-2048 20.2 -> 18.8, 20 of 1-8000 38.4 ->
-// 37.7 (layers one behind the other without a pause: 22.1 -> 21.1, 17.7 -> 17.8, 35.1 ->
-// 36.0).  With equal lengths, one level each, it loses: 24 of 2000 27.8 -> 28.6, 64 of
-// 500 23.6 -> 25.2.
+// would take two levels, which a batch of unequal lengths then waits for.  By tickets and by
+// the launch, one layer again and again and eight layers in turn: 16 slots of 256-4096
+// positions 27.8 and 25.0 us, 24.8 and 23.9; 20 of 1-8000 44.6 and 42.8, 41.5 and 41.8; 32 of
+// 32-2048 the same.  A second launch for segments of one level loses: 24 of 2000 27.6 and
+// 29.8 us, 64 of 500 23.6 and 30.3.
 inline bool plan_wide_combine(int32_t max_parts) {
     return max_parts > kMergeSingleMax && max_parts <= kCombineMaxParts;
 }
@@ -419,9 +419,9 @@ inline BatchView bind_plan(const int32_t *d, int32_t n, int32_t G, const PlanSum
 
 // The most key blocks one CTA of a window attention takes, of tiles with `blocks`
 // each.  Where the tiles alone do not fill the GPU's SMs, the least for which their
-// parts still run at once (700 tokens into an empty slot: 27 us at 3 blocks, 40 at 2,
-// where a few parts start a second wave; 37 tokens behind 770: 19 us at 1, 21 at 2, 25 at
-// 3).  Otherwise an SM's share of all blocks, so that no long tile ends the launch alone.
+// parts still run at once (700 F32 tokens into an empty slot: 26 us at 3 blocks, 34 at 2,
+// where a few parts start a second wave, 29 at 4; 37 tokens behind 770: 17 us at 1, 19 at 2,
+// 23 at 3).  Otherwise an SM's share of all blocks, so that no long tile ends the launch alone.
 inline int64_t window_split(const std::vector<int64_t> &blocks, int64_t n_head_kv, int64_t sms) {
     auto ctas = [&](int64_t most) {
         int64_t n = 0;

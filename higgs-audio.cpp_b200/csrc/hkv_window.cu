@@ -31,10 +31,12 @@
 //
 // What bounds it: the chain S, softmax, P, O of a block, which the two tiles of a CTA
 // take in turns; tensor pipe, exponentials and issue slots are each under half.  8 KV
-// heads, 8-bit cache: a BF16 prompt of 8100 595-640 us by its data (0.56-0.52 of the
-// measured bf16 rate); 8 F32 windows of 4-1024 behind 584-4000 461 us (0.51 of the rate
-// for the doubled products; the softmax's longer chain and the moves of o weigh most); 37 behind
-// 770 16.5 us (launch, one block's chain, the join).
+// heads, 8-bit cache: a BF16 prompt of 8100 605-645 us by its data (0.55-0.51 of the
+// measured bf16 rate), of F16 695, of F32 1033; 8 F32 windows of 4-1024 behind 584-4000 466 us
+// (0.51 of the rate for the doubled products; the softmax's longer chain and the moves of
+// o weigh most); 37 behind 770 16.7 us (launch, one block's chain, the join).  On an F16
+// cache, whose K and V the converters bring through registers at twice the bytes: the
+// prompt 1028 us in BF16 or F16, 1268 in F32.
 //
 // The rescaling of o when the bound m moves is put off until a row passes it by
 // 2^kSlack (weights up to 2^kSlack then enter the product); o is rescaled in TMEM
@@ -92,8 +94,8 @@ constexpr int kShift = 7;               // weights enter 2^7 larger: at most 2^1
 // the part) and is added there in F32.  The tensor cores cut their sums instead of
 // rounding them: each of a block's 16 products takes about 2^-24 of o away, always
 // towards zero, 1e-5 of it over 4000 keys.  Eight ragged windows (1024 keys on average
-// behind 2034): error 5.7e-6 and 390 us without, 2.5e-6 and 430 us every 8 blocks,
-// 1.5e-6 and 461 us every 4 (some 40 us more with sums read back and rescaled each time).
+// behind 2034): error 5.7e-6 and 391 us without, 2.5e-6 and 432 us every 8 blocks,
+// 1.5e-6 and 461 us every 4.
 constexpr int kDrainBlocks = 4;
 // V exponents this far below the largest so far: a weight of such a page may underflow in
 // F32 though its key weighs, so the sum of the weights is formed apart.  At less, terms
@@ -140,8 +142,9 @@ struct Shape {
     static constexpr bool kCodeK = kE4m3 && std::is_same<T, __nv_bfloat16>::value;
     static constexpr int kParts = kSplit || kCodeK ? 2 : 1;  // of q
     // F32: the products of half a block's weights start while the other half's are
-    // formed (8100 tokens 1230 -> 1197 us); a BF16 block's softmax is too short for that
-    // to pay for its second store and barrier (611 -> 616 us).
+    // formed (8100 tokens: 1033 us, 1086 without; on an F16 cache, which waits for its
+    // converters, 1265 and 1245); a 16-bit block's softmax is too short for that to pay for its second store and
+    // barrier (8 ragged windows: BF16 279 us, 283 with; 8100 tokens of F16 694 and 716).
     static constexpr bool kEarly = kSplit;
     static constexpr int kQPart = kCodeK ? kCodeTileBytes : kTileBytes;
     static constexpr int kKTile = kCodeK ? kCodeTileBytes : kTileBytes;
@@ -487,8 +490,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     BlockScale *scales = reinterpret_cast<BlockScale *>(ctl + 1);
     const int G = pool.n_head_kv;
     // The heads of a tile stand together, so that CTAs start in the order of the tiles,
-    // longest first (all tiles of a head, then the next head's: 8100 F32 tokens 1197 ->
-    // 1022 us, BF16 607 -> 600; 8 ragged windows F32 472 -> 453, BF16 267 -> 275)
+    // longest first: 8100 F32 tokens 1033 us, BF16 615, 8 ragged windows F32 461, BF16 279;
+    // with all tiles of a head, then the next head's, 1214, 630, 488 and 273
     const int h = blockIdx.x % G;
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -1193,8 +1196,8 @@ void launch_window_t(const PoolView &pool, const WindowArgs &a, DeviceError *err
     cfg.stream = stream;
     cfg.attrs = &attr;
     // A launch of one wave is set up while the kernel before it runs (37 tokens behind
-    // 770: 25 -> 19 us with the parts of one block that this makes worth it); one of
-    // several waves ends 4% later so, its first CTAs then waiting in the places of the last.
+    // 770: 16.7 us, 18.6 without); of one of several waves the first CTAs would wait in the
+    // places of the last (8100 tokens F32 1033 us, 1049 so; BF16 within 1%).
     cfg.numAttrs = a.one_wave ? 1 : 0;
     cudaLaunchKernelEx(&cfg, window_kernel<T, kE4m3>, pool, a.tiles, a.pages, a.layer, static_cast<const T *>(a.q),
                        a.q_stride, out, a.out_stride, a.work, a.scale_log2, err);

@@ -149,7 +149,9 @@ int hkv_abi_version(void);
  * least 2^(e-6), and at most 2^(e-10) below that.  A value that is not finite is
  * stored as NaN and leaves e alone.  As rows join a page, e only grows; the rows
  * already there are then rounded once more.  A write to the first row of a page
- * starts its blocks anew: the page's other rows are undefined until written. */
+ * starts its blocks anew: the page's other rows are undefined until written.  After
+ * hkv_slot_set_len or hkv_slot_fork into the middle of a page, e still covers the rows
+ * that were dropped there. */
 typedef enum hkv_cache_type { HKV_CACHE_F16 = 0, HKV_CACHE_E4M3 = 1 } hkv_cache_type;
 
 /* hkv_engine_create with the cache format chosen (hkv_engine_create: F16).  Every
