@@ -723,8 +723,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (__any_sync(0xffffffffu, mx > m + kSlack)) {
                 const float m_new = fmaxf(m, mx);
                 const float corr = (m_new == -INFINITY ? 1.f : exp2_fast(m - m_new));
+                if (kE4m3) {
+                    // in two steps: where V's exponent makes the bound jump, corr may
+                    // underflow though the keys so far weigh
+                    const float h = m_new == -INFINITY ? 1.f : exp2_fast(0.5f * (m - m_new));
+                    l = l * h * h;
+                } else {
+                    l *= corr;
+                }
                 m = m_new;
-                l *= corr;
                 kept *= corr;
                 if (j > 0 && !drain) {
 #pragma unroll 1

@@ -506,3 +506,33 @@ def test_windows_one_after_another(hkv_lib, cache):
         for s in slots:
             eng.release(s)
     eng.close()
+
+
+@pytest.mark.parametrize("low,high", [(0.0, 1e12), (0.0, 1e30), (1e-25, 1e20), (1e25, 0.0)])
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+def test_window_where_v_jumps_between_blocks(hkv_lib, name, low, high):
+    """Whole blocks of keys whose V is far below, or above, that of the next ones, at like weights: the sum of
+    weights keeps both, in whole tiles (19 slots of 8 heads) and in split ones."""
+    import hkv
+    rng = np.random.default_rng(121)
+    n, t = 640, 20
+    for G, count in ((1, 1), (8, 19)):
+        eng = engine(hkv, G, "e4m3", max_slots=count)
+        slots = [eng.acquire() for _ in range(count)]
+        for s in slots:
+            v = rows(rng, n + t, G)
+            v[:256] *= np.float32(low)
+            v[256:] *= np.float32(high)
+            k = rows(rng, n + t, G) * np.float32(0.3)
+            eng.rope_append_range(0, s, n, dev(k[:n]), dev(v[:n]))
+            eng.advance([s], n)
+            eng.rope_append_range(0, s, t, dev(k[n:]), dev(v[n:]))
+        q = torch.from_numpy(rng.standard_normal((count * t, 4 * G, D)).astype(np.float32)).to(DEV)
+        out = window(eng, hkv, slots, [t] * count, q, name).double().cpu().numpy().reshape(count, t, 4 * G, D)
+        x = q.to(DT[name]).double().cpu().numpy().reshape(count, t, 4 * G, D)
+        for i in range(0, count, 9):
+            k, v = cached(eng, hkv, slots[i], n + t, G)
+            want, bound = weighed(x[i][:, :4], k[:, :1], v[:, :1], n, name, 7)
+            over = np.abs(out[i][:, :4] - want) - bound
+            assert over.max() <= 0, (G, i, np.unravel_index(over.argmax(), over.shape), over.max())
+        eng.close()
