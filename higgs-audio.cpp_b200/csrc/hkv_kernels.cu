@@ -68,8 +68,8 @@ constexpr int kCtaSmem = kAttnWarps * 2 * kCtaPartBytes + 32;
 constexpr int kMaxCluster = 16;
 constexpr int kClusterSmem = kMaxCluster * kCtaPartBytes + 16;
 constexpr int kPShift = 14;  // o's weights are 2^14 larger in the 8-bit format: at most 16384 in F16
-// V exponents this far below the share's largest so far (8-bit format): a weight may
-// underflow though its key weighs, so l's terms are formed apart.
+// V exponents this far apart in a share (8-bit format): a weight, or the step of the
+// maximum from one page to the next, may underflow though the key weighs, so l is formed apart.
 constexpr int kFarExp = 100;
 constexpr int kWhereAppend = 0;
 constexpr int kWhereAttn = 1;
@@ -1435,6 +1435,7 @@ __global__ void __launch_bounds__(Ring<kE4m3, kCtaMerge>::kWarps * 32, 1)
                 }
                 if (e_top == INT32_MIN) {
                     e0 = min(max(ev[0], -6), 0);
+                    e_top = ev[0];
                 }
 #pragma unroll
                 for (int hh = 0; hh < 2; ++hh) {
@@ -1484,9 +1485,11 @@ __global__ void __launch_bounds__(Ring<kE4m3, kCtaMerge>::kWarps * 32, 1)
             }
             const float mn_a = fmaxf(m_a, mx_a);
             const float mn_b = fmaxf(m_b, mx_b);
+            const int e_low = min(e_top, min(ev[0], ev[1]));
             e_top = max(e_top, max(ev[0], ev[1]));
             const float alpha_a = exp2f(m_a - mn_a);
             const float alpha_b = exp2f(m_b - mn_b);
+            const float m_old_a = m_a, m_old_b = m_b;
             m_a = mn_a;
             m_b = mn_b;
             float sum_a = 0.f, sum_b = 0.f;
@@ -1536,16 +1539,20 @@ __global__ void __launch_bounds__(Ring<kE4m3, kCtaMerge>::kWarps * 32, 1)
                     }
                 }
             }
-            if (min(ev[0], ev[1]) < e_top - kFarExp) {
-                sum_a = sum_b = 0.f;
+            if (e_low < e_top - kFarExp) {
+                // and l itself in two steps, where the maximum jumps by V's exponent
+                const float h_a = exp2f(0.5f * (m_old_a - mn_a)), h_b = exp2f(0.5f * (m_old_b - mn_b));
+                l_a = l_a * h_a * h_a;
+                l_b = l_b * h_b * h_b;
 #pragma unroll
                 for (int hh = 0; hh < 2; ++hh) {
-                    sum_a += exp2f((sv[hh][0] - ef[hh]) - mn_a) + exp2f((sv[hh][2] - ef[hh]) - mn_a);
-                    sum_b += exp2f((sv[hh][1] - ef[hh]) - mn_b) + exp2f((sv[hh][3] - ef[hh]) - mn_b);
+                    l_a += exp2f((sv[hh][0] - ef[hh]) - mn_a) + exp2f((sv[hh][2] - ef[hh]) - mn_a);
+                    l_b += exp2f((sv[hh][1] - ef[hh]) - mn_b) + exp2f((sv[hh][3] - ef[hh]) - mn_b);
                 }
+            } else {
+                l_a = l_a * alpha_a + sum_a;
+                l_b = l_b * alpha_b + sum_b;
             }
-            l_a = l_a * alpha_a + sum_a;
-            l_b = l_b * alpha_b + sum_b;
             __syncwarp();
             if (lane == 0) {
                 fence_proxy_async_smem();

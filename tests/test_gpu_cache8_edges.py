@@ -105,3 +105,30 @@ def test_a_failed_call_does_not_fail_the_next(cache8):
     work.synchronize()
     want, _ = c.read(s, 0, 20, dtype=torch.float16)
     assert np.array_equal(k.cpu().numpy().view(np.float16), want)
+
+
+@pytest.mark.parametrize("low,high", [(0.0, 1e12), (0.0, 1e30), (1e-25, 1e20), (1e25, 0.0)])
+@pytest.mark.parametrize("G,lens", [(8, [700]), (1, [700]), (8, [650, 640, 300]), (8, [640] * 20), (8, [1900] * 30), (1, [31000])])
+def test_decode_where_v_jumps(cache8, low, high, G, lens):
+    """The first 256 rows' V far below, or above, that of the others, at like weights."""
+    rng = np.random.default_rng(123)
+    c = cache8(G=G, n_pages=4000, max_slots=32)
+    slots = []
+    for n in lens:
+        s = c.slot(n + 1)
+        v = rows(rng, n, G)
+        v[:256] *= np.float32(low)
+        v[256:] *= np.float32(high)
+        c.eng.rope_append_range(0, s, n, dev(rows(rng, n, G) * np.float32(0.3)), dev(v))
+        c.eng.advance([s], n)
+        slots.append(s)
+    n = len(slots)
+    q = rng.standard_normal((n, 4 * G, D)).astype(np.float32)
+    out = torch.empty((n, 4 * G * D), device=DEV)
+    c.eng.decode_step(0, slots, dev(q), dev(rows(rng, n, G)), dev(rows(rng, n, G) * np.float32(high)), out)
+    out = out.double().cpu().numpy().reshape(n, 4 * G, D)
+    for i in range(0, n, 6):
+        kk, vv = cached(c.eng, c.hkv, slots[i], lens[i] + 1, G)
+        want, bound = weighed(c.rope(q[i:i + 1], [lens[i]]).astype(np.float64), kk, vv, lens[i], "f32", 14)
+        over = np.abs(out[i:i + 1] - want) - bound
+        assert over.max() <= 0, (i, np.unravel_index(over.argmax(), over.shape), over.max())
