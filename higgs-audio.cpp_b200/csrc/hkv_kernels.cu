@@ -999,15 +999,16 @@ __global__ void __launch_bounds__(Ring<kE4m3, kCtaMerge>::kWarps * 32, 1)
         l_b += __shfl_xor_sync(0xffffffffu, l_b, 16);
         float unit = 1.f, own_a = 1.f, own_b = 1.f;
         if (kE4m3) {
-            // l brought to [2^-12, 2^-11) by a power of two that m takes up: a partial's
-            // weight is then that of its logits, and no merge of 2^11 of them overflows
+            // l and o brought to l in [1, 2) by a power of two that m takes up, which is then
+            // the size of a logit again; both times 2^-12, so that no merge of up to 2^11
+            // partials overflows
             auto exponent = [](float l) {
-                return min(max(static_cast<int>((__float_as_uint(l) >> 23) & 255u) - 127 + 12, -126), 126);
+                return min(max(static_cast<int>((__float_as_uint(l) >> 23) & 255u) - 127, -126), 114);
             };
             const int ea = exponent(l_a), eb = exponent(l_b);
             unit = pow2(e0 - kPShift);
-            own_a = pow2(-ea);
-            own_b = pow2(-eb);
+            own_a = pow2(-ea - 12);
+            own_b = pow2(-eb - 12);
             l_a *= own_a;
             l_b *= own_b;
             m_a += static_cast<float>(ea);

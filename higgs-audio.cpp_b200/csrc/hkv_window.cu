@@ -867,13 +867,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_after();
             const uint32_t odd = *reinterpret_cast<volatile uint32_t *>(&ctl->odd_v);
             // F16 cache: o and l carry 2^kShift, a part's o is not normalised.  8-bit cache:
-            // o carries it, and a part's o and l are brought to l in [1, 2) by a power of
-            // two that m takes up, so that o is of the size of V and its weight in the
-            // join that of its logits.
+            // o carries it, and a part's l and o are brought to l in [1, 2) by a power of two
+            // that m takes up, which is then the size of a logit again; both times 2^-12, so
+            // that no join of up to 2^11 parts overflows.
             float own = t.part < 0 ? 1.f / l : 1.f;
             if (kE4m3 && t.part >= 0) {
-                const int e = min(max(static_cast<int>((__float_as_uint(l) >> 23) & 255u) - 127 + 12, -126), 126);
-                own = pow2(-e);
+                const int e = min(max(static_cast<int>((__float_as_uint(l) >> 23) & 255u) - 127, -126), 114);
+                own = pow2(-e - 12);
                 l *= own;
                 m += static_cast<float>(e);
             }
