@@ -130,7 +130,7 @@ struct Control {
     // them, so what a tile writes must not lie over what the other may still read.
     union TileRows {
         int q_exp[kTile];             // of a row of q in E4M3 parts
-        float half[2][kTile];         // of a row's logits the largest, by each of its threads; l at the end
+        float half[2][kTile];         // of a block, the bound of a row by each of its threads; l at the end
     } rows[2];
 };
 static_assert(sizeof(Control) % 16 == 0, "the scales follow it");
@@ -143,8 +143,9 @@ struct Shape {
     static constexpr int kParts = kSplit || kCodeK ? 2 : 1;  // of q
     // F32: the products of half a block's weights start while the other half's are
     // formed (8100 tokens: 1033 us, 1086 without; on an F16 cache, which waits for its
-    // converters, 1265 and 1245); a 16-bit block's softmax is too short for that to pay for its second store and
-    // barrier (8 ragged windows: BF16 279 us, 283 with; 8100 tokens of F16 694 and 716).
+    // converters, 1265 and 1245); a 16-bit block's softmax is too short for that to pay for
+    // its second store and barrier (8 ragged windows: BF16 279 us, 283 with; 8100 tokens of
+    // F16 694 and 716).
     static constexpr bool kEarly = kSplit;
     static constexpr int kQPart = kCodeK ? kCodeTileBytes : kTileBytes;
     static constexpr int kKTile = kCodeK ? kCodeTileBytes : kTileBytes;
