@@ -36,7 +36,9 @@
  *     head h reads KV head h / (n_head / n_head_kv) (:441-456).
  *   * Slot operations are thread-safe (one mutex per engine).  Compute calls
  *     on one engine share its split-partial buffers: issue them on one stream
- *     (or order the streams) in the order the GPU should run them.
+ *     (or order the streams) in the order the GPU should run them.  A stream has
+ *     to live until the calls on the next one: plans are kept from call to call,
+ *     and a new one records on the last stream that read the old.
  */
 #ifndef HKV_H
 #define HKV_H
